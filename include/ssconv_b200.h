@@ -587,6 +587,28 @@ int ssc_gate_bwd(const float *x, const float *gy, int n, int c_total, int c_out,
                  const int32_t *gate_of_channel, const int32_t *field_start, const int32_t *field_len,
                  int scalar_act, int gate_act, float *gx, void *stream);
 
+/* Group norm of the rows of ragged samples with the gated activation behind it, and its gradients.  No counterpart in the
+ * reference (batch norm only, SS_Conv_lib/ss_conv/batchnorm.py:13-136).
+ * x [n, c] rows of `type` (SSC_PREC_FP32 / F16 / BF16), offsets int32 [batch + 1] on the device, ascending; rows outside them come out
+ * as zeros.  Channels are fields (copies of order l, 2l+1 channels each), n_scalar of them with l = 0; a group is a run of copies of one
+ * order.  The last n_gate channels are gates (scalars), one for each field of order l > 0 in order, and are not part of the result:
+ * out [n, c - n_gate].  table int32 on the device, one after the other: group_of_channel [c], field_of_channel [c],
+ * scalar_of_channel [c] (-1 for l > 0), gate_of_channel [c - n_gate] (-2 copy, -1 scalar activation, else the gate),
+ * field_first [n_field], field_len [n_field], field_scalar [n_field], gate_field [n_gate], group_first [n_group], group_len [n_group],
+ * group_copies [n_group].  weight [n_field] and bias [n_scalar] float32 or NULL.  Activations: 0 identity, 1 relu, 2 sigmoid,
+ * 3 silu, 4 gelu (erf).  out_type is `type`, or any for float32 rows.  stats [batch, n_group, 2] float32 receives mean (0 for l > 0) and
+ * (variance + eps)^-1/2 of every sample that has rows, which the backward call reads.  Sums are float32, in a fixed order.
+ * c is at most 512 channels, 1024 / 2048 / 4096 where c, c - n_gate and the addresses are multiples of 2 / 4 / 8 channels
+ * (8: 16-bit rows).  gx has the type of x; d_weight [n_field], d_bias [n_scalar] float32. */
+size_t ssc_group_norm_scratch_bytes(int n, int batch, int c, int n_group, int n_field, int n_scalar);
+int ssc_group_norm_fwd(const void *x, int type, int n, int c, const int32_t *offsets, int batch, const int32_t *table, int n_field,
+                       int n_scalar, int n_group, int n_gate, const float *weight, const float *bias, float eps, int scalar_act,
+                       int gate_act, void *out, int out_type, float *stats, void *scratch, size_t scratch_bytes, void *stream);
+int ssc_group_norm_bwd(const void *x, const void *gy, int type, int n, int c, const int32_t *offsets, int batch,
+                       const int32_t *table, int n_field, int n_scalar, int n_group, int n_gate, const float *weight,
+                       const float *bias, float eps, int scalar_act, int gate_act, const float *stats, void *gx, float *d_weight,
+                       float *d_bias, void *scratch, size_t scratch_bytes, void *stream);
+
 /* Measurement support, no counterpart in the reference: issues nothing but fp32 scatter-add
  * reductions (red.global.add.v4.f32) of 1.0 into out[rows[j], :] for steps * 32 * (warps of the grid)
  * list positions j, wrapping round the list of n_idx row numbers.  lanes_per_row (1, 2, 4, 8) =

@@ -9,6 +9,7 @@ from . import utils
 from . import convolution
 from . import activation
 from . import batchnorm
+from . import groupnorm
 from . import pool
 from . import dropout
 from . import parallel

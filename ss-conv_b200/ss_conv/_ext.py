@@ -10,6 +10,7 @@ variants of convolution and pools); only the functions the reference's own Pytho
 (indice_field_maxpool_*, voxelize_idx, point_recover_*) and the 2-D rulebooks raise NotImplementedError.
 """
 import ctypes
+import functools
 import os
 import threading
 
@@ -158,6 +159,11 @@ SIGNATURES = {
                            c_void_p, c_float, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "ssc_gate_bwd": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
                              c_void_p, c_void_p]),
+    "ssc_group_norm_scratch_bytes": (c_size_t, [c_int] * 6),
+    "ssc_group_norm_fwd": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
+                                   c_float, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "ssc_group_norm_bwd": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p,
+                                   c_void_p, c_float, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "ssc_scatter_add_rate": (c_int, [c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
 }
 
@@ -1695,6 +1701,54 @@ def gate_backward(x, gy, c_out, gate_of_channel, field_start, field_len, scalar_
                               _p(gate_of_channel, torch.int32), _p(field_start), _p(field_len), int(scalar_act),
                               int(gate_act), _p(gx), _stream()))
     return gx
+
+
+# ================================================================ group norm
+ROW_TYPES = {torch.float32: PREC_FP32, torch.float16: PREC_F16, torch.bfloat16: PREC_BF16}
+
+
+def _on_device_of(call):
+    """The call with its first argument's device as the current one: launches and streams are the current device's."""
+    @functools.wraps(call)
+    def there(t, *args):
+        if t.device.index == torch._C._cuda_getDevice():
+            return call(t, *args)
+        with torch.cuda.device(t.device):
+            return call(t, *args)
+    return there
+
+
+@_on_device_of
+def group_norm_forward(x, offsets, layout, weight, bias, eps, codes, out_dtype):
+    """(result [n, c_out], statistics [samples, groups, 2]); layout: the channel tables (groupnorm._Layout)."""
+    x, offsets = x.contiguous(), offsets.contiguous()
+    weight, bias = (p if p is None else p.detach().contiguous() for p in (weight, bias))
+    n, batch, dev = x.shape[0], offsets.shape[0] - 1, x.device
+    out = _empty((n, layout.c_out), out_dtype, dev)
+    stats = _empty((batch, layout.n_group, 2), torch.float32, dev)
+    nbytes = int(lib().ssc_group_norm_scratch_bytes(n, batch, layout.c, layout.n_group, 0, 0))
+    scratch = _empty(nbytes, torch.uint8, dev)
+    _check(lib().ssc_group_norm_fwd(_p(x), ROW_TYPES[x.dtype], n, layout.c, _p(offsets, torch.int32), batch, _p(layout.table(dev)), layout.n_field,
+                                    layout.n_scalar, layout.n_group, layout.n_gate, _p(weight, torch.float32), _p(bias, torch.float32), eps,
+                                    codes[0], codes[1], _p(out), ROW_TYPES[out_dtype], _p(stats), _p(scratch), nbytes, _stream()))
+    return out, stats
+
+
+@_on_device_of
+def group_norm_backward(x, gy, offsets, layout, weight, bias, eps, codes, stats):
+    """(gx, d_weight [fields], d_bias [scalars]) of group_norm_forward at x and the gradient gy of its result."""
+    x, gy, offsets = x.contiguous(), gy.contiguous(), offsets.contiguous()
+    weight, bias = (p if p is None else p.detach().contiguous() for p in (weight, bias))
+    n, batch, dev = x.shape[0], offsets.shape[0] - 1, x.device
+    gx = torch.empty_like(x)
+    grads = _empty(layout.n_field + max(layout.n_scalar, 1), torch.float32, dev)
+    nbytes = int(lib().ssc_group_norm_scratch_bytes(n, batch, layout.c, layout.n_group, layout.n_field, layout.n_scalar))
+    scratch = _empty(nbytes, torch.uint8, dev)
+    _check(lib().ssc_group_norm_bwd(_p(x), _p(gy, x.dtype), ROW_TYPES[x.dtype], n, layout.c, _p(offsets, torch.int32), batch, _p(layout.table(dev)),
+                                    layout.n_field, layout.n_scalar, layout.n_group, layout.n_gate, _p(weight, torch.float32),
+                                    _p(bias, torch.float32), eps, codes[0], codes[1], _p(stats), _p(gx), _p(grads), _p(grads[layout.n_field:]),
+                                    _p(scratch), nbytes, _stream()))
+    return gx, grads[:layout.n_field], grads[layout.n_field:layout.n_field + layout.n_scalar]
 
 
 def scatter_add_rate(out, rows, steps, lanes_per_row=8, warps_per_sm=16):

@@ -1,0 +1,200 @@
+"""Group normalisation of sparse rows with the gated activation behind it.
+
+The reference has batch norm only (SS_Conv_lib/ss_conv/batchnorm.py:13-136), whose statistics mix the samples of a batch;
+here every sample has its own, so a row's result does not depend on what else is in the batch, and training and
+inference compute the same.  Scalars are centred and scaled, fields of order l > 0 are scaled by the mean of
+their squared norm, which keeps the layer equivariant."""
+import functools
+import itertools
+
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
+
+from . import _ext
+from .activation import _act_code
+
+
+def act_code(fn):
+    """0 identity, 1 relu, 2 sigmoid, 3 silu, 4 gelu; ValueError for anything else."""
+    code = _act_code(fn)
+    if code is None and (fn is F.silu or isinstance(fn, nn.SiLU)):
+        code = 3
+    if code is None and (fn is F.gelu or (isinstance(fn, nn.GELU) and fn.approximate == "none")):
+        code = 4
+    if code is None:
+        raise ValueError("the activation must be None, relu, sigmoid, silu or gelu (got %r)" % (fn,))
+    return code
+
+
+class _Layout(object):
+    """Channel tables of rows Rs in `groups` groups for each entry; gated: the last entry's scalars are the gates of
+    the fields of order l > 0 (as SS_Conv lays them out)."""
+
+    def __init__(self, Rs, groups, gated, scalar_act):
+        fields = [l for m, l in Rs for _ in range(m)]
+        dims = [2 * l + 1 for l in fields]
+        first = list(itertools.accumulate(dims, initial=0))[:-1]
+        self.c, self.n_field, self.n_scalar = sum(dims), len(fields), fields.count(0)
+        self.n_gate = sum(1 for l in fields if l > 0) if gated else 0
+        if gated and (not Rs or Rs[-1][1] != 0 or Rs[-1][0] != self.n_gate):
+            raise ValueError("the last entry of Rs must hold one gate scalar for each of the %d fields of order l > 0 (got %s)"
+                             % (self.n_gate, Rs[-1:]))
+        self.c_out = self.c - self.n_gate
+        slots, slot = [], 0
+        for l in fields:
+            slots.append(slot if l == 0 else -1)
+            slot += l == 0
+        group_of_field, group_first, group_len, copies = [], [], [], []
+        f = 0
+        for m, l in Rs:
+            if m % groups:
+                raise ValueError("%d copies of order %d do not divide into %d groups" % (m, l, groups))
+            for g in range(groups if m else 0):
+                group_first.append(first[f])
+                group_len.append(m // groups * (2 * l + 1))
+                copies.append(m // groups)
+                group_of_field += [len(copies) - 1] * (m // groups)
+                f += m // groups
+        self.n_group = len(copies)
+        gates, gate_field = [], []
+        for i, l in enumerate(fields):
+            if gated and first[i] >= self.c_out:
+                break
+            if l == 0:
+                gates += [-1 if scalar_act else -2]
+            else:
+                gates += [len(gate_field) if gated else -2] * (2 * l + 1)
+                if gated:
+                    gate_field.append(i)
+        spread = lambda v: [x for x, d in zip(v, dims) for _ in range(d)]  # noqa: E731
+        self.rows = (spread(group_of_field) + spread(range(self.n_field)) + spread(slots) + gates + first + dims + slots
+                     + gate_field + group_first + group_len + copies)
+        self.tables = {}
+
+    def table(self, device):
+        kept = self.tables.get(device)
+        if kept is None:
+            kept = self.tables[device] = torch.tensor(self.rows, dtype=torch.int32).to(device)
+        return kept
+
+
+@functools.lru_cache(maxsize=256)
+def _layout(Rs, groups, gated, scalar_act):
+    if not Rs or groups < 1 or any(m < 0 or l < 0 for m, l in Rs) or sum(m for m, _ in Rs) == 0:
+        raise ValueError("Rs must be [(copies, order), ...] and the number of groups positive (got %s, %s)" % (list(Rs), groups))
+    return _Layout(Rs, groups, gated, scalar_act)
+
+
+class _GroupNormFn(torch.autograd.Function):
+    """Saves the rows and the statistics; everything between is computed again on the way back."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, offsets, layout, eps, codes):
+        y, stats = _ext.group_norm_forward(x, offsets, layout, weight, bias, eps, codes, x.dtype)
+        ctx.save_for_backward(x, weight, bias, offsets, stats)
+        ctx.layout, ctx.eps, ctx.codes = layout, eps, codes
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        x, weight, bias, offsets, stats = ctx.saved_tensors
+        gx, gw, gb = _ext.group_norm_backward(x, gy, offsets, ctx.layout, weight, bias, ctx.eps, ctx.codes, stats)
+        need = ctx.needs_input_grad
+        return gx, gw if need[1] else None, gb if need[2] else None, None, None, None, None
+
+
+def _normed(x, offsets, layout, weight, bias, eps, codes, out_dtype=None):
+    if not x.is_cuda:
+        raise RuntimeError("ssconv_b200 runs on CUDA tensors only (got a %s tensor)" % x.device.type)
+    if x.dim() != 2 or x.shape[1] != layout.c:
+        raise ValueError("features must be [n, %d] (got %s)" % (layout.c, tuple(x.shape)))
+    if x.dtype not in _ext.ROW_TYPES:
+        raise TypeError("features must be float32, float16 or bfloat16 (got %s)" % x.dtype)
+    if offsets.dim() != 1 or offsets.shape[0] < 2 or offsets.dtype != torch.int32 or offsets.device != x.device:
+        raise ValueError("offsets must be int32 [samples + 1] on %s (got %s %s on %s)" % (x.device, offsets.dtype, tuple(offsets.shape),
+                                                                                      offsets.device))
+    for name, p, size in (("weight", weight, layout.n_field), ("bias", bias, layout.n_scalar)):
+        if p is not None and (p.shape != (size,) or p.device != x.device or not p.is_floating_point()):
+            raise ValueError("%s must hold %d floating point values on %s (got %s %s on %s)" % (name, size, x.device, p.dtype,
+                                                                                            tuple(p.shape), p.device))
+    weight, bias = (p if p is None or p.dtype == torch.float32 else p.float() for p in (weight, bias))
+    if torch.is_grad_enabled() and (x.requires_grad or any(p is not None and p.requires_grad for p in (weight, bias))):
+        y = _GroupNormFn.apply(x, weight, bias, offsets, layout, eps, codes)
+        return y if out_dtype in (None, x.dtype) else y.to(out_dtype)
+    return _ext.group_norm_forward(x, offsets, layout, weight, bias, eps, codes, out_dtype or x.dtype)[0]
+
+
+def group_norm(features, offsets, Rs, num_groups=1, weight=None, bias=None, eps=1e-5, activation=None):
+    """act(norm(features)): features [N, C] float32 / float16 / bfloat16 of fields Rs = [(copies, order), ...], the samples one
+    behind the other, offsets [samples + 1] int32 on the device (ascending; samples may be empty).
+
+    The copies of every entry of Rs are split into num_groups groups, normalised over the rows of a sample and the copies of
+    the group.  weight [fields] and bias [scalars] as in BatchNorm.  activation: one callable, or (scalar, gate) as in
+    Activation; with a gate and fields of order l > 0 the last entry of Rs holds one gate scalar for each of them, and
+    the result has the channels before it.  relu, sigmoid, silu, gelu or None.  Statistics and parameters are float32, the
+    result has the type of the rows; rows of no sample (outside the offsets) come out as zeros."""
+    scalar, gate = activation if isinstance(activation, tuple) else (activation, activation)
+    Rs = tuple((int(m), int(l)) for m, l in Rs)
+    gated = gate is not None and any(l > 0 and m > 0 for m, l in Rs)
+    codes = (act_code(scalar), act_code(gate) if gated else 0)
+    if not eps > 0:
+        raise ValueError("eps must be positive (got %r)" % (eps,))
+    return _normed(features, offsets, _layout(Rs, int(num_groups), gated, codes[0] != 0), weight, bias, float(eps), codes)
+
+
+class GroupNorm(nn.Module):
+    """group_norm of a SparseTensor's rows, each sample by itself (`weight` [fields], `bias` [scalars]); takes BatchNorm's place
+    in SS_Conv(norm_groups=...)."""
+
+    def __init__(self, Rs, num_groups=1, eps=1e-5, affine=True, activation=None):
+        super().__init__()
+        self.Rs, self.num_groups, self.eps, self.affine, self.activation = [(int(m), int(l)) for m, l in Rs], int(num_groups), eps, affine, activation
+        scalar, gate = activation if isinstance(activation, tuple) else (activation, activation)
+        gated = gate is not None and any(l > 0 and m > 0 for m, l in self.Rs)
+        act_code(scalar), act_code(gate) if gated else None
+        layout = _layout(tuple(self.Rs), self.num_groups, gated, scalar is not None)
+        if affine:
+            self.weight = nn.Parameter(torch.ones(layout.n_field))
+            self.bias = nn.Parameter(torch.zeros(layout.n_scalar))
+        else:
+            self.register_parameter('weight', None)
+            self.register_parameter('bias', None)
+
+    def __repr__(self):
+        return "{} (Rs={}, num_groups={}, eps={})".format(self.__class__.__name__, self.Rs, self.num_groups, self.eps)
+
+    def _apply_to(self, input, rows):
+        """input with `rows`(features, offsets) in place of its features."""
+        if torch.is_grad_enabled() and (input.raw()[0].requires_grad or any(p.requires_grad for p in self.parameters())):
+            input.features = rows(input.features, input.get_offsets())
+            return input
+        # (nothing to record: a pending row count stays on the device)
+        input.features = rows(input.raw()[0], input.get_offsets())
+        if input.pending():
+            input._rows.post.append(lambda f: rows(f, input.get_offsets()))
+        return input
+
+    def norm_and_gate(self, input, act):
+        """act(self(input)) in one operator where the activation is the library's (an Activation that fuses, without biases), else None."""
+        if self.activation is not None or not (input.raw()[0].is_cuda and act.fusable_gate()):
+            return None
+        gated = act.gate_act is not None
+        layout = _layout(tuple(self.Rs), self.num_groups, gated, act.scalar_act is not None)
+        if act.c_in() != layout.c or act.c_out() != layout.c_out:
+            return None
+        codes = act._codes()
+
+        def rows(f, offsets):
+            out = f.dtype
+            if out == torch.float32 and not torch.is_grad_enabled():
+                out = _ext._stored_type(f.shape[0], layout.c, layout.c_out, layout.c_out, _ext.get_feature_storage()) or out
+            return _normed(f, offsets, layout, self.weight, self.bias, float(self.eps), codes, out)
+
+        return self._apply_to(input, rows)
+
+    def forward(self, input):
+        return self._apply_to(input, lambda f, offsets: group_norm(f, offsets, self.Rs, self.num_groups, self.weight, self.bias, self.eps,
+                                                                   self.activation))

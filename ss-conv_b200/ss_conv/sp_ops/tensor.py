@@ -229,10 +229,10 @@ class SparseTensor(object):
                 self._cut = n
             return False
         with torch.set_grad_enabled(r.grad):
-            feats, inds = r.redo()
+            feats, self._indices = r.redo()   # (what works sample by sample looks at the new rows' indices)
             for fn in r.post:
                 feats = fn(feats)
-        self._features, self._indices = feats, inds
+        self._features = feats
         self._recomputed = True
         return True
 

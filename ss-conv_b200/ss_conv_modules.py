@@ -15,6 +15,7 @@ from ss_conv.activation import Activation
 from ss_conv.batchnorm import BatchNorm
 from ss_conv.convolution import Convolution
 from ss_conv.dropout import Dropout
+from ss_conv.groupnorm import GroupNorm
 from ss_conv.sp_ops.tensor import SparseTensor
 from ss_conv.sp_ops.voxelize import Point2Voxel, Voxel2Point
 from ss_conv.utils import SO3
@@ -33,12 +34,13 @@ def _unwatched(module, kind):
 class SS_Conv(nn.Module):
     """irrep_in / irrep_out: multiplicities per order, e.g. (4, 4, 4, 4).  With a gate activation
     the convolution produces one extra scalar per non-scalar output field
-    (Common_utils/ss_conv_modules.py:26-117)."""
+    (Common_utils/ss_conv_modules.py:26-117).  norm_groups: group norm with so many groups for each order in
+    the place of the batch norm (same parameters, no running statistics)."""
 
     def __init__(self, irrep_in, irrep_out, kernel_size, dropout_p=None, radial_window=radial_window, dyn_iso=False,
                  verbose=False, stride=1, padding=0, dilation=1, groups=1, bias=False, subm=False, output_padding=0,
                  transposed=False, inverse=False, use_bn=True, bn_momentum=0.01, bn_affine=True, activation=(None, None),
-                 activation_bias=False, activation_checkpoint=True, indice_key=None):
+                 activation_bias=False, activation_checkpoint=True, indice_key=None, norm_groups=None):
         super().__init__()
         Rs_in = [(m, l) for l, m in enumerate(irrep_in)]
         Rs_out = [(m, l) for l, m in enumerate(irrep_out)]
@@ -51,7 +53,10 @@ class SS_Conv(nn.Module):
                                 dyn_iso=dyn_iso, verbose=verbose, stride=stride, padding=padding, dilation=dilation,
                                 groups=groups, bias=bias, subm=subm, output_padding=output_padding, transposed=transposed,
                                 inverse=inverse, indice_key=indice_key)
-        self.bn = BatchNorm(Rs_gated, momentum=bn_momentum, affine=bn_affine) if use_bn else None
+        if use_bn and norm_groups is not None:
+            self.bn = GroupNorm(Rs_gated, norm_groups, affine=bn_affine)
+        else:
+            self.bn = BatchNorm(Rs_gated, momentum=bn_momentum, affine=bn_affine) if use_bn else None
         if scalar_act is not None or gate_act is not None:
             self.activation = Activation(Rs_out, activation, bias=activation_bias, checkpoint=activation_checkpoint)
         else:
@@ -83,7 +88,8 @@ class SS_Conv(nn.Module):
             return x if self.dropout is None else self.dropout(x)
         x = self.conv(x)
         both = None
-        if _unwatched(self.bn, BatchNorm) and _unwatched(self.activation, Activation) and not _has_any_global_hook():
+        if ((_unwatched(self.bn, BatchNorm) or _unwatched(self.bn, GroupNorm)) and _unwatched(self.activation, Activation)
+                and not _has_any_global_hook()):
             both = self.bn.norm_and_gate(x, self.activation)
         if both is not None:
             x = both
