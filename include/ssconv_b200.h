@@ -609,6 +609,26 @@ int ssc_group_norm_bwd(const void *x, const void *gy, int type, int n, int c, co
                        const float *bias, float eps, int scalar_act, int gate_act, const float *stats, void *gx, float *d_weight,
                        float *d_bias, void *scratch, size_t scratch_bytes, void *stream);
 
+/* Gated feed-forward of rows: out = (act(x Wg' + bg) * (x Wu' + bu)) Wo' + bo (+ residual), and its gradients.  No counterpart in
+ * the reference, whose networks end in plain linear layers (LineMOD/model.py).
+ * x [n, c], w_in [2, hidden, c] (gate, up), w_out [c_out, hidden], b_in [2, hidden], b_out [c_out], residual and out [n, c_out], all of
+ * `type` (SSC_PREC_FP32 / F16 / BF16); the biases and the residual may be NULL.  act: 0 identity, 1 relu, 2 sigmoid, 3 silu,
+ * 4 gelu (erf).  Products are added in float32; float32 operands are used to 24 bits; in 16 bits the hidden rows h = act(.) * (.), and
+ * in the backward call their gradients, are rounded to the rows' type (up to 16 rows forward: not rounded).  A value that is not
+ * finite makes what depends on it infinite or NaN.  Sizes are at most 65536; any address and width is accepted, 16-bit widths that are
+ * multiples of 8 at addresses that are multiples of 16 are read in place, others are copied to scratch first.
+ * scratch: ssc_gated_ff_scratch_bytes(...) bytes, 16-byte aligned; rows are taken in turns so that it stays below about
+ * a gigabyte beside the weights.  Sums have a fixed order.
+ * ssc_gated_ff_bwd: gy [n, c_out]; gx, gw_in, gw_out, gb_in, gb_out of the shapes above, each may be NULL (the residual's
+ * gradient is gy).  status: as in ssc_conv_fwd. */
+size_t ssc_gated_ff_scratch_bytes(int type, int n, int c, int hidden, int c_out, int backward);
+int ssc_gated_ff_fwd(const void *x, int type, int n, int c, int hidden, int c_out, const void *w_in, const void *w_out,
+                     const void *b_in, const void *b_out, const void *residual, int act, void *out, int32_t *status,
+                     void *scratch, size_t scratch_bytes, void *stream);
+int ssc_gated_ff_bwd(const void *x, const void *gy, int type, int n, int c, int hidden, int c_out, const void *w_in,
+                     const void *w_out, const void *b_in, int act, void *gx, void *gw_in, void *gw_out, void *gb_in, void *gb_out,
+                     int32_t *status, void *scratch, size_t scratch_bytes, void *stream);
+
 /* Measurement support, no counterpart in the reference: issues nothing but fp32 scatter-add
  * reductions (red.global.add.v4.f32) of 1.0 into out[rows[j], :] for steps * 32 * (warps of the grid)
  * list positions j, wrapping round the list of n_idx row numbers.  lanes_per_row (1, 2, 4, 8) =

@@ -1,0 +1,973 @@
+// Gated feed-forward of rows: y = (act(x Wg' + bg) * (x Wu' + bu)) Wo' + bo (+ residual), and its gradients.
+//
+// Forward: one product for gate and up, whose epilogue applies the activation and multiplies (h leaves the SM once, in
+// the rows' type), one product for the way out.  Backward: gate and up are computed again together with dh = dy Wo, and the epilogue
+// turns the three into h, dg = dh u act'(g) and du = dh act(g) (keeping g and u would cost more memory traffic than their products
+// cost time up to 700 channels, and two roundings); then dx = dg Wg + du Wu, dWin = [dg, du]' x and dWo = dy' h, whose long sums
+// are split over the rows and added in a fixed order.
+//
+// All of them are one kernel: tiles of 128 rows in tensor memory, operands by TMA, a warp that issues the products and eight
+// that empty the accumulators, two of which are in turn.  Operands are 16-bit; float32 rows are the sum of
+// three bfloat16 planes (24 bits), and a product the sum of the six products of planes that reach 2^-24, the small ones first.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "ssc_common.cuh"
+#include "ssc_rows_act.cuh"
+#include "ssc_tc_ptx.cuh"
+
+namespace ssc {
+namespace {
+
+constexpr int kBox = 64;                      // TMA boxes: 64 x 64 elements, 128-byte rows
+constexpr uint32_t kBoxBytes = kBox * kBox * 2;
+constexpr int kTileM = 128;
+constexpr int kStageBoxes = 6;                // two of A, up to four of B
+constexpr uint32_t kStageBytes = kStageBoxes * kBoxBytes;
+constexpr int kStages = 4;
+constexpr int kThreads = 384;                 // TMA, products, tensor memory, one idle warp, eight for the accumulators
+constexpr uint32_t kSmemBytes = kStages * kStageBytes + 1024;
+
+enum Epilogue { kGate, kBack, kRows, kPart };
+enum Half { kNone, kByK, kByBox, kByM };      // what chooses between the two matrices of an operand (gate and up)
+
+struct Segment {
+  int a_mn, b_mn;            // 1: stored with the rows of the product (not the summed index) contiguous
+  int a_half, b_half;
+  int a_planes, b_planes;    // matrices of one plane: 1 or 2
+  int blocks;                // of 64 along the summed index
+  int half_blocks;           // kByK: blocks of the first matrix
+  int boxes_b;
+  int col;                   // accumulator column
+};
+struct FfMaps {
+  CUtensorMap a[2], b[2];
+};
+struct FfParams {
+  Segment seg[2];
+  int n_seg, pairs, f16;
+  int tiles_m, tiles_n, splits, m_half;        // tiles; m_half: tiles of the first matrix (kByM)
+  int step_n;                                  // columns of the result to a tile
+  int rows, cols;                              // of the result (one matrix)
+  int act;
+  const void *bias;                            // of the result's columns; kGate / kBack: [2][hidden]
+  const void *residual;
+  void *out, *out2;                            // kGate: h; kBack: h, dg|du; kRows: result; kPart: float [splits][rows of all][cols]
+  int pitch;                                   // of out
+  size_t plane, plane2;                        // elements from one plane to the next (of out, of a matrix of out2)
+  int vec;                                     // rows of out (and residual) are aligned to 16 bytes
+  int accumulate;                              // kPart: add to what is there
+  int32_t *status, *alarm;
+};
+
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map),
+               "r"(x), "r"(y), "r"(z), "r"(bar)
+               : "memory");
+}
+
+// Operands of a stage: rows of 128 bytes, 128-byte swizzle.  Summed index contiguous: groups of eight rows 1024 bytes
+// apart, 32 bytes a step of 16.  Rows contiguous: blocks of 64 rows a box apart, eight steps of the summed index 1024 bytes.
+__device__ __forceinline__ uint32_t operand_lo(uint32_t addr, int mn) { return ((addr >> 4) & 0x3FFFu) | (mn ? (kBoxBytes >> 4) << 16 : 1u << 16); }
+
+__constant__ const int8_t kPlaneA[6] = {2, 0, 1, 1, 0, 0}, kPlaneB[6] = {0, 2, 1, 0, 1, 0};
+
+template <class T>
+__device__ __forceinline__ void put16(T *p, const float *v, int left, int vec) {
+  if (vec && left >= 16) {
+    constexpr int N = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 16; i += N) {
+      struct alignas(16) { T v[N]; } k;
+#pragma unroll
+      for (int q = 0; q < N; ++q) k.v[q] = (T)v[i + q];
+      *(int4 *)(p + i) = *(const int4 *)&k;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (i < left) p[i] = (T)v[i];
+  }
+}
+template <class T>
+__device__ __forceinline__ void add16(float *v, const T *p, int left, int vec) {
+  if (vec && left >= 16) {
+    constexpr int N = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 16; i += N) {
+      struct alignas(16) { T v[N]; } k;
+      *(int4 *)&k = *(const int4 *)(p + i);
+#pragma unroll
+      for (int q = 0; q < N; ++q) v[i + q] += (float)k.v[q];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (i < left) v[i] += (float)p[i];
+  }
+}
+// v as three bfloat16 planes; what is not finite is in the first one alone.
+__device__ __forceinline__ void planes_of(float v, float &a, float &b, float &c) {
+  a = __bfloat162float(__float2bfloat16_rn(v));
+  const float r = v - a;
+  b = fabsf(a) < INFINITY ? __bfloat162float(__float2bfloat16_rn(r)) : 0.f;
+  c = fabsf(a) < INFINITY ? r - b : 0.f;
+}
+// 16 columns of an intermediate: rows of T, or the planes of float32 ones.  (pitch and buffers are aligned)
+template <class T>
+__device__ __forceinline__ void put_hidden(void *base, size_t at, size_t plane, const float *v, int left) {
+  if (sizeof(T) == 2) {
+    put16<T>((T *)base + at, v, left, 1);
+  } else {
+    float a[16], b[16], c[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) planes_of(v[i], a[i], b[i], c[i]);
+    __nv_bfloat16 *p = (__nv_bfloat16 *)base + at;
+    put16<__nv_bfloat16>(p, a, left, 1);
+    put16<__nv_bfloat16>(p + plane, b, left, 1);
+    put16<__nv_bfloat16>(p + 2 * plane, c, left, 1);
+  }
+}
+__device__ __forceinline__ void tmem_floats(float *v, uint32_t addr) { tmem_ld16((uint32_t *)v, addr); }
+__device__ __forceinline__ void tmem_arrived() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// Activations of results that are rounded to 16 bits: two steps of 2^-22 or so do not show.
+template <bool EXACT>
+__device__ __forceinline__ float gate_value(float z, int kind) {
+  if (!EXACT && kind == 3) return __fdividef(z, 1.0f + __expf(-z));
+  return act_value(z, kind);
+}
+template <bool EXACT>
+__device__ __forceinline__ void gate_both(float z, int kind, float &value, float &slope) {
+  if (!EXACT && kind == 3) {
+    const float s = __fdividef(1.0f, 1.0f + __expf(-z));
+    value = z * s;
+    slope = s * fmaf(z, 1.f - s, 1.f);
+    return;
+  }
+  value = act_value(z, kind);
+  slope = act_slope(z, kind);
+}
+
+struct Tile {
+  int m, n, split;      // tile numbers
+};
+__device__ __forceinline__ Tile tile_of(const FfParams &p, int t) {
+  Tile k;
+  k.n = t % p.tiles_n;
+  t /= p.tiles_n;
+  k.m = t % p.tiles_m;
+  k.split = t / p.tiles_m;
+  return k;
+}
+__device__ __forceinline__ int split_begin(int blocks, int split, int splits) { return (int)((long long)blocks * split / splits); }
+
+// The steps of a tile's sum: `blocks` of 64 for each pair of planes.  Tensor memory's additions cut off instead of rounding, which
+// adds up (1.5e-6 of gx over 1024 terms): float32 results leave tensor memory after every kLeave blocks of the last
+// pair, the largest one, and are added up in registers.  16-bit results stay.
+constexpr int kLeave = 4;
+__device__ __forceinline__ int part_count(int blocks, int pairs) { return pairs == 1 || blocks <= kLeave ? 1 : (blocks + kLeave - 1) / kLeave; }
+__device__ __forceinline__ int part_begin(int blocks, int pairs, int part) {
+  return part == 0 ? 0 : min((pairs - 1) * blocks + part * (pairs == 1 ? blocks : kLeave), pairs * blocks);
+}
+
+__device__ __forceinline__ int parts_of(const FfParams &p, const Tile &k) {
+  int most = 1;
+  for (int g = 0; g < p.n_seg; ++g)
+    most = max(most, part_count(split_begin(p.seg[g].blocks, k.split + 1, p.splits) - split_begin(p.seg[g].blocks, k.split, p.splits), p.pairs));
+  return most;
+}
+
+// 16 columns from column n on of a row of the result: v (kGate: gate, u: up; kBack: d = dh too).
+template <int EPI, class T>
+__device__ __forceinline__ void finish(const FfParams &p, int split, int half_m, int row, int n, float *v, float *u, float *d) {
+  const int left = p.cols - n;
+  if (EPI == kGate || EPI == kBack) {
+    if (p.bias) {
+      add16<T>(v, (const T *)p.bias + n, left, 0);
+      add16<T>(u, (const T *)p.bias + p.cols + n, left, 0);
+    }
+  }
+  if (EPI == kGate) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = gate_value<sizeof(T) == 4>(v[i], p.act) * u[i];
+    if (row < p.rows) put_hidden<T>(p.out, (size_t)row * p.pitch + n, p.plane, v, left);
+  } else if (EPI == kBack) {
+    float h[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float a, s;
+      gate_both<sizeof(T) == 4>(v[i], p.act, a, s);
+      h[i] = a * u[i];
+      v[i] = d[i] * u[i] * s;
+      u[i] = d[i] * a;
+    }
+    if (row < p.rows) {
+      const size_t at = (size_t)row * p.pitch + n;
+      put_hidden<T>(p.out, at, p.plane, h, left);
+      put_hidden<T>(p.out2, at, 2 * p.plane2, v, left);
+      put_hidden<T>(p.out2, p.plane2 + at, 2 * p.plane2, u, left);
+    }
+  } else if (EPI == kRows) {
+    if (p.bias) add16<T>(v, (const T *)p.bias + n, left, 0);
+    if (row < p.rows) {
+      const size_t at = (size_t)row * p.pitch + n;
+      if (p.residual) add16<T>(v, (const T *)p.residual + at, left, p.vec);
+      put16<T>((T *)p.out + at, v, left, p.vec);
+    }
+  } else if (row < p.rows) {
+    float *o = (float *)p.out + (size_t)split * p.plane + ((size_t)half_m * p.rows + row) * p.pitch + n;
+    if (p.accumulate) add16<float>(v, o, left, p.vec);
+    put16<float>(o, v, left, p.vec);
+  }
+}
+
+template <int EPI, class T>
+__global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_constant__ FfMaps maps, const FfParams p) {
+  after_previous();
+  extern __shared__ uint8_t raw[];
+  __shared__ alignas(8) uint64_t bars[2 * kStages + 5];
+  __shared__ uint32_t tmem_base;
+  __shared__ volatile int abort_flag;
+  const uint32_t ring = (smem_u32(raw) + 1023u) & ~1023u;
+  const uint32_t full = smem_u32(bars), empty = full + 8 * kStages, acc_full = empty + 8 * kStages, acc_empty = acc_full + 16, done = acc_empty + 16;
+  const int warp = warp_id(), tiles = p.tiles_m * p.tiles_n * p.splits;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full + 8 * s, 1);
+      mbar_init(empty + 8 * s, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(acc_full + 8 * b, 1);
+      mbar_init(acc_empty + 8 * b, 8);
+    }
+    mbar_init(done, 1);
+    abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_base)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base;
+
+  if (warp == 0) {
+    // operands
+    const bool one = elect_one();
+    uint32_t step = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      const Tile k = tile_of(p, t);
+      const int half_m = k.m >= p.m_half ? 1 : 0, m0 = (k.m - half_m * p.m_half) * kTileM, n0 = k.n * p.step_n;
+      const int parts = parts_of(p, k);
+      for (int part = 0; part < parts && ok; ++part)
+        for (int g = 0; g < p.n_seg && ok; ++g) {
+          const Segment &s = p.seg[g];
+          const int kb0 = split_begin(s.blocks, k.split, p.splits), blocks = split_begin(s.blocks, k.split + 1, p.splits) - kb0;
+          if (part >= part_count(blocks, p.pairs)) continue;
+          const uint32_t bytes = (2 + s.boxes_b) * kBoxBytes;
+          const int per = s.b_half == kByBox ? s.boxes_b / 2 : s.boxes_b, end = part_begin(blocks, p.pairs, part + 1);
+          int i = part_begin(blocks, p.pairs, part), pair = blocks > 0 ? i / blocks : 0, kb = kb0 + i - pair * blocks;
+          for (; i < end; ++i, ++step) {
+            const uint32_t slot = step % kStages, turn = step / kStages;
+            ok = mbar_wait_uniform(empty + 8 * slot, (turn & 1) ^ 1, &abort_flag);
+            if (!ok) break;
+            if (one) {
+              const int pa = p.pairs == 1 ? 0 : kPlaneA[pair], pb = p.pairs == 1 ? 0 : kPlaneB[pair];
+              const uint32_t at = ring + slot * kStageBytes, bar = full + 8 * slot;
+              mbar_expect_tx(bar, bytes);
+              const int by_k = kb >= s.half_blocks ? 1 : 0, kk = (kb - by_k * s.half_blocks) * kBox;
+              const int za = pa * s.a_planes + (s.a_half == kByK ? by_k : s.a_half == kByM ? half_m : 0);
+              for (int j = 0; j < 2; ++j) {
+                const int m = m0 + j * kBox;
+                tma_box(at + j * kBoxBytes, &maps.a[g], s.a_mn ? m : kk, s.a_mn ? kk : m, za, bar);
+              }
+              for (int j = 0; j < s.boxes_b; ++j) {
+                const int h = j / per, n = n0 + (j - h * per) * kBox, zb = pb * s.b_planes + (s.b_half == kByK ? by_k : h);
+                tma_box(at + (2 + j) * kBoxBytes, &maps.b[g], s.b_mn ? n : kk, s.b_mn ? kk : n, zb, bar);
+              }
+            }
+            if (++kb == kb0 + blocks) kb = kb0, ++pair;
+          }
+        }
+    }
+    if (!ok)      // copies in flight arrive before the block leaves
+      for (uint32_t s = step > kStages ? step - kStages : 0; s < step; ++s) mbar_wait_drain(full + 8 * (s % kStages), (s / kStages) & 1);
+  } else if (warp == 1) {
+    // products
+    const bool one = elect_one();
+    uint32_t step = 0, turn = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      const Tile k = tile_of(p, t);
+      const int parts = parts_of(p, k);
+      for (int part = 0; part < parts && ok; ++part, ++turn) {
+        const uint32_t buf = turn & 1;
+        ok = mbar_wait_uniform(acc_empty + 8 * buf, ((turn >> 1) & 1) ^ 1, &abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        for (int g = 0; g < p.n_seg && ok; ++g) {
+          const Segment &s = p.seg[g];
+          const int blocks = split_begin(s.blocks, k.split + 1, p.splits) - split_begin(s.blocks, k.split, p.splits);
+          if (part >= part_count(blocks, p.pairs)) continue;
+          const int steps = part_begin(blocks, p.pairs, part + 1) - part_begin(blocks, p.pairs, part);
+          const uint32_t type = p.f16 ? 0u : 1u;
+          const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)s.a_mn << 15) | ((uint32_t)s.b_mn << 16) |
+                                 ((uint32_t)(s.boxes_b * kBox >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24);
+          const uint32_t d = tmem + buf * 256 + s.col, ua = s.a_mn ? 128 : 2, ub = s.b_mn ? 128 : 2;
+          for (int i = 0; i < steps; ++i, ++step) {
+            const uint32_t slot = step % kStages;
+            ok = mbar_wait_uniform(full + 8 * slot, (step / kStages) & 1, &abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t at = ring + slot * kStageBytes;
+            const uint32_t a = operand_lo(at, s.a_mn), b = operand_lo(at + 2 * kBoxBytes, s.b_mn);
+            if (one) {
+#pragma unroll
+              for (uint32_t q = 0; q < 4; ++q) mma_f16_ss(d, a + q * ua, b + q * ub, idesc, i > 0 || q > 0 ? 1u : 0u);
+              mma_commit(empty + 8 * slot);
+            }
+            __syncwarp();
+          }
+        }
+        if (ok && one) mma_commit(acc_full + 8 * buf);
+        __syncwarp();
+      }
+    }
+  } else if (warp >= 4) {
+    // accumulators: a thread has a row and half of a tile's columns, kGroups times 16 of them from kSets products
+    constexpr int kSets = EPI == kGate ? 2 : EPI == kBack ? 3 : 1, kGroups = EPI == kGate ? 4 : EPI == kBack ? 2 : 8;
+    const int quad = warp & 3, side = (warp - 4) >> 2, lane = threadIdx.x & 31;
+    const uint32_t lanes = (uint32_t)(32 * quad) << 16;
+    uint32_t turn = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      const Tile k = tile_of(p, t);
+      const int half_m = k.m >= p.m_half ? 1 : 0, m0 = (k.m - half_m * p.m_half) * kTileM, n0 = k.n * p.step_n;
+      const int row = m0 + 32 * quad + lane, each = p.step_n / 2;
+      if constexpr (sizeof(T) == 4) {
+        float sum[kSets][kGroups][16];
+#pragma unroll
+        for (int s = 0; s < kSets; ++s)
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum[s][g][i] = 0.f;
+        const int parts = parts_of(p, k);
+        for (int part = 0; part < parts && ok; ++part, ++turn) {
+          const uint32_t buf = turn & 1, acc = tmem + buf * 256 + lanes;
+          ok = mbar_wait_uniform(acc_full + 8 * buf, (turn >> 1) & 1, &abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int s = 0; s < kSets; ++s) {
+            const Segment &from = p.seg[EPI == kBack && s == 2 ? 1 : 0];
+            const int blocks = split_begin(from.blocks, k.split + 1, p.splits) - split_begin(from.blocks, k.split, p.splits);
+            if (blocks == 0 || part >= part_count(blocks, p.pairs)) continue;
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g)
+              if (16 * g < each) {
+                float v[16];
+                tmem_floats(v, acc + s * p.step_n + side * each + 16 * g);
+                tmem_arrived();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sum[s][g][i] += v[i];
+              }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(acc_empty + 8 * buf);
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          const int n = n0 + side * each + 16 * g;
+          if (16 * g < each && n < p.cols)
+            finish<EPI, T>(p, k.split, half_m, row, n, sum[0][g], sum[kSets > 1 ? 1 : 0][g], sum[kSets > 2 ? 2 : 0][g]);
+        }
+      } else {
+        const uint32_t buf = turn & 1, acc = tmem + buf * 256 + lanes;
+        ok = mbar_wait_uniform(acc_full + 8 * buf, (turn >> 1) & 1, &abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const bool none = split_begin(p.seg[0].blocks, k.split, p.splits) == split_begin(p.seg[0].blocks, k.split + 1, p.splits);
+        for (int c = side * each; c < (side + 1) * each; c += 16) {
+          const int n = n0 + c;
+          if (n >= p.cols) break;
+          float v[kSets][16];
+#pragma unroll
+          for (int s = 0; s < kSets; ++s) tmem_floats(v[s], acc + s * p.step_n + c);
+          tmem_arrived();
+          if (EPI == kPart && none) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[0][i] = 0.f;      // (an empty share)
+          }
+          finish<EPI, T>(p, k.split, half_m, row, n, v[0], v[kSets > 1 ? 1 : 0], v[kSets > 2 ? 2 : 0]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(acc_empty + 8 * buf);
+        ++turn;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (abort_flag) {
+    if (warp == 1) {      // products that are still running end before tensor memory is given back
+      if (elect_one()) mma_commit(done);
+      __syncwarp();
+      mbar_wait_drain(done, 0);
+    }
+    if (threadIdx.x == 0) report_expired(p.status, p.alarm);
+    __syncthreads();
+  }
+  if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+// Rows [rows][cols] of float32 as three bfloat16 planes, or 16-bit rows that TMA cannot read as they are (a width or an address
+// that is no multiple of 16 bytes), to rows of `pitch` elements.
+template <class T>
+__global__ void __launch_bounds__(256) ff_planes_kernel(const T *__restrict__ src, long long rows, int cols, int pitch, void *dst) {
+  after_previous();
+  const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int per = pitch / 8;
+  const long long row = t / per;
+  if (row >= rows) return;
+  const int c0 = (int)(t - row * per) * 8;
+  T v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = c0 + i < cols ? src[row * cols + c0 + i] : (T)0.f;
+  if (sizeof(T) == 2) {
+    struct alignas(16) { T v[8]; } k;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) k.v[i] = v[i];
+    *(int4 *)((T *)dst + row * pitch + c0) = *(const int4 *)&k;
+  } else {
+    struct alignas(16) { __nv_bfloat16 v[8]; } a, b, c;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float x, y, z;
+      planes_of((float)v[i], x, y, z);
+      a.v[i] = __float2bfloat16_rn(x);
+      b.v[i] = __float2bfloat16_rn(y);
+      c.v[i] = __float2bfloat16_rn(z);
+    }
+    const size_t plane = (size_t)rows * pitch;
+    __nv_bfloat16 *p = (__nv_bfloat16 *)dst + row * pitch + c0;
+    *(int4 *)p = *(const int4 *)&a;
+    *(int4 *)(p + plane) = *(const int4 *)&b;
+    *(int4 *)(p + 2 * plane) = *(const int4 *)&c;
+  }
+}
+
+// out[i] = sum over `parts` of part[k * stride + i], in order.
+template <class T>
+__global__ void __launch_bounds__(256) ff_sum_kernel(const float *__restrict__ part, int parts, size_t stride, size_t total, T *__restrict__ out) {
+  after_previous();
+  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= total) return;
+  float v = 0.f;
+  for (int k = 0; k < parts; ++k) v += part[(size_t)k * stride + i];
+  out[i] = (T)v;
+}
+
+// Column sums of rows [rows][pitch] (planes of float32 ones added up), a block's share of the rows: part[blockIdx.y][cols].
+template <class T>
+__global__ void __launch_bounds__(256) ff_columns_kernel(const T *__restrict__ src, long long rows, int cols, int pitch, int planes, size_t plane,
+                                                         float *__restrict__ part, int accumulate) {
+  after_previous();
+  __shared__ float sm[8][32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+  const long long lo = rows * blockIdx.y / gridDim.y, hi = rows * (blockIdx.y + 1) / gridDim.y;
+  float v = 0.f;
+  if (col < cols)
+    for (int k = planes - 1; k >= 0; --k)
+      for (long long r = lo + w; r < hi; r += 8) v += (float)src[k * plane + r * pitch + col];
+  sm[w][lane] = v;
+  __syncthreads();
+  if (w == 0 && col < cols) {
+    for (int i = 1; i < 8; ++i) v += sm[i][lane];
+    float *o = part + (size_t)blockIdx.y * cols + col;
+    *o = accumulate ? *o + v : v;
+  }
+}
+
+// Few rows: the weights are read once and bound the time; a warp to an output, rows in shared memory, sums in float32 and h
+// never rounded.  kR rows at a time.
+constexpr int kR = 8;
+template <class T>
+__device__ __forceinline__ void dot_rows(const T *__restrict__ w, const float *__restrict__ xs, int k, int stride, int live, float *acc, int vec) {
+  constexpr int N = 16 / sizeof(T);
+  const int lane = threadIdx.x & 31;
+  if (vec) {
+    for (int i = lane * N; i < k; i += 32 * N) {
+      struct alignas(16) { T v[N]; } q;
+      *(int4 *)&q = *(const int4 *)(w + i);
+#pragma unroll
+      for (int r = 0; r < kR; ++r)
+        if (r < live) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) acc[r] = fmaf((float)q.v[e], xs[r * stride + i + e], acc[r]);
+        }
+    }
+  } else {
+    for (int i = lane; i < k; i += 32)
+#pragma unroll
+      for (int r = 0; r < kR; ++r)
+        if (r < live) acc[r] = fmaf((float)w[i], xs[r * stride + i], acc[r]);
+  }
+#pragma unroll
+  for (int r = 0; r < kR; ++r)
+    for (int d = 16; d > 0; d >>= 1) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], d);
+}
+
+template <class T>
+__global__ void __launch_bounds__(256) ff_few_hidden_kernel(const T *__restrict__ x, int rows, int c, int hidden, const T *__restrict__ w_in, const T *__restrict__ b_in,
+                                                            int act, float *__restrict__ h, int vec) {
+  after_previous();
+  extern __shared__ float xs[];                 // [kR][c rounded up to 8]
+  const int r0 = blockIdx.y * kR, live = min(kR, rows - r0), stride = (c + 7) & ~7;
+  for (int i = threadIdx.x; i < live * c; i += 256) {
+    const int r = i / c;
+    xs[r * stride + i - r * c] = (float)x[(size_t)(r0 + r) * c + i - r * c];
+  }
+  __syncthreads();
+  const int j = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (j >= hidden) return;
+  float g[kR] = {}, u[kR] = {};
+  dot_rows<T>(w_in + (size_t)j * c, xs, c, stride, live, g, vec);
+  dot_rows<T>(w_in + (size_t)(hidden + j) * c, xs, c, stride, live, u, vec);
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int r = 0; r < kR; ++r)
+    if (r < live && lane == r) {
+      const float bg = b_in ? (float)b_in[j] : 0.f, bu = b_in ? (float)b_in[hidden + j] : 0.f;
+      h[(size_t)(r0 + r) * hidden + j] = act_value(g[r] + bg, act) * (u[r] + bu);
+    }
+}
+
+template <class T>
+__global__ void __launch_bounds__(256) ff_few_out_kernel(const float *__restrict__ h, int rows, int hidden, int c_out, const T *__restrict__ w_out, const T *__restrict__ b_out,
+                                                         const T *__restrict__ residual, T *__restrict__ y, int vec) {
+  after_previous();
+  const int r0 = blockIdx.y * kR, live = min(kR, rows - r0);
+  const int o = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (o >= c_out) return;
+  float v[kR] = {};
+  dot_rows<T>(w_out + (size_t)o * hidden, h + (size_t)r0 * hidden, hidden, hidden, live, v, vec);
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int r = 0; r < kR; ++r)
+    if (r < live && lane == r) {
+      float out = v[r] + (b_out ? (float)b_out[o] : 0.f);
+      const size_t at = (size_t)(r0 + r) * c_out + o;
+      if (residual) out += (float)residual[at];
+      y[at] = (T)out;
+    }
+}
+
+// ------------------------------------------------------------------------------------------- host
+typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                             const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static const EncodeFn fn = [] {
+    void *f = nullptr;
+    cudaDriverEntryPointQueryResult how;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &how) != cudaSuccess || how != cudaDriverEntryPointSuccess) {
+      (void)cudaGetLastError();
+      f = nullptr;
+    }
+    return (EncodeFn)f;
+  }();
+  return fn;
+}
+
+// `planes` matrices [rows][cols] with rows of `pitch` elements, one behind the other.
+struct Matrix {
+  const void *p;
+  long long rows;
+  int cols, pitch, planes;
+};
+int make_map(CUtensorMap *map, const Matrix &m, bool f16) {
+  const EncodeFn fn = encode_fn();
+  if (fn == nullptr) return fail(SSC_ERR_CUDA, "gated_ff: the driver has no cuTensorMapEncodeTiled");
+  const cuuint64_t dims[3] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows, (cuuint64_t)m.planes};
+  const cuuint64_t strides[2] = {(cuuint64_t)m.pitch * 2, (cuuint64_t)m.pitch * 2 * (cuuint64_t)m.rows};
+  const cuuint32_t box[3] = {kBox, kBox, 1}, each[3] = {1, 1, 1};
+  const CUresult r = fn(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(m.p), dims, strides, box, each,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(SSC_ERR_CUDA, "gated_ff: no tensor map for [%lld, %d] (error %d)", m.rows, m.cols, (int)r);
+  return SSC_OK;
+}
+
+int pitch_of(int cols) { return (cols + 7) & ~7; }
+int planes_for(int type) { return type == SSC_PREC_FP32 ? 3 : 1; }
+
+// Scratch is handed out piece by piece; a null base counts the bytes.
+struct Scratch {
+  char *base;
+  size_t used;
+  void *take(size_t bytes) {
+    void *p = base ? base + used : nullptr;
+    used += align_up(bytes, 256);
+    return p;
+  }
+};
+
+struct Ff {
+  int type, n, c, hidden, c_out, act;
+  cudaStream_t st;
+  int32_t *status;
+  int launches;
+  cudaError_t err;
+};
+
+// The matrix as TMA reads it: itself, or planes / padded rows in scratch.
+template <class T>
+Matrix operand(Ff &f, Scratch &s, const void *p, long long rows, int cols, int each) {
+  const int pitch = pitch_of(cols), planes = planes_for(f.type);
+  if (sizeof(T) == 2 && pitch == cols && ((uintptr_t)p & 15) == 0) return {p, rows / each, cols, cols, each};
+  void *to = s.take((size_t)rows * pitch * 2 * planes);
+  if (s.base != nullptr) {
+    const long long threads = rows * (pitch / 8);
+    const cudaError_t e = launch_ready(ff_planes_kernel<T>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, f.st, (const T *)p, rows, cols, pitch, to);
+    if (e != cudaSuccess) f.err = e;
+    ++f.launches;
+  }
+  return {to, rows / each, cols, pitch, planes * each};
+}
+// (what operand() may take of the scratch; whether an address is aligned is not known when sizes are asked for)
+size_t operand_bytes(int type, long long rows, int cols) { return align_up((size_t)rows * pitch_of(cols) * 2 * planes_for(type), 256); }
+
+template <int EPI, class T>
+int launch_gemm(Ff &f, const FfMaps &maps, FfParams &p) {
+  p.pairs = planes_for(f.type) == 3 ? 6 : 1;
+  p.f16 = f.type == SSC_PREC_F16;
+  p.act = f.act;
+  p.status = f.status;
+  p.alarm = alarm_word();
+  const long long tiles = (long long)p.tiles_m * p.tiles_n * p.splits;
+  SSC_REQUIRE(tiles < 1ll << 30, "gated_ff: too many tiles");
+  const int sms = sm_count();
+  cudaError_t e = allow_smem((const void *)ff_gemm_kernel<EPI, T>, kSmemBytes);
+  if (e == cudaSuccess) e = launch_ready(ff_gemm_kernel<EPI, T>, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(kThreads), kSmemBytes, f.st, maps, p);
+  if (e != cudaSuccess) return fail(SSC_ERR_CUDA, "gated_ff: %s", cudaGetErrorString(e));
+  ++f.launches;
+  return SSC_OK;
+}
+
+Segment segment(int k, int boxes_b) {
+  Segment s = {};
+  s.a_planes = s.b_planes = 1;
+  s.blocks = ceil_div(k, kBox);
+  s.half_blocks = 1 << 30;
+  s.boxes_b = boxes_b;
+  return s;
+}
+
+// Result tiles of 64, 128 or 256 columns: the widest that is not mostly empty.
+int tile_columns(int cols) { return cols <= 64 ? 64 : cols <= 128 ? 128 : 256; }
+
+// C [rows][cols] = A B' (+ bias, residual) as rows of T; B as stored (b_mn: [k][cols]).
+template <class T>
+int rows_product(Ff &f, const Matrix &a, const Matrix &b, int b_mn, bool halves, int k, int cols, const void *bias, const void *residual, void *out) {
+  FfMaps maps = {};
+  FfParams p = {};
+  if (int e = make_map(&maps.a[0], a, f.type == SSC_PREC_F16)) return e;
+  if (int e = make_map(&maps.b[0], b, f.type == SSC_PREC_F16)) return e;
+  p.step_n = tile_columns(cols);
+  p.seg[0] = segment(k, p.step_n / kBox);
+  p.seg[0].b_mn = b_mn;
+  if (halves) {
+    p.seg[0].a_half = p.seg[0].b_half = kByK;
+    p.seg[0].a_planes = p.seg[0].b_planes = 2;
+    p.seg[0].half_blocks = p.seg[0].blocks;
+    p.seg[0].blocks *= 2;
+  }
+  p.n_seg = 1;
+  p.rows = (int)a.rows;
+  p.cols = p.pitch = cols;
+  p.tiles_m = ceil_div(p.rows, kTileM);
+  p.m_half = 1 << 30;
+  p.tiles_n = ceil_div(cols, p.step_n);
+  p.splits = 1;
+  p.bias = bias;
+  p.residual = residual;
+  p.out = out;
+  p.vec = cols % (16 / (int)sizeof(T)) == 0 && (((uintptr_t)out | (uintptr_t)residual) & 15) == 0;
+  return launch_gemm<kRows, T>(f, maps, p);
+}
+
+template <class T>
+int gate_product(Ff &f, const Matrix &x, const Matrix &w_in, const void *b_in, void *h) {
+  FfMaps maps = {};
+  FfParams p = {};
+  if (int e = make_map(&maps.a[0], x, f.type == SSC_PREC_F16)) return e;
+  if (int e = make_map(&maps.b[0], w_in, f.type == SSC_PREC_F16)) return e;
+  p.step_n = f.hidden <= 64 ? 64 : 128;
+  p.seg[0] = segment(f.c, 2 * p.step_n / kBox);
+  p.seg[0].b_half = kByBox;
+  p.seg[0].b_planes = 2;
+  p.n_seg = 1;
+  p.rows = (int)x.rows;
+  p.cols = f.hidden;
+  p.pitch = pitch_of(f.hidden);
+  p.plane = (size_t)p.rows * p.pitch;
+  p.tiles_m = ceil_div(p.rows, kTileM);
+  p.m_half = 1 << 30;
+  p.tiles_n = ceil_div(f.hidden, p.step_n);
+  p.splits = 1;
+  p.bias = b_in;
+  p.out = h;
+  return launch_gemm<kGate, T>(f, maps, p);
+}
+
+// h, dg and du: gate and up again, and dy Wo.
+template <class T>
+int back_product(Ff &f, const Matrix &x, const Matrix &w_in, const Matrix &gy, const Matrix &w_out, const void *b_in, void *h, void *dgu) {
+  FfMaps maps = {};
+  FfParams p = {};
+  const bool f16 = f.type == SSC_PREC_F16;
+  if (int e = make_map(&maps.a[0], x, f16)) return e;
+  if (int e = make_map(&maps.b[0], w_in, f16)) return e;
+  if (int e = make_map(&maps.a[1], gy, f16)) return e;
+  if (int e = make_map(&maps.b[1], w_out, f16)) return e;
+  p.step_n = 64;
+  p.seg[0] = segment(f.c, 2);
+  p.seg[0].b_half = kByBox;
+  p.seg[0].b_planes = 2;
+  p.seg[1] = segment(f.c_out, 1);
+  p.seg[1].b_mn = 1;
+  p.seg[1].col = 2 * p.step_n;
+  p.n_seg = 2;
+  p.rows = (int)x.rows;
+  p.cols = f.hidden;
+  p.pitch = pitch_of(f.hidden);
+  p.plane = p.plane2 = (size_t)p.rows * p.pitch;
+  p.tiles_m = ceil_div(p.rows, kTileM);
+  p.m_half = 1 << 30;
+  p.tiles_n = ceil_div(f.hidden, p.step_n);
+  p.splits = 1;
+  p.bias = b_in;
+  p.out = h;
+  p.out2 = dgu;
+  return launch_gemm<kBack, T>(f, maps, p);
+}
+
+// Shares of a long sum: enough tiles for every SM, at least eight blocks of 64 to a share.
+int filter_splits(long long rows, int halves, int m, int cols) {
+  const int tiles = halves * ceil_div(m, kTileM) * ceil_div(cols, tile_columns(cols)), blocks = ceil_div(rows, kBox);
+  int s = sm_count() / (tiles > 0 ? tiles : 1);
+  if (s > blocks / 8) s = blocks / 8;
+  return s < 1 ? 1 : s;
+}
+// part [splits][halves m][cols] (+)= A' B, A [k rows][m] and B [k rows][cols] as stored.
+template <class T>
+int filter_product(Ff &f, const Matrix &a, const Matrix &b, int halves, int m, int cols, int splits, float *part, int accumulate) {
+  FfMaps maps = {};
+  FfParams p = {};
+  if (int e = make_map(&maps.a[0], a, f.type == SSC_PREC_F16)) return e;
+  if (int e = make_map(&maps.b[0], b, f.type == SSC_PREC_F16)) return e;
+  p.step_n = tile_columns(cols);
+  p.seg[0] = segment((int)a.rows, p.step_n / kBox);
+  p.seg[0].a_mn = p.seg[0].b_mn = 1;
+  p.seg[0].a_planes = halves;
+  p.seg[0].a_half = halves == 2 ? kByM : kNone;
+  p.n_seg = 1;
+  p.rows = m;
+  p.cols = p.pitch = cols;
+  p.plane = (size_t)halves * m * cols;
+  p.m_half = ceil_div(m, kTileM);
+  p.tiles_m = halves * p.m_half;
+  p.tiles_n = ceil_div(cols, p.step_n);
+  p.splits = splits;
+  p.out = part;
+  p.vec = cols % 4 == 0;
+  p.accumulate = accumulate;
+  return launch_gemm<kPart, T>(f, maps, p);
+}
+
+template <class T>
+cudaError_t sum_parts(Ff &f, const float *part, int parts, size_t total, void *out) {
+  ++f.launches;
+  return launch_ready(ff_sum_kernel<T>, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, f.st, part, parts, total, total, (T *)out);
+}
+constexpr int kColumnShares = 32;
+
+// Rows of one go, so that what lies between the products is at most about a gigabyte.
+long long rows_at_once(const Ff &f, bool backward) {
+  const long long per = (long long)pitch_of(f.hidden) * 2 * planes_for(f.type) * (backward ? 3 : 1) + (long long)(pitch_of(f.c) + pitch_of(f.c_out)) * 2 * planes_for(f.type);
+  long long rows = (1ll << 30) / per / kTileM * kTileM;
+  if (rows < 32 * kTileM) rows = 32 * kTileM;
+  return rows < f.n ? rows : f.n;
+}
+
+// Rows up to which the weights are read once by a warp to an output instead of by tiles of 128 rows.
+bool few(const Ff &f) { return f.n <= (f.type == SSC_PREC_FP32 ? 64 : 16) && f.c <= 4096; }
+
+template <class T>
+int forward(Ff &f, Scratch s, const void *x, const void *w_in, const void *w_out, const void *b_in, const void *b_out, const void *residual, void *out) {
+  if (few(f)) {
+    float *h = (float *)s.take((size_t)f.n * f.hidden * sizeof(float));
+    const int vec_in = f.c % (16 / (int)sizeof(T)) == 0 && ((uintptr_t)w_in & 15) == 0, vec_out = f.hidden % (16 / (int)sizeof(T)) == 0 && ((uintptr_t)w_out & 15) == 0;
+    const size_t room = (size_t)kR * ((f.c + 7) & ~7) * sizeof(float);
+    cudaError_t e = allow_smem((const void *)ff_few_hidden_kernel<T>, room);
+    if (e == cudaSuccess)
+      e = launch_ready(ff_few_hidden_kernel<T>, dim3(ceil_div(f.hidden, 8), ceil_div(f.n, kR)), dim3(256), room, f.st, (const T *)x, f.n, f.c, f.hidden, (const T *)w_in,
+                       (const T *)b_in, f.act, h, vec_in);
+    if (e == cudaSuccess)
+      e = launch_ready(ff_few_out_kernel<T>, dim3(ceil_div(f.c_out, 8), ceil_div(f.n, kR)), dim3(256), 0, f.st, (const float *)h, f.n, f.hidden, f.c_out, (const T *)w_out,
+                       (const T *)b_out, (const T *)residual, (T *)out, vec_out);
+    if (e != cudaSuccess) return fail(SSC_ERR_CUDA, "gated_ff_fwd: %s", cudaGetErrorString(e));
+    f.launches += 2;
+    return SSC_OK;
+  }
+  const Matrix wi = operand<T>(f, s, w_in, 2ll * f.hidden, f.c, 2), wo = operand<T>(f, s, w_out, f.c_out, f.hidden, 1);
+  const long long most = rows_at_once(f, false);
+  const int pitch = pitch_of(f.hidden), planes = planes_for(f.type);
+  void *h = s.take((size_t)most * pitch * 2 * planes);
+  for (long long r = 0; r < f.n; r += most) {
+    const long long rows = f.n - r < most ? f.n - r : most;
+    Scratch here = s;
+    const Matrix xm = operand<T>(f, here, (const T *)x + r * f.c, rows, f.c, 1);
+    if (int e = gate_product<T>(f, xm, wi, b_in, h)) return e;
+    const Matrix hm = {h, rows, f.hidden, pitch, planes};
+    if (int e = rows_product<T>(f, hm, wo, 0, false, f.hidden, f.c_out, b_out, residual ? (const T *)residual + r * f.c_out : nullptr, (T *)out + r * f.c_out)) return e;
+  }
+  return SSC_OK;
+}
+
+template <class T>
+int backward(Ff &f, Scratch s, const void *x, const void *gy, const void *w_in, const void *w_out, const void *b_in, void *gx, void *gw_in, void *gw_out, void *gb_in,
+             void *gb_out) {
+  const Matrix wi = operand<T>(f, s, w_in, 2ll * f.hidden, f.c, 2), wo = operand<T>(f, s, w_out, f.c_out, f.hidden, 1);
+  const long long most = rows_at_once(f, true);
+  const int pitch = pitch_of(f.hidden), planes = planes_for(f.type);
+  const size_t size_in = 2 * (size_t)f.hidden * f.c, size_out = (size_t)f.c_out * f.hidden;
+  const int split_in = filter_splits(most, 2, f.hidden, f.c), split_out = filter_splits(most, 1, f.c_out, f.hidden);
+  void *h = s.take((size_t)most * pitch * 2 * planes), *dgu = s.take((size_t)most * pitch * 4 * planes);
+  float *part_in = (float *)s.take(split_in * size_in * sizeof(float)), *part_out = (float *)s.take(split_out * size_out * sizeof(float));
+  float *cols_in = (float *)s.take((size_t)kColumnShares * 2 * f.hidden * sizeof(float)), *cols_out = (float *)s.take((size_t)kColumnShares * f.c_out * sizeof(float));
+  cudaError_t e = cudaSuccess;
+  for (long long r = 0; r < f.n; r += most) {
+    const long long rows = f.n - r < most ? f.n - r : most;
+    Scratch here = s;
+    const int more = r > 0;
+    const Matrix xm = operand<T>(f, here, (const T *)x + r * f.c, rows, f.c, 1), gm = operand<T>(f, here, (const T *)gy + r * f.c_out, rows, f.c_out, 1);
+    if (int k = back_product<T>(f, xm, wi, gm, wo, b_in, h, dgu)) return k;
+    const Matrix hm = {h, rows, f.hidden, pitch, planes}, dm = {dgu, rows, f.hidden, pitch, 2 * planes};
+    if (gx)
+      if (int k = rows_product<T>(f, dm, wi, 1, true, f.hidden, f.c, nullptr, nullptr, (T *)gx + r * f.c)) return k;
+    if (gw_in)
+      if (int k = filter_product<T>(f, dm, xm, 2, f.hidden, f.c, split_in, part_in, more)) return k;
+    if (gw_out)
+      if (int k = filter_product<T>(f, gm, hm, 1, f.c_out, f.hidden, split_out, part_out, more)) return k;
+    const size_t plane = (size_t)rows * pitch;
+    if (gb_in)
+      for (int half = 0; half < 2 && e == cudaSuccess; ++half) {
+        float *to = cols_in + (size_t)half * kColumnShares * f.hidden;
+        const dim3 grid(ceil_div(f.hidden, 32), kColumnShares);
+        if (sizeof(T) == 2)
+          e = launch_ready(ff_columns_kernel<T>, grid, dim3(256), 0, f.st, (const T *)dgu + half * plane, rows, f.hidden, pitch, 1, plane, to, more);
+        else
+          e = launch_ready(ff_columns_kernel<__nv_bfloat16>, grid, dim3(256), 0, f.st, (const __nv_bfloat16 *)dgu + half * plane, rows, f.hidden, pitch, 3, 2 * plane, to,
+                           more);
+        ++f.launches;
+      }
+    if (gb_out && e == cudaSuccess) {
+      e = launch_ready(ff_columns_kernel<T>, dim3(ceil_div(f.c_out, 32), kColumnShares), dim3(256), 0, f.st, (const T *)gy + r * f.c_out, rows, f.c_out, f.c_out, 1, (size_t)0,
+                       cols_out, more);
+      ++f.launches;
+    }
+  }
+  if (gw_in && e == cudaSuccess) e = sum_parts<T>(f, part_in, split_in, size_in, gw_in);
+  if (gw_out && e == cudaSuccess) e = sum_parts<T>(f, part_out, split_out, size_out, gw_out);
+  if (gb_in)
+    for (int half = 0; half < 2 && e == cudaSuccess; ++half)
+      e = sum_parts<T>(f, cols_in + (size_t)half * kColumnShares * f.hidden, kColumnShares, f.hidden, (T *)gb_in + (size_t)half * f.hidden);
+  if (gb_out && e == cudaSuccess) e = sum_parts<T>(f, cols_out, kColumnShares, f.c_out, gb_out);
+  if (e != cudaSuccess) return fail(SSC_ERR_CUDA, "gated_ff_bwd: %s", cudaGetErrorString(e));
+  return SSC_OK;
+}
+
+size_t scratch_bytes_for(const Ff &f, bool back) {
+  if (!back && few(f)) return align_up((size_t)f.n * f.hidden * sizeof(float), 256) + 256;
+  const long long most = rows_at_once(f, back);
+  const size_t hidden = align_up((size_t)most * pitch_of(f.hidden) * 2 * planes_for(f.type), 256);
+  size_t b = 256 + operand_bytes(f.type, 2ll * f.hidden, f.c) + operand_bytes(f.type, f.c_out, f.hidden) + operand_bytes(f.type, most, f.c);
+  if (!back) return b + hidden;
+  const size_t size_in = 2 * (size_t)f.hidden * f.c, size_out = (size_t)f.c_out * f.hidden;
+  b += operand_bytes(f.type, most, f.c_out) + 3 * hidden + 512;
+  b += align_up(filter_splits(most, 2, f.hidden, f.c) * size_in * 4, 256) + align_up(filter_splits(most, 1, f.c_out, f.hidden) * size_out * 4, 256);
+  return b + align_up((size_t)kColumnShares * 8 * f.hidden, 256) + align_up((size_t)kColumnShares * 4 * f.c_out, 256);
+}
+
+constexpr int kMostChannels = 65536;
+int ff_check(const Ff &f, const char *what) {
+  SSC_REQUIRE(f.type == SSC_PREC_FP32 || f.type == SSC_PREC_F16 || f.type == SSC_PREC_BF16, "%s: unknown type", what);
+  SSC_REQUIRE(f.n >= 0 && f.c >= 1 && f.hidden >= 1 && f.c_out >= 1 && f.c <= kMostChannels && f.hidden <= kMostChannels && f.c_out <= kMostChannels, "%s: bad sizes", what);
+  SSC_REQUIRE(f.act >= 0 && f.act <= 4, "%s: unknown activation", what);
+  return SSC_OK;
+}
+
+}  // namespace
+}  // namespace ssc
+
+extern "C" size_t ssc_gated_ff_scratch_bytes(int type, int n, int c, int hidden, int c_out, int backward) {
+  ssc::Ff f = {type, n, c, hidden, c_out, 0};
+  if (ssc::ff_check(f, "gated_ff_scratch_bytes") != SSC_OK) return 0;
+  return ssc::scratch_bytes_for(f, backward != 0);
+}
+
+extern "C" int ssc_gated_ff_fwd(const void *x, int type, int n, int c, int hidden, int c_out, const void *w_in, const void *w_out, const void *b_in, const void *b_out,
+                                const void *residual, int act, void *out, int32_t *status, void *scratch, size_t scratch_bytes, void *stream) {
+  using namespace ssc;
+  Ff f = {type, n, c, hidden, c_out, act, as_stream(stream), status, 0, cudaSuccess};
+  if (int e = ff_check(f, "gated_ff_fwd")) return e;
+  SSC_REQUIRE(w_in && w_out && (n == 0 || (x && out)), "gated_ff_fwd: null pointer");
+  if (n == 0) return SSC_OK;
+  if (scratch == nullptr || ((uintptr_t)scratch & 15) != 0 || scratch_bytes < scratch_bytes_for(f, false)) return fail(SSC_ERR_SCRATCH, "gated_ff_fwd: scratch too small");
+  const Scratch s = {(char *)(((uintptr_t)scratch + 255) & ~(uintptr_t)255), 0};
+  int e = type == SSC_PREC_FP32  ? forward<float>(f, s, x, w_in, w_out, b_in, b_out, residual, out)
+          : type == SSC_PREC_F16 ? forward<__half>(f, s, x, w_in, w_out, b_in, b_out, residual, out)
+                                 : forward<__nv_bfloat16>(f, s, x, w_in, w_out, b_in, b_out, residual, out);
+  note_launches(f.launches);
+  if (e != SSC_OK) return e;
+  if (f.err != cudaSuccess) return fail(SSC_ERR_CUDA, "gated_ff_fwd: %s", cudaGetErrorString(f.err));
+  SSC_CHECK_LAUNCH("gated_ff_fwd");
+  return SSC_OK;
+}
+
+extern "C" int ssc_gated_ff_bwd(const void *x, const void *gy, int type, int n, int c, int hidden, int c_out, const void *w_in, const void *w_out, const void *b_in, int act,
+                                void *gx, void *gw_in, void *gw_out, void *gb_in, void *gb_out, int32_t *status, void *scratch, size_t scratch_bytes, void *stream) {
+  using namespace ssc;
+  Ff f = {type, n, c, hidden, c_out, act, as_stream(stream), status, 0, cudaSuccess};
+  if (int e = ff_check(f, "gated_ff_bwd")) return e;
+  SSC_REQUIRE(w_in && w_out && (n == 0 || (x && gy)), "gated_ff_bwd: null pointer");
+  if (n == 0) {
+    const size_t size = type == SSC_PREC_FP32 ? 4 : 2;
+    cudaError_t e = cudaSuccess;
+    if (gw_in) e = cudaMemsetAsync(gw_in, 0, 2 * (size_t)hidden * c * size, f.st);
+    if (gw_out && e == cudaSuccess) e = cudaMemsetAsync(gw_out, 0, (size_t)c_out * hidden * size, f.st);
+    if (gb_in && e == cudaSuccess) e = cudaMemsetAsync(gb_in, 0, 2 * (size_t)hidden * size, f.st);
+    if (gb_out && e == cudaSuccess) e = cudaMemsetAsync(gb_out, 0, (size_t)c_out * size, f.st);
+    if (e != cudaSuccess) return fail(SSC_ERR_CUDA, "gated_ff_bwd: %s", cudaGetErrorString(e));
+    return SSC_OK;
+  }
+  if (scratch == nullptr || ((uintptr_t)scratch & 15) != 0 || scratch_bytes < scratch_bytes_for(f, true)) return fail(SSC_ERR_SCRATCH, "gated_ff_bwd: scratch too small");
+  const Scratch s = {(char *)(((uintptr_t)scratch + 255) & ~(uintptr_t)255), 0};
+  int e = type == SSC_PREC_FP32  ? backward<float>(f, s, x, gy, w_in, w_out, b_in, gx, gw_in, gw_out, gb_in, gb_out)
+          : type == SSC_PREC_F16 ? backward<__half>(f, s, x, gy, w_in, w_out, b_in, gx, gw_in, gw_out, gb_in, gb_out)
+                                 : backward<__nv_bfloat16>(f, s, x, gy, w_in, w_out, b_in, gx, gw_in, gw_out, gb_in, gb_out);
+  note_launches(f.launches);
+  if (e != SSC_OK) return e;
+  if (f.err != cudaSuccess) return fail(SSC_ERR_CUDA, "gated_ff_bwd: %s", cudaGetErrorString(f.err));
+  SSC_CHECK_LAUNCH("gated_ff_bwd");
+  return SSC_OK;
+}

@@ -213,7 +213,7 @@ PyObject *head(PyObject *, PyObject *const *args, Py_ssize_t n) {
   X(ssc_p2v_keep_scratch_bytes) X(ssc_p2v_keep) X(ssc_voxel_centres) X(ssc_point_rows) X(ssc_nn_weights) \
   X(ssc_p2v_count) X(ssc_p2v_fill) X(ssc_three_nn_scratch_bytes) X(ssc_three_nn) X(ssc_three_interpolate_fwd) \
   X(ssc_bn_fold) X(ssc_bn_gate_fwd) X(ssc_bn_gate_fwd16) X(ssc_bn_scratch_bytes) X(ssc_bn_stats) X(ssc_bn_train) \
-  X(ssc_group_norm_scratch_bytes) X(ssc_group_norm_fwd) X(ssc_group_norm_bwd) \
+  X(ssc_group_norm_scratch_bytes) X(ssc_group_norm_fwd) X(ssc_group_norm_bwd) X(ssc_gated_ff_scratch_bytes) X(ssc_gated_ff_fwd) X(ssc_gated_ff_bwd) \
   X(ssc_bn_gate_bwd) X(ssc_bn_bwd) X(ssc_gate_bwd) X(ssc_scatter_add_rate)
 
 #define X(name) {#name, (PyCFunction)(void (*)())entry<&name>, METH_FASTCALL, nullptr},

@@ -10,6 +10,7 @@ from . import convolution
 from . import activation
 from . import batchnorm
 from . import groupnorm
+from . import feedforward
 from . import pool
 from . import dropout
 from . import parallel

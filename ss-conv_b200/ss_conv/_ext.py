@@ -164,6 +164,9 @@ SIGNATURES = {
                                    c_float, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
     "ssc_group_norm_bwd": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p,
                                    c_void_p, c_float, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "ssc_gated_ff_scratch_bytes": (c_size_t, [c_int] * 6),
+    "ssc_gated_ff_fwd": (c_int, [c_void_p] + [c_int] * 5 + [c_void_p] * 5 + [c_int] + [c_void_p] * 3 + [c_size_t, c_void_p]),
+    "ssc_gated_ff_bwd": (c_int, [c_void_p] * 2 + [c_int] * 5 + [c_void_p] * 3 + [c_int] + [c_void_p] * 7 + [c_size_t, c_void_p]),
     "ssc_scatter_add_rate": (c_int, [c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
 }
 
@@ -1749,6 +1752,32 @@ def group_norm_backward(x, gy, offsets, layout, weight, bias, eps, codes, stats)
                                     _p(bias, torch.float32), eps, codes[0], codes[1], _p(stats), _p(gx), _p(grads), _p(grads[layout.n_field:]),
                                     _p(scratch), nbytes, _stream()))
     return gx, grads[:layout.n_field], grads[layout.n_field:layout.n_field + layout.n_scalar]
+
+
+# ================================================================ gated feed-forward
+@_on_device_of
+def gated_ff_forward(x, w_in, w_out, b_in, b_out, residual, act):
+    """(act(x w_in[0]' + b_in[0]) * (x w_in[1]' + b_in[1])) w_out' + b_out (+ residual); contiguous tensors of one type."""
+    n, (c_out, hidden), dev, kind = x.shape[0], w_out.shape, x.device, ROW_TYPES[x.dtype]
+    out = _empty((n, c_out), x.dtype, dev)
+    nbytes = int(lib().ssc_gated_ff_scratch_bytes(kind, n, x.shape[1], hidden, c_out, 0))
+    scratch = _empty(nbytes, torch.uint8, dev)
+    _check(lib().ssc_gated_ff_fwd(_p(x), kind, n, x.shape[1], hidden, c_out, _p(w_in), _p(w_out), _p(b_in), _p(b_out), _p(residual), act,
+                                  _p(out), _p(status_word(dev)), _p(scratch), nbytes, _stream()))
+    return out
+
+
+@_on_device_of
+def gated_ff_backward(x, gy, w_in, w_out, b_in, act, need):
+    """(gx, gw_in, gw_out, gb_in, gb_out), None where `need` says so."""
+    n, (c_out, hidden), dev, kind = x.shape[0], w_out.shape, x.device, ROW_TYPES[x.dtype]
+    shapes = (x.shape, w_in.shape, w_out.shape, (2, hidden), (c_out,))
+    grads = [_empty(tuple(s), x.dtype, dev) if k else None for s, k in zip(shapes, need)]
+    nbytes = int(lib().ssc_gated_ff_scratch_bytes(kind, n, x.shape[1], hidden, c_out, 1))
+    scratch = _empty(nbytes, torch.uint8, dev)
+    _check(lib().ssc_gated_ff_bwd(_p(x), _p(gy, x.dtype), kind, n, x.shape[1], hidden, c_out, _p(w_in), _p(w_out), _p(b_in), act,
+                                  *(_p(g) for g in grads), _p(status_word(dev)), _p(scratch), nbytes, _stream()))
+    return grads
 
 
 def scatter_add_rate(out, rows, steps, lanes_per_row=8, warps_per_sm=16):

@@ -48,3 +48,33 @@ def test_library_refuses_bad_arguments_of_the_norm():
         assert forward(**bad) == 1, bad
     assert forward(n=5) == 3 and b"scratch" in L.ssc_last_error()
     assert L.ssc_group_norm_scratch_bytes(-1, 1, 8, 2, 8, 8) == 0
+
+
+def test_feedforward_refusals():
+    from ss_conv import _ext
+    from ss_conv.feedforward import GatedFeedForward, gated_feedforward
+    L = _ext.lib()
+
+    def forward(type=0, n=0, c=8, hidden=8, out=8, act=3, w=64):
+        return L.ssc_gated_ff_fwd(64, type, n, c, hidden, out, w, 64, None, None, None, act, 64, None, None, 0, None)
+
+    assert forward() == 0
+    for bad in (dict(type=1), dict(type=4), dict(n=-1), dict(c=0), dict(hidden=0), dict(out=0), dict(hidden=65537), dict(act=5), dict(act=-1), dict(w=None)):
+        assert forward(**bad) == 1, bad
+    assert forward(n=5) == 3 and b"scratch" in L.ssc_last_error()
+    assert L.ssc_gated_ff_bwd(64, 64, 0, 5, 8, 8, 8, 64, 64, None, 3, 64, None, None, None, None, None, None, 0, None) == 3
+    assert L.ssc_gated_ff_scratch_bytes(0, 5, 0, 8, 8, 0) == 0
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        gated_feedforward(torch.zeros(2, 4), torch.zeros(2, 8, 4), torch.zeros(4, 8))
+    with pytest.raises(ValueError):
+        GatedFeedForward(4, 8, activation=torch.tanh)
+
+
+def test_feedforward_scratch_is_bounded_and_covers_its_pieces():
+    """A million wide rows are taken in turns; scratch never shrinks with more rows."""
+    from ss_conv import _ext
+    L = _ext.lib()
+    for kind in (0, 2, 3):
+        for back in (0, 1):
+            sizes = [int(L.ssc_gated_ff_scratch_bytes(kind, n, 512, 2048, 512, back)) for n in (1, 16, 17, 64, 65, 1000, 100000, 1000000, 2 ** 31 - 1)]
+            assert sizes[-1] == sizes[-2] < 3 * 2 ** 30 and all(s > 0 for s in sizes)
