@@ -132,24 +132,6 @@ __device__ __forceinline__ void put_hidden(void *base, size_t at, size_t plane, 
 __device__ __forceinline__ void tmem_floats(float *v, uint32_t addr) { tmem_ld16((uint32_t *)v, addr); }
 __device__ __forceinline__ void tmem_arrived() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
-// Activations of results that are rounded to 16 bits: two steps of 2^-22 or so do not show.
-template <bool EXACT>
-__device__ __forceinline__ float gate_value(float z, int kind) {
-  if (!EXACT && kind == 3) return __fdividef(z, 1.0f + __expf(-z));
-  return act_value(z, kind);
-}
-template <bool EXACT>
-__device__ __forceinline__ void gate_both(float z, int kind, float &value, float &slope) {
-  if (!EXACT && kind == 3) {
-    const float s = __fdividef(1.0f, 1.0f + __expf(-z));
-    value = z * s;
-    slope = s * fmaf(z, 1.f - s, 1.f);
-    return;
-  }
-  value = act_value(z, kind);
-  slope = act_slope(z, kind);
-}
-
 struct Tile {
   int m, n, split;      // tile numbers
 };
@@ -190,17 +172,18 @@ __device__ __forceinline__ void finish(const FfParams &p, int split, int half_m,
     }
   }
   if (EPI == kGate) {
+    act_values<sizeof(T) == 4, 16>(v, p.act);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = gate_value<sizeof(T) == 4>(v[i], p.act) * u[i];
+    for (int i = 0; i < 16; ++i) v[i] *= u[i];
     if (row < p.rows) put_hidden<T>(p.out, (size_t)row * p.pitch + n, p.plane, v, left);
   } else if (EPI == kBack) {
-    float h[16];
+    float s[16], h[16];
+    act_slopes<sizeof(T) == 4, 16>(v, s, p.act);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      float a, s;
-      gate_both<sizeof(T) == 4>(v[i], p.act, a, s);
+      const float a = v[i];
       h[i] = a * u[i];
-      v[i] = d[i] * u[i] * s;
+      v[i] = d[i] * u[i] * s[i];
       u[i] = d[i] * a;
     }
     if (row < p.rows) {
@@ -548,7 +531,9 @@ __global__ void __launch_bounds__(256) ff_few_hidden_kernel(const T *__restrict_
   for (int r = 0; r < kR; ++r)
     if (r < live && lane == r) {
       const float bg = b_in ? (float)b_in[j] : 0.f, bu = b_in ? (float)b_in[hidden + j] : 0.f;
-      h[(size_t)(r0 + r) * hidden + j] = act_value(g[r] + bg, act) * (u[r] + bu);
+      float a = g[r] + bg;
+      act_values<true, 1>(&a, act);
+      h[(size_t)(r0 + r) * hidden + j] = a * (u[r] + bu);
     }
 }
 

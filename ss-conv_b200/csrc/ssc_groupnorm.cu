@@ -272,6 +272,10 @@ __global__ void __launch_bounds__(kGnThreads) gn_apply_kernel(GnArgs a) {
     shift[q] = sc >= 0 && a.bias ? a.bias[sc] : 0.f;
     gate[q] = body ? a.t.gate_of_channel[ch + q] : -2;
   }
+  bool mixed = false;                                 // scalars to be activated beside other channels
+#pragma unroll
+  for (int q = 1; q < VEC; ++q) mixed |= (gate[q] == -1) != (gate[0] == -1);
+  constexpr bool EXACT = sizeof(TO) == 4;
   const T *x = (const T *)a.x + ch;
   float *gates = sm + 2 * a.n_group;
   for (int row0 = k.lo; row0 < k.hi; row0 += 4 * R) {
@@ -292,22 +296,34 @@ __global__ void __launch_bounds__(kGnThreads) gn_apply_kernel(GnArgs a) {
       for (int q = 0; q < VEC; ++q) v[u][q] = fmaf(v[u][q] - mu[q], scale[q], shift[q]);
     if (GATED) {
       if (!body) {
+        act_values<EXACT, 4 * VEC>(&v[0][0], a.gate_act);
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
-          for (int q = 0; q < VEC; ++q) gates[(u * R + ty) * a.n_gate + ch - a.c_out + q] = act_value(v[u][q], a.gate_act);
+          for (int q = 0; q < VEC; ++q) gates[(u * R + ty) * a.n_gate + ch - a.c_out + q] = v[u][q];
       }
       __syncthreads();
     }
     if (body) {
+      if (!mixed) {
+        if (gate[0] == -1) act_values<EXACT, 4 * VEC>(&v[0][0], a.scalar_act);
+      } else {
+        float f[4 * VEC];
+#pragma unroll
+        for (int i = 0; i < 4 * VEC; ++i) f[i] = (&v[0][0])[i];
+        act_values<EXACT, 4 * VEC>(f, a.scalar_act);
+#pragma unroll
+        for (int i = 0; i < 4 * VEC; ++i)
+          if (gate[i % VEC] == -1) (&v[0][0])[i] = f[i];
+      }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int row = row0 + u * R + ty;
         if (row >= k.hi) continue;
+        if (GATED) {
 #pragma unroll
-        for (int q = 0; q < VEC; ++q) {
-          if (gate[q] == -1) v[u][q] = act_value(v[u][q], a.scalar_act);
-          else if (GATED && gate[q] >= 0) v[u][q] *= gates[(u * R + ty) * a.n_gate + gate[q]];
+          for (int q = 0; q < VEC; ++q)
+            if (gate[q] >= 0) v[u][q] *= gates[(u * R + ty) * a.n_gate + gate[q]];
         }
         store<TO, VEC>(out + (size_t)row * a.c_out, v[u]);
       }
@@ -322,10 +338,12 @@ struct GnBack {
   float mu[VEC], r[VEC], w[VEC], b[VEC];
   int gate[VEC];
   int first[VEC], len[VEC];      // gate channels: the field behind the gate
+  bool scalars;                  // some channel has the scalar activation
   float *gates, *prods;          // [2 R][n_gate], [2 R][c_out]
 
   __device__ __forceinline__ void setup(const GnArgs &a, const Chunk &k, int ch, float *room) {
     const bool body = ch < a.c_out;
+    scalars = false;
 #pragma unroll
     for (int q = 0; q < VEC; ++q) {
       const int g = a.t.group_of_channel[ch + q], sc = a.t.scalar_of_channel[ch + q];
@@ -335,6 +353,7 @@ struct GnBack {
       w[q] = a.weight ? a.weight[a.t.field_of_channel[ch + q]] : 1.f;
       b[q] = sc >= 0 && a.bias ? a.bias[sc] : 0.f;
       gate[q] = body ? a.t.gate_of_channel[ch + q] : -2;
+      scalars |= gate[q] == -1;
       if (GATED) {
         const int f = body ? 0 : a.t.gate_field[ch - a.c_out + q];
         first[q] = body ? 0 : a.t.field_first[f];
@@ -348,7 +367,8 @@ struct GnBack {
   __device__ __forceinline__ void rows(const GnArgs &a, const Chunk &k, int row0, int ch, float (&hat)[2][VEC], float (&dz)[2][VEC]) {
     const int R = blockDim.y, ty = threadIdx.y;
     const bool body = ch < a.c_out;
-    float z[2][VEC];
+    constexpr bool EXACT = sizeof(T) == 4;
+    float z[2][VEC], slope[2][VEC];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int row = row0 + u * R + ty;
@@ -359,35 +379,39 @@ struct GnBack {
       if (live && body) load<T, VEC>((const T *)a.gy + (size_t)row * a.c_out + ch, dz[u]);
     }
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int q = 0; q < VEC; ++q) {
         hat[u][q] = (hat[u][q] - mu[q]) * r[q];
         z[u][q] = fmaf(hat[u][q], w[q], b[q]);
       }
-      if (GATED) {
-        const int at = u * R + ty;
-        if (body) {
+    if (GATED && body) {
 #pragma unroll
-          for (int q = 0; q < VEC; ++q) prods[at * a.c_out + ch + q] = dz[u][q] * z[u][q];
-        } else {
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int q = 0; q < VEC; ++q) gates[at * a.n_gate + ch - a.c_out + q] = act_value(z[u][q], a.gate_act);
-        }
-      }
+        for (int q = 0; q < VEC; ++q) prods[(u * R + ty) * a.c_out + ch + q] = dz[u][q] * z[u][q];
     }
-    if (GATED) __syncthreads();
+    if (!body || scalars) act_slopes<EXACT, 2 * VEC>(&z[0][0], &slope[0][0], body ? a.scalar_act : a.gate_act);
+    if (GATED) {
+      if (!body) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int q = 0; q < VEC; ++q) gates[(u * R + ty) * a.n_gate + ch - a.c_out + q] = z[u][q];
+      }
+      __syncthreads();
+    }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int at = u * R + ty;
 #pragma unroll
       for (int q = 0; q < VEC; ++q) {
-        if (gate[q] == -1) dz[u][q] *= act_slope(z[u][q], a.scalar_act);
+        if (gate[q] == -1) dz[u][q] *= slope[u][q];
         else if (GATED && gate[q] >= 0) dz[u][q] *= gates[at * a.n_gate + gate[q]];
         else if (GATED && !body) {
           float s = 0.f;
           for (int i = 0; i < len[q]; ++i) s += prods[at * a.c_out + first[q] + i];
-          dz[u][q] = row0 + at < k.hi ? s * act_slope(z[u][q], a.gate_act) : 0.f;
+          dz[u][q] = row0 + at < k.hi ? s * slope[u][q] : 0.f;
         }
       }
     }
