@@ -598,16 +598,19 @@ int ssc_gate_bwd(const float *x, const float *gy, int n, int c_total, int c_out,
  * group_copies [n_group].  weight [n_field] and bias [n_scalar] float32 or NULL.  Activations: 0 identity, 1 relu, 2 sigmoid,
  * 3 silu, 4 gelu (erf).  out_type is `type`, or any for float32 rows.  stats [batch, n_group, 2] float32 receives mean (0 for l > 0) and
  * (variance + eps)^-1/2 of every sample that has rows, which the backward call reads.  Sums are float32, in a fixed order.
- * c is at most 512 channels, 1024 / 2048 / 4096 where c, c - n_gate and the addresses are multiples of 2 / 4 / 8 channels
- * (8: 16-bit rows).  gx has the type of x; d_weight [n_field], d_bias [n_scalar] float32. */
-size_t ssc_group_norm_scratch_bytes(int n, int batch, int c, int n_group, int n_field, int n_scalar);
+ * c is at most 512 channels, 1024 / 2048 where c and c - n_gate are multiples of 2 / 4,
+ * with at most 512 gates.  Rows and scratch
+ * start at multiples of 16 bytes.  scratch: ssc_group_norm_scratch_bytes(...) (forward: n_field = n_scalar = 0 will do).  status: as in
+ * ssc_conv_fwd.  gx has the type of x; d_weight [n_field], d_bias [n_scalar] float32. */
+size_t ssc_group_norm_scratch_bytes(int batch, int n_group, int n_field, int n_scalar);
 int ssc_group_norm_fwd(const void *x, int type, int n, int c, const int32_t *offsets, int batch, const int32_t *table, int n_field,
                        int n_scalar, int n_group, int n_gate, const float *weight, const float *bias, float eps, int scalar_act,
-                       int gate_act, void *out, int out_type, float *stats, void *scratch, size_t scratch_bytes, void *stream);
+                       int gate_act, void *out, int out_type, float *stats, int32_t *status, void *scratch, size_t scratch_bytes,
+                       void *stream);
 int ssc_group_norm_bwd(const void *x, const void *gy, int type, int n, int c, const int32_t *offsets, int batch,
                        const int32_t *table, int n_field, int n_scalar, int n_group, int n_gate, const float *weight,
                        const float *bias, float eps, int scalar_act, int gate_act, const float *stats, void *gx, float *d_weight,
-                       float *d_bias, void *scratch, size_t scratch_bytes, void *stream);
+                       float *d_bias, int32_t *status, void *scratch, size_t scratch_bytes, void *stream);
 
 /* Gated feed-forward of rows: out = (act(x Wg' + bg) * (x Wu' + bu)) Wo' + bo (+ residual), and its gradients.  No counterpart in
  * the reference, whose networks end in plain linear layers (LineMOD/model.py).

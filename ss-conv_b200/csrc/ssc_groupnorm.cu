@@ -5,14 +5,17 @@
 // rotations.  With r = (v + eps)^-1/2: z = (x - mu) r w + b; the activation follows.  Backward, with a = dz w, xhat = (x - mu) r and M =
 // rows * copies: dx = r (a - [scalars] sum(a) / M - xhat sum(a xhat) / M), dw = sum dz xhat, db = sum dz.
 //
-// Memory-bound: each direction is two passes over the rows, sums first.  The samples are cut into chunks of equal length,
-// one to a block, about four blocks to an SM; a block leaves one partial result for each group, and every block of the second pass adds up
-// those of its own sample in a fixed order (no atomics: the same bits every time).
+// Memory-bound: each direction is two passes over the rows, sums first.  The rows are cut into equal ranges, one to a block, two blocks to an SM,
+// whatever the samples' lengths; a block walks through the pieces of samples in its range and leaves a partial result for each, and the second
+// pass adds up those of a sample in a fixed order (no atomics: the same bits every time).  Rows come by bulk copies into a ring of
+// tiles: with loads in the threads themselves, registers for the rows in flight left room for two blocks of
+// 256 threads, which waited for memory half of the time.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include "ssc_common.cuh"
 #include "ssc_rows_act.cuh"
+#include "ssc_tc_ptx.cuh"
 
 namespace ssc {
 namespace {
@@ -33,77 +36,19 @@ struct GnArgs {
   const float *weight, *bias;
   float eps;
   int scalar_act, gate_act;
-  int chunk_rows, max_chunks;
-  float *partial;      // [max_chunks][n_group][2]
-  float *fields;       // [max_chunks][n_field + n_scalar]
+  int threads, tile, range, blocks, stages;    // threads and rows of a tile and of a block; blocks; tiles of the ring
+  uint32_t x_bytes, stage_bytes;               // of a stage: rows of x, then of gy
+  float *partial;      // [blocks + batch][n_group][2]: block b's piece of sample s at b + s
+  float *fields;       // [blocks][n_field + n_scalar]
   float *stats;        // [batch][n_group][2]: mu, r
   float *d_weight, *d_bias;
+  int32_t *status, *alarm;
 };
 
 constexpr int kGnThreads = 512;             // at most; 256 where a row has fewer slots than that
+constexpr int kGnStages = 8;
+constexpr int kGnGateRows = 4;             // rows side by side in the gates' part of the backward passes, where a row leaves room for fewer
 constexpr int kGnSum = 32;                  // columns of d_weight | d_bias to a block of the second backward pass
-
-struct Chunk {
-  int sample;        // -1: rows of no sample, -2: nothing
-  int lo, hi;        // rows
-  int first, chunks; // the sample's chunks
-  int rows;          // of the sample
-  int total;         // chunks of all samples
-};
-
-// The chunk of block b: samples are cut one after the other, the rows before the first and behind the last one come last.
-// Offsets beyond the rows are cut down to them.  Called by the whole block.
-__device__ __forceinline__ Chunk find_chunk(const GnArgs &a, int b, Chunk *shared) {
-  if (threadIdx.y == 0 && threadIdx.x == 0) shared->sample = -2;
-  const int t = threadIdx.y * blockDim.x + threadIdx.x;
-  __syncthreads();
-  if (t < 32) {
-    int base = 0, edge0 = 0, edge1 = 0;
-    for (int s0 = 0; s0 < a.batch; s0 += 32) {
-      const int s = s0 + t;
-      int lo = 0, hi = 0;
-      if (s < a.batch) {
-        lo = min(max(a.offsets[s], 0), a.n);
-        hi = min(max(a.offsets[s + 1], lo), a.n);
-        if (s == 0) edge0 = lo;
-        if (s == a.batch - 1) edge1 = hi;
-      }
-      const int mine = (int)(((long long)(hi - lo) + a.chunk_rows - 1) / a.chunk_rows);
-      int upto = mine;
-      for (int d = 1; d < 32; d <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, upto, d);
-        if (t >= d) upto += v;
-      }
-      const int first = base + upto - mine;
-      if (b >= first && b < first + mine) {
-        shared->sample = s;
-        shared->lo = lo + (b - first) * a.chunk_rows;
-        shared->hi = min(shared->lo + a.chunk_rows, hi);
-        shared->first = first;
-        shared->chunks = mine;
-        shared->rows = hi - lo;
-      }
-      base += __shfl_sync(0xffffffffu, upto, 31);
-    }
-    edge0 = __shfl_sync(0xffffffffu, edge0, 0);
-    edge1 = __shfl_sync(0xffffffffu, edge1, (a.batch - 1) & 31);
-    if (t == 0) {
-      shared->total = min(base, a.max_chunks);
-      if (b >= base) {
-        const int before = (int)(((long long)edge0 + a.chunk_rows - 1) / a.chunk_rows), k = b - base;
-        const int lo = k < before ? k * a.chunk_rows : edge1 + (k - before) * a.chunk_rows;
-        const int end = k < before ? edge0 : a.n;
-        if (lo >= 0 && lo < end) {
-          shared->sample = -1;
-          shared->lo = lo;
-          shared->hi = min(lo + a.chunk_rows, end);
-        }
-      }
-    }
-  }
-  __syncthreads();
-  return *shared;
-}
 
 // Rows of T, VEC channels at a time.
 template <class T, int VEC>
@@ -122,481 +67,677 @@ __device__ __forceinline__ void store(T *p, const float *v) {
   *(Pack<T, VEC> *)p = k;
 }
 
-// Two sets of values as (count, mean, sum of squared distances from it), added to one (Chan et al. 1979).  Sums of squares and
-// of values alone would lose the variance of rows far from zero.
-__device__ __forceinline__ void merge(float &n, float &m, float &q, float n2, float m2, float q2) {
-  const float tot = n + n2;
-  if (tot <= 0.f) return;
-  const float f = __fdividef(n2, tot), d = m2 - m;
-  m = fmaf(d, f, m);
-  q += q2 + d * d * n * f;
-  n = tot;
-}
+// The block's range of rows as tiles of a ring in shared memory, which thread 0 feeds as it goes: one tile behind, so that it does not wait for
+// the slowest warp.  (A ninth warp that feeds it costs a quarter of the registers.)
+struct GnRing {
+  uint32_t ring, full, empty;
+  char *base;
+  volatile int *abort_flag;
+  int r0, r1, x_row, gy_row;
+  int issued;               // thread 0: tiles so far, the slot of the next one and the phase of its copies
+  uint32_t put_slot, put_phase;
+  // the tile they are at, its first row, its slot and the slot's phase, whether it has been waited for
+  int first;
+  uint32_t slot, phase;
+  bool here;
 
-// First pass, forward: mean and sum of squared distances of each group of a chunk.  A thread takes four rows at a time, exactly
-// (mean first), and adds them to its running values.
+  __device__ __forceinline__ void open(const GnArgs &a, int block, char *smem, uint64_t *bars, volatile int *flag, int size, int size_gy) {
+    ring = smem_u32(smem);
+    base = smem;
+    full = smem_u32(bars);
+    empty = full + 8 * kGnStages;
+    abort_flag = flag;
+    r0 = (int)min((long long)block * a.range, (long long)a.n);
+    r1 = (int)min((long long)r0 + a.range, (long long)a.n);
+    first = r0;
+    slot = phase = 0;
+    here = false;
+    x_row = a.c * size;
+    gy_row = a.c_out * size_gy;
+    issued = 0;
+    put_slot = put_phase = 0;
+    if (threadIdx.x == 0) {
+      for (int s = 0; s < a.stages; ++s) {
+        mbar_init(full + 8 * s, 1);
+        mbar_init(empty + 8 * s, a.threads / 32);
+      }
+      *flag = 0;
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    if (threadIdx.x == 0)
+      for (int s = 0; s < a.stages; ++s) issue(a);
+  }
+  // (one thread) rows [row, row + rows) of a matrix of `bytes` wide rows; returns what the copy engine brings, which takes 16 bytes at a time:
+  // the end of the last row of all may be left to this thread.
+  static __device__ __forceinline__ uint32_t piece(const void *src, int row, int rows, int bytes, bool issue, char *dst, uint32_t at, uint32_t bar) {
+    const char *from = (const char *)src + (size_t)row * bytes;
+    const uint32_t all = (uint32_t)rows * bytes, whole = all & ~15u;
+    if (!issue) {
+      for (uint32_t i = whole; i < all; i += 2) *(uint16_t *)(dst + i) = *(const uint16_t *)(from + i);
+    } else if (whole) {
+      bulk_g2s(at, from, whole, bar);
+    }
+    return whole;
+  }
+  // (thread 0) the next tile into its slot, once all warps have left the one that was there.
+  __device__ __forceinline__ void issue(const GnArgs &a) {
+    const int row = r0 + issued * a.tile;
+    if (row >= r1) return;
+    const uint32_t at = put_slot * a.stage_bytes, bar = full + 8 * put_slot;
+    if (issued >= a.stages && !mbar_wait(empty + 8 * put_slot, put_phase ^ 1, abort_flag)) return;
+    const int rows = min(a.tile, r1 - row);
+    uint32_t bytes = piece(a.x, row, rows, x_row, false, base + at, 0, 0);
+    if (gy_row) bytes += piece(a.gy, row, rows, gy_row, false, base + at + a.x_bytes, 0, 0);
+    mbar_expect_tx(bar, bytes);
+    piece(a.x, row, rows, x_row, true, nullptr, ring + at, bar);
+    if (gy_row) piece(a.gy, row, rows, gy_row, true, nullptr, ring + at + a.x_bytes, bar);
+    ++issued;
+    if (++put_slot == (uint32_t)a.stages) put_slot = 0, put_phase ^= 1;
+  }
+  // The block's end: copies that nobody has waited for arrive before it leaves.
+  __device__ __forceinline__ void close(const GnArgs &a) {
+    __syncthreads();
+    if (*abort_flag && threadIdx.x == 0) {
+      for (int s = max(issued - a.stages, 0); s < issued; ++s) mbar_wait_drain(full + 8 * (s % a.stages), (s / a.stages) & 1);
+      report_expired(a.status, a.alarm);
+    }
+  }
+  // The tile at hand.  After a wait that has run out the walk goes on to its end, on whatever is there: the consumers wait for one
+  // another on the way.
+  __device__ __forceinline__ const char *tile(const GnArgs &a) {
+    if (!here) {
+      (void)mbar_wait(full + 8 * slot, phase, abort_flag);
+      here = true;
+    }
+    return base + slot * a.stage_bytes;
+  }
+  __device__ __forceinline__ int end(const GnArgs &a) const { return min(first + a.tile, r1); }
+  // Rows up to `row` are done.
+  __device__ __forceinline__ void release(const GnArgs &a, int row) {
+    if (row < end(a)) return;
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(empty + 8 * slot);
+    if (threadIdx.x == 0 && first > r0) issue(a);
+    first += a.tile;
+    here = false;
+    if (++slot == (uint32_t)a.stages) slot = 0, phase ^= 1;
+  }
+};
+
+// The sample that holds a row (-1 before the first one, batch behind the last one), by 32 looks at a time; and where its piece ends.  Offsets are
+// cut down to the rows; in a list that does not ascend the pieces are arbitrary, but the walk still ends.
+struct GnWalk {
+  int s, lo, hi;
+  __device__ __forceinline__ int edge(const GnArgs &a, int i) const { return min(max(a.offsets[i], 0), a.n); }
+  __device__ __forceinline__ void find(const GnArgs &a, int row) {
+    const int lane = threadIdx.x & 31;
+    int from = 0, to = a.batch + 1;           // offsets that are at most row: their number lies between
+    while (from < to) {
+      const int step = (to - from + 31) / 32, at = from + (lane + 1) * step - 1;
+      const int many = __popc(__ballot_sync(0xffffffffu, at < to && a.offsets[at] <= row));
+      from += many * step;
+      to = min(to, from + step - 1);
+    }
+    s = from - 1;
+    place(a, row);
+  }
+  __device__ __forceinline__ void place(const GnArgs &a, int row) {
+    for (;; ++s) {
+      lo = s < 0 ? 0 : edge(a, s);
+      hi = s >= a.batch ? a.n : edge(a, s + 1);
+      if (s >= a.batch || hi > row) break;
+    }
+  }
+  __device__ __forceinline__ bool live(const GnArgs &a) const { return s >= 0 && s < a.batch; }
+};
+
+// First pass, forward: mean and sum of squared distances of each group of a piece.  A thread takes four rows at a time, exactly
+// (mean first), and adds them to its running values (Chan et al. 1979): sums of squares and of values alone would lose the
+// variance of rows far from zero.
 template <class T, int VEC>
-__global__ void __launch_bounds__(kGnThreads) gn_stats_kernel(GnArgs a) {
+__global__ void __launch_bounds__(kGnThreads, 1) gn_stats_kernel(GnArgs a) {
   after_previous();
-  __shared__ Chunk shared;
-  extern __shared__ float sm[];                       // [R][c] means, [R][c] squares
-  const Chunk k = find_chunk(a, blockIdx.x, &shared);
-  if (k.sample < 0) return;
-  const int R = blockDim.y, ty = threadIdx.y, ch = threadIdx.x * VEC;
-  float mean[VEC], sq[VEC], centred[VEC];
+  extern __shared__ __align__(128) char smem[];
+  __shared__ alignas(8) uint64_t bars[2 * kGnStages];
+  __shared__ volatile int abort_flag;
+  GnRing ring;
+  ring.open(a, blockIdx.x, smem, bars, &abort_flag, sizeof(T), 0);
+  const int t = threadIdx.x;
+  float *sm = (float *)(smem + a.stages * a.stage_bytes);       // [R][c] means, [R][c] squares
+  const int slots = a.c / VEC, R = a.threads / slots, ty = t / slots, ch = (t - ty * slots) * VEC;
+  const bool works = ty < R;
+  float *sq_s = sm + R * a.c, *sums = sq_s + R * a.c, centred[VEC];       // sums: [c] twice
 #pragma unroll
-  for (int q = 0; q < VEC; ++q) {
-    mean[q] = sq[q] = 0.f;
-    centred[q] = a.t.scalar_of_channel[ch + q] >= 0 ? 1.f : 0.f;
-  }
-  const T *x = (const T *)a.x + ch;
-  int row = k.lo + ty;
-  float have = 0.f;
-  for (; row + 3 * R < k.hi; row += 4 * R) {
-    float v[4][VEC];
+  for (int q = 0; q < VEC; ++q) centred[q] = works && a.t.scalar_of_channel[ch + q] >= 0 ? 1.f : 0.f;
+  GnWalk walk;
+  if (ring.r0 < ring.r1) walk.find(a, ring.r0);
+  for (int row = ring.r0; row < ring.r1;) {
+    const int begin = row, end = min(walk.hi, ring.r1);
+    float mean[VEC] = {}, sq[VEC] = {}, have = 0.f;
+    while (row < end) {
+      const T *x = (const T *)ring.tile(a) + ch;
+      const int first = ring.first, last = min(end, ring.end(a));
+      if (works && walk.live(a)) {
+        int i = row - first + ty;
+        const int stop = last - first;
+        for (; i + 3 * R < stop; i += 4 * R) {
+          float v[4][VEC];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) load<T, VEC>(x + (size_t)(row + u * R) * a.c, v[u]);
-    const float f = __fdividef(4.f, have + 4.f);
+          for (int u = 0; u < 4; ++u) load<T, VEC>(x + (i + u * R) * a.c, v[u]);
+          const float f = __fdividef(4.f, have + 4.f);
 #pragma unroll
-    for (int q = 0; q < VEC; ++q) {
-      const float mb = ((v[0][q] + v[1][q]) + (v[2][q] + v[3][q])) * (0.25f * centred[q]);
-      float s = 0.f;
+          for (int q = 0; q < VEC; ++q) {
+            const float mb = ((v[0][q] + v[1][q]) + (v[2][q] + v[3][q])) * (0.25f * centred[q]);
+            float s = 0.f;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) s = fmaf(v[u][q] - mb, v[u][q] - mb, s);
-      const float d = mb - mean[q];
-      mean[q] = fmaf(d, f, mean[q]);
-      sq[q] += fmaf(d * d, have * f, s);
-    }
-    have += 4.f;
-  }
-  for (; row < k.hi; row += R) {
-    float v[VEC];
-    load<T, VEC>(x + (size_t)row * a.c, v);
-    const float f = __fdividef(1.f, have + 1.f);
+            for (int u = 0; u < 4; ++u) s = fmaf(v[u][q] - mb, v[u][q] - mb, s);
+            const float d = mb - mean[q];
+            mean[q] = fmaf(d, f, mean[q]);
+            sq[q] += fmaf(d * d, have * f, s);
+          }
+          have += 4.f;
+        }
+        for (; i < stop; i += R) {
+          float v[VEC];
+          load<T, VEC>(x + i * a.c, v);
+          const float f = __fdividef(1.f, have + 1.f);
 #pragma unroll
-    for (int q = 0; q < VEC; ++q) {
-      const float mb = v[q] * centred[q], d = mb - mean[q], e = v[q] - mb;
-      mean[q] = fmaf(d, f, mean[q]);
-      sq[q] += fmaf(d * d, have * f, e * e);
-    }
-    have += 1.f;
-  }
-  float *sq_s = sm + R * a.c;
-#pragma unroll
-  for (int q = 0; q < VEC; ++q) {
-    sm[ty * a.c + ch + q] = mean[q];
-    sq_s[ty * a.c + ch + q] = sq[q];
-  }
-  __syncthreads();
-  const int t = ty * blockDim.x + threadIdx.x, threads = blockDim.x * R, rows = k.hi - k.lo;
-  for (int i = t; i < a.c; i += threads) {
-    float n = 0.f, m = 0.f, s = 0.f;
-    for (int r = 0; r < R; ++r)
-      if (r < rows) merge(n, m, s, (float)((rows - r + R - 1) / R), sm[r * a.c + i], sq_s[r * a.c + i]);
-    sm[i] = m;
-    sq_s[i] = s;
-  }
-  __syncthreads();
-  const int lane = t & 31, warps = threads >> 5;      // (the whole ones; a block has more than 128 threads)
-  if (t < warps * 32)
-    for (int g = t >> 5; g < a.n_group; g += warps) {
-      const int first = a.t.group_first[g], len = a.t.group_len[g];
-      float n = 0.f, m = 0.f, s = 0.f;
-      for (int i = lane; i < len; i += 32) merge(n, m, s, (float)rows, sm[first + i], sq_s[first + i]);
-      for (int d = 1; d < 32; d <<= 1) {
-        const float n2 = __shfl_down_sync(0xffffffffu, n, d), m2 = __shfl_down_sync(0xffffffffu, m, d), s2 = __shfl_down_sync(0xffffffffu, s, d);
-        merge(n, m, s, n2, m2, s2);
-      }
-      if (lane == 0) {
-        float *p = a.partial + ((size_t)blockIdx.x * a.n_group + g) * 2;
-        p[0] = m;
-        p[1] = s;
-      }
-    }
-}
-
-// mu and r of the block's sample, from the partial results of its chunks, to shared memory; the first chunk's block keeps them.
-__device__ __forceinline__ void sample_stats(const GnArgs &a, const Chunk &k, float *gs) {
-  const int t = threadIdx.y * blockDim.x + threadIdx.x, threads = blockDim.x * blockDim.y;
-  const int lane = t & 31, warps = threads >> 5;
-  if (t < warps * 32)
-    for (int g = t >> 5; g < a.n_group; g += warps) {
-      const float copies = (float)a.t.group_copies[g];
-      float n = 0.f, m = 0.f, s = 0.f;
-      for (int i = lane; i < k.chunks && k.first + i < a.max_chunks; i += 32) {
-        const float *p = a.partial + ((size_t)(k.first + i) * a.n_group + g) * 2;
-        merge(n, m, s, (float)min(a.chunk_rows, k.rows - i * a.chunk_rows) * copies, p[0], p[1]);
-      }
-      for (int d = 1; d < 32; d <<= 1) {
-        const float n2 = __shfl_down_sync(0xffffffffu, n, d), m2 = __shfl_down_sync(0xffffffffu, m, d), s2 = __shfl_down_sync(0xffffffffu, s, d);
-        merge(n, m, s, n2, m2, s2);
-      }
-      if (lane == 0) {
-        const float r = 1.0f / sqrtf(s / ((float)k.rows * copies) + a.eps);
-        gs[2 * g] = m;
-        gs[2 * g + 1] = r;
-        if (k.first == (int)blockIdx.x) {
-          a.stats[((size_t)k.sample * a.n_group + g) * 2] = m;
-          a.stats[((size_t)k.sample * a.n_group + g) * 2 + 1] = r;
+          for (int q = 0; q < VEC; ++q) {
+            const float mb = v[q] * centred[q], d = mb - mean[q], e = v[q] - mb;
+            mean[q] = fmaf(d, f, mean[q]);
+            sq[q] += fmaf(d * d, have * f, e * e);
+          }
+          have += 1.f;
         }
       }
+      ring.release(a, last);
+      row = last;
     }
+    if (walk.live(a)) {
+      if (works) {
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) {
+          sm[ty * a.c + ch + q] = mean[q];
+          sq_s[ty * a.c + ch + q] = sq[q];
+        }
+      }
+      __shared__ float count[kGnThreads];
+      if (works && ch == 0) count[ty] = have;
+      __syncthreads();
+      // (about the first mean of the group from here on: near enough to all of them)
+      for (int i = t; i < a.c; i += a.threads) {
+        const float about = sm[a.t.group_first[a.t.group_of_channel[i]]];
+        float u = 0.f, v = 0.f;
+        for (int r = 0; r < R; ++r) {
+          const float d = sm[r * a.c + i] - about, nd = count[r] * d;
+          u += nd;
+          v += fmaf(nd, d, sq_s[r * a.c + i]);
+        }
+        sums[i] = u;
+        sums[a.c + i] = v;
+      }
+      __syncthreads();
+      const int lane = t & 31;
+      for (int g = t >> 5; g < a.n_group; g += a.threads >> 5) {
+        const int from = a.t.group_first[g], len = a.t.group_len[g];
+        float u = 0.f, v = 0.f;
+        for (int i = lane; i < len; i += 32) u += sums[from + i], v += sums[a.c + from + i];
+        for (int d = 16; d > 0; d >>= 1) u += __shfl_xor_sync(0xffffffffu, u, d), v += __shfl_xor_sync(0xffffffffu, v, d);
+        if (lane == 0) {
+          const float n = (float)(end - begin) * (float)a.t.group_copies[g], mean = u / n;
+          *(float2 *)(a.partial + ((size_t)(blockIdx.x + walk.s) * a.n_group + g) * 2) = {sm[from] + mean, fmaxf(v - u * mean, 0.f)};
+        }
+      }
+      __syncthreads();
+    }
+    if (row < ring.r1) walk.place(a, row);
+  }
+  ring.close(a);
+}
+
+// The partial results of the walk's sample: from block `first` on, `many` of them.
+__device__ __forceinline__ void sample_pieces(const GnArgs &a, const GnWalk &k, int &first, int &many) {
+  first = k.lo / a.range;
+  many = k.hi > k.lo ? (k.hi - 1) / a.range - first + 1 : 0;
+}
+__device__ __forceinline__ int piece_rows(const GnArgs &a, const GnWalk &k, int block) {
+  const long long lo = (long long)block * a.range;
+  return (int)(min(lo + a.range, (long long)k.hi) - max(lo, (long long)k.lo));
+}
+
+// Lanes to a group where the pieces of a sample are added up: most samples have few.
+__device__ __forceinline__ int lanes_for(int many) { return many <= 4 ? 4 : many <= 8 ? 8 : 32; }
+
+// mu and r of the walk's sample, from the partial results of its pieces, to shared memory; the block with its first row keeps them.
+__device__ __forceinline__ void sample_stats(const GnArgs &a, const GnWalk &k, float *gs) {
+  int first, many;
+  sample_pieces(a, k, first, many);
+  const int width = lanes_for(many), lane = threadIdx.x & (width - 1), rows = k.hi - k.lo;
+  const float *from = a.partial + (size_t)(first + k.s) * a.n_group * 2;
+  for (int g0 = 0; g0 < a.n_group; g0 += a.threads / width) {
+    const int g = g0 + threadIdx.x / width;
+    float u = 0.f, v = 0.f, about = 0.f;
+    if (g < a.n_group) {
+      about = from[2 * g];
+      const float over = 1.0f / (float)a.t.group_copies[g];
+      for (int i = lane; i < many; i += width) {
+        const float2 p = *(const float2 *)(from + ((size_t)i * a.n_group + g) * 2);
+        const float d = p.x - about, nd = (float)piece_rows(a, k, first + i) * d;
+        u += nd;
+        v += fmaf(nd, d, p.y * over);
+      }
+    }
+    for (int d = width / 2; d > 0; d >>= 1) u += __shfl_xor_sync(0xffffffffu, u, d), v += __shfl_xor_sync(0xffffffffu, v, d);
+    if (lane == 0 && g < a.n_group) {
+      const float mean = u / (float)rows;
+      const float2 r = {about + mean, 1.0f / sqrtf(fmaxf(v - u * mean, 0.f) / (float)rows + a.eps)};
+      *(float2 *)(gs + 2 * g) = r;
+      if (first == (int)blockIdx.x) *(float2 *)(a.stats + ((size_t)k.s * a.n_group + g) * 2) = r;
+    }
+  }
   __syncthreads();
 }
 
-// Second pass, forward.  Gates go through shared memory, two buffers in turn: one wait for four rows of a thread.
+// Second pass, forward.  The gates of a tile's rows are computed first, by all threads, into one of two buffers in turn: one wait a
+// tile.
 template <class T, class TO, int VEC, bool GATED>
-__global__ void __launch_bounds__(kGnThreads) gn_apply_kernel(GnArgs a) {
+__global__ void __launch_bounds__(kGnThreads, 1) gn_apply_kernel(GnArgs a) {
   after_previous();
-  __shared__ Chunk shared;
-  extern __shared__ float sm[];                       // [n_group][2], gates: 2 x [4 R][n_gate]
-  const Chunk k = find_chunk(a, blockIdx.x, &shared);
-  if (k.sample == -2) return;
-  const int R = blockDim.y, ty = threadIdx.y, ch = threadIdx.x * VEC;
-  const bool body = ch < a.c_out;
-  TO *out = (TO *)a.out + ch;
-  if (k.sample < 0) {                                 // rows of no sample
-    const float zero[VEC] = {};
-    if (body)
-      for (int row = k.lo + ty; row < k.hi; row += R) store<TO, VEC>(out + (size_t)row * a.c_out, zero);
-    return;
-  }
-  sample_stats(a, k, sm);
-  float mu[VEC], scale[VEC], shift[VEC];
-  int gate[VEC];
-#pragma unroll
-  for (int q = 0; q < VEC; ++q) {
-    const int g = a.t.group_of_channel[ch + q], sc = a.t.scalar_of_channel[ch + q];
-    mu[q] = sm[2 * g];
-    scale[q] = sm[2 * g + 1] * (a.weight ? a.weight[a.t.field_of_channel[ch + q]] : 1.f);
-    shift[q] = sc >= 0 && a.bias ? a.bias[sc] : 0.f;
-    gate[q] = body ? a.t.gate_of_channel[ch + q] : -2;
-  }
-  bool mixed = false;                                 // scalars to be activated beside other channels
-#pragma unroll
-  for (int q = 1; q < VEC; ++q) mixed |= (gate[q] == -1) != (gate[0] == -1);
+  extern __shared__ __align__(128) char smem[];
+  __shared__ alignas(8) uint64_t bars[2 * kGnStages];
+  __shared__ volatile int abort_flag;
+  GnRing ring;
+  ring.open(a, blockIdx.x, smem, bars, &abort_flag, sizeof(T), 0);
+  const int t = threadIdx.x;
   constexpr bool EXACT = sizeof(TO) == 4;
-  const T *x = (const T *)a.x + ch;
-  float *gates = sm + 2 * a.n_group;
-  for (int row0 = k.lo; row0 < k.hi; row0 += 4 * R) {
-    float v[4][VEC];
+  float *gs = (float *)(smem + a.stages * a.stage_bytes);       // [n_group][2]
+  float *gates = gs + 2 * a.n_group;                            // 2 x [tile][n_gate]
+  const int slots = a.c_out / VEC, R = a.threads / slots, ty = t / slots, ch = (t - ty * slots) * VEC;
+  const bool works = ty < R;
+  TO *out = (TO *)a.out + ch;
+  float w[VEC], b[VEC];
+  int group[VEC], gate[VEC];
+  bool mixed = false;                                           // scalars to be activated beside other channels
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int row = row0 + u * R + ty;
-      if (row < k.hi) {
-        load<T, VEC>(x + (size_t)row * a.c, v[u]);
-      } else {
-#pragma unroll
-        for (int q = 0; q < VEC; ++q) v[u][q] = 0.f;
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-      for (int q = 0; q < VEC; ++q) v[u][q] = fmaf(v[u][q] - mu[q], scale[q], shift[q]);
-    if (GATED) {
-      if (!body) {
-        act_values<EXACT, 4 * VEC>(&v[0][0], a.gate_act);
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-          for (int q = 0; q < VEC; ++q) gates[(u * R + ty) * a.n_gate + ch - a.c_out + q] = v[u][q];
-      }
-      __syncthreads();
-    }
-    if (body) {
-      if (!mixed) {
-        if (gate[0] == -1) act_values<EXACT, 4 * VEC>(&v[0][0], a.scalar_act);
-      } else {
-        float f[4 * VEC];
-#pragma unroll
-        for (int i = 0; i < 4 * VEC; ++i) f[i] = (&v[0][0])[i];
-        act_values<EXACT, 4 * VEC>(f, a.scalar_act);
-#pragma unroll
-        for (int i = 0; i < 4 * VEC; ++i)
-          if (gate[i % VEC] == -1) (&v[0][0])[i] = f[i];
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int row = row0 + u * R + ty;
-        if (row >= k.hi) continue;
-        if (GATED) {
-#pragma unroll
-          for (int q = 0; q < VEC; ++q)
-            if (gate[q] >= 0) v[u][q] *= gates[(u * R + ty) * a.n_gate + gate[q]];
-        }
-        store<TO, VEC>(out + (size_t)row * a.c_out, v[u]);
-      }
-    }
-    if (GATED) gates = gates == sm + 2 * a.n_group ? gates + 4 * R * a.n_gate : sm + 2 * a.n_group;
+  for (int q = 0; q < VEC; ++q) {
+    const int c = works ? ch + q : 0, sc = a.t.scalar_of_channel[c];
+    group[q] = 2 * a.t.group_of_channel[c];
+    w[q] = a.weight ? a.weight[a.t.field_of_channel[c]] : 1.f;
+    b[q] = sc >= 0 && a.bias ? a.bias[sc] : 0.f;
+    gate[q] = a.t.gate_of_channel[c];
+    mixed |= (gate[q] == -1) != (gate[0] == -1);
   }
-}
-
-// dz and xhat of two rows of a thread; products with the gates' fields go through shared memory.
-template <class T, int VEC, bool GATED>
-struct GnBack {
-  float mu[VEC], r[VEC], w[VEC], b[VEC];
-  int gate[VEC];
-  int first[VEC], len[VEC];      // gate channels: the field behind the gate
-  bool scalars;                  // some channel has the scalar activation
-  float *gates, *prods;          // [2 R][n_gate], [2 R][c_out]
-
-  __device__ __forceinline__ void setup(const GnArgs &a, const Chunk &k, int ch, float *room) {
-    const bool body = ch < a.c_out;
-    scalars = false;
+  // a thread's gate, every GR-th row
+  const int GR = GATED ? a.threads / a.n_gate : 1, gj = GATED ? t % a.n_gate : 0, gr = GATED ? t / a.n_gate : 0;
+  float gw = 1.f, gb = 0.f;
+  int gg = 0;
+  if (GATED) {
+    const int c = a.c_out + gj, sc = a.t.scalar_of_channel[c];
+    gg = 2 * a.t.group_of_channel[c];
+    if (a.weight) gw = a.weight[a.t.field_of_channel[c]];
+    if (a.bias) gb = a.bias[sc];
+  }
+  GnWalk walk;
+  if (ring.r0 < ring.r1) walk.find(a, ring.r0);
+  for (int row = ring.r0; row < ring.r1;) {
+    const int end = min(walk.hi, ring.r1);
+    const bool live = walk.live(a);
+    float scale[VEC], shift[VEC], gscale = 0.f, gshift = 0.f;
+    if (live) {
+      sample_stats(a, walk, gs);
 #pragma unroll
-    for (int q = 0; q < VEC; ++q) {
-      const int g = a.t.group_of_channel[ch + q], sc = a.t.scalar_of_channel[ch + q];
-      const float *s = a.stats + ((size_t)k.sample * a.n_group + g) * 2;
-      mu[q] = s[0];
-      r[q] = s[1];
-      w[q] = a.weight ? a.weight[a.t.field_of_channel[ch + q]] : 1.f;
-      b[q] = sc >= 0 && a.bias ? a.bias[sc] : 0.f;
-      gate[q] = body ? a.t.gate_of_channel[ch + q] : -2;
-      scalars |= gate[q] == -1;
+      for (int q = 0; q < VEC; ++q) {
+        scale[q] = gs[group[q] + 1] * w[q];
+        shift[q] = fmaf(-gs[group[q]], scale[q], b[q]);      // (mu itself is rounded by as much)
+      }
       if (GATED) {
-        const int f = body ? 0 : a.t.gate_field[ch - a.c_out + q];
-        first[q] = body ? 0 : a.t.field_first[f];
-        len[q] = body ? 0 : a.t.field_len[f];
+        gscale = gs[gg + 1] * gw;
+        gshift = fmaf(-gs[gg], gscale, gb);
       }
     }
-    gates = room;
-    prods = room + 2 * blockDim.y * a.n_gate;
+    while (row < end) {
+      const T *tile = (const T *)ring.tile(a);
+      const int first = ring.first, last = min(end, ring.end(a));
+      if (GATED && live) {
+        for (int i = row - first + gr; i < last - first; i += GR)
+          if (gr < GR) {
+            float z = fmaf((float)tile[i * a.c + a.c_out + gj], gscale, gshift);
+            act_values<EXACT, 1>(&z, a.gate_act);
+            gates[i * a.n_gate + gj] = z;
+          }
+        __syncthreads();
+      }
+      if (works) {
+        for (int i = row - first + ty; i < last - first; i += 2 * R) {
+          float v[2][VEC];
+          const bool two = i + R < last - first;
+          if (live) {
+            load<T, VEC>(tile + i * a.c + ch, v[0]);
+            load<T, VEC>(tile + (two ? i + R : i) * a.c + ch, v[1]);
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int q = 0; q < VEC; ++q) v[u][q] = fmaf(v[u][q], scale[q], shift[q]);
+            if (!mixed) {
+              if (gate[0] == -1) act_values<EXACT, 2 * VEC>(&v[0][0], a.scalar_act);
+            } else {
+              float f[2 * VEC];
+#pragma unroll
+              for (int k = 0; k < 2 * VEC; ++k) f[k] = (&v[0][0])[k];
+              act_values<EXACT, 2 * VEC>(f, a.scalar_act);
+#pragma unroll
+              for (int k = 0; k < 2 * VEC; ++k)
+                if (gate[k % VEC] == -1) (&v[0][0])[k] = f[k];
+            }
+            if (GATED) {
+#pragma unroll
+              for (int q = 0; q < VEC; ++q)
+                if (gate[q] >= 0) {
+                  v[0][q] *= gates[i * a.n_gate + gate[q]];
+                  v[1][q] *= gates[(two ? i + R : i) * a.n_gate + gate[q]];
+                }
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 2 * VEC; ++k) (&v[0][0])[k] = 0.f;
+          }
+          store<TO, VEC>(out + (size_t)(first + i) * a.c_out, v[0]);
+          if (two) store<TO, VEC>(out + (size_t)(first + i + R) * a.c_out, v[1]);
+        }
+      }
+      ring.release(a, last);
+      if (GATED) gates = gates == gs + 2 * a.n_group ? gates + a.tile * a.n_gate : gs + 2 * a.n_group;
+      row = last;
+    }
+    if (live) __syncthreads();
+    if (row < ring.r1) walk.place(a, row);
   }
-  // (called by the whole block; rows behind the chunk's end give zeros)
-  __device__ __forceinline__ void rows(const GnArgs &a, const Chunk &k, int row0, int ch, float (&hat)[2][VEC], float (&dz)[2][VEC]) {
-    const int R = blockDim.y, ty = threadIdx.y;
-    const bool body = ch < a.c_out;
-    constexpr bool EXACT = sizeof(T) == 4;
-    float z[2][VEC], slope[2][VEC];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int row = row0 + u * R + ty;
-      const bool live = row < k.hi;
-#pragma unroll
-      for (int q = 0; q < VEC; ++q) hat[u][q] = mu[q], dz[u][q] = 0.f;
-      if (live) load<T, VEC>((const T *)a.x + (size_t)row * a.c + ch, hat[u]);
-      if (live && body) load<T, VEC>((const T *)a.gy + (size_t)row * a.c_out + ch, dz[u]);
+  ring.close(a);
+}
+
+// Both backward passes.  SUMS: the sums of dz and dz xhat of each channel, as the groups' sums of a and a xhat of each piece and as the block's
+// share of the parameters' gradients.  Else dx; the first blocks add up the parameters' gradients, kGnSum of them each.
+// The gates of a tile's rows come first, by all threads: value, and (from the products with their fields) dz of the gate channels.
+template <class T, int VEC, bool GATED, bool SUMS>
+__global__ void __launch_bounds__(kGnThreads, 1) gn_bwd_kernel(GnArgs a, int sum_blocks) {
+  after_previous();
+  extern __shared__ __align__(128) char smem[];
+  __shared__ alignas(8) uint64_t bars[2 * kGnStages];
+  __shared__ volatile int abort_flag;
+  const int t = threadIdx.x;
+  if (!SUMS && (int)blockIdx.x < sum_blocks) {
+    float *sm = (float *)smem;
+    const int cols = a.n_field + a.n_scalar, col = blockIdx.x * kGnSum + (t & 31), part = t >> 5, parts = blockDim.x >> 5;
+    float v = 0.f;
+    if (col < cols)
+      for (int i = part; i < a.blocks; i += parts) v += a.fields[(size_t)i * cols + col];
+    sm[t] = v;
+    __syncthreads();
+    if (t < 32 && col < cols) {
+      for (int p = 1; p < parts; ++p) v += sm[p * 32 + t];
+      if (col < a.n_field) a.d_weight[col] = v;
+      else a.d_bias[col - a.n_field] = v;
     }
+    return;
+  }
+  const int block = SUMS ? (int)blockIdx.x : (int)blockIdx.x - sum_blocks;
+  GnRing ring;
+  ring.open(a, block, smem, bars, &abort_flag, sizeof(T), sizeof(T));
+  constexpr bool EXACT = sizeof(T) == 4;
+  const int slots = a.c_out / VEC, R = a.threads / slots, ty = t / slots, ch = (t - ty * slots) * VEC;
+  const bool works = ty < R;
+  const int GR = GATED ? min(a.threads / a.n_gate, max(R, kGnGateRows)) : 1, gj = GATED ? t % a.n_gate : 0, gr = GATED ? t / a.n_gate : 0;
+  float *gs = (float *)(smem + a.stages * a.stage_bytes);       // !SUMS: [n_group][2]
+  float *gates = gs + (SUMS ? 0 : 2 * a.n_group), *const gates0 = gates;      // 2 x [tile][n_gate]
+  float *sums = gates0 + 2 * a.tile * a.n_gate;                 // SUMS: [max(R, GR)][c] twice, totals [c] twice
+  const int RS = max(R, GR);
+  float *tot = sums + 2 * RS * a.c;
+  T *out = (T *)a.out + ch;
+  float w[VEC], b[VEC];
+  int group[VEC], gate[VEC];
+  bool scalars = false;
+  unsigned centred = 0;
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+  for (int q = 0; q < VEC; ++q) {
+    const int c = works ? ch + q : 0, sc = a.t.scalar_of_channel[c];
+    group[q] = a.t.group_of_channel[c];
+    w[q] = a.weight ? a.weight[a.t.field_of_channel[c]] : 1.f;
+    b[q] = sc >= 0 && a.bias ? a.bias[sc] : 0.f;
+    gate[q] = a.t.gate_of_channel[c];
+    scalars |= gate[q] == -1;
+    centred |= (sc >= 0 ? 1u : 0u) << q;
+  }
+  float gw = 1.f, gb = 0.f, fw = 1.f;
+  int gg = 0, gf = 0, flen = 0, fg = 0;                         // the gate's group; its field's first channel, length and group
+  if (GATED) {
+    const int c = a.c_out + gj, f = a.t.gate_field[gj];
+    gg = a.t.group_of_channel[c];
+    if (a.weight) gw = a.weight[a.t.field_of_channel[c]];
+    if (a.bias) gb = a.bias[a.t.scalar_of_channel[c]];
+    gf = a.t.field_first[f];
+    flen = a.t.field_len[f];
+    fg = a.t.group_of_channel[gf];
+    if (a.weight) fw = a.weight[f];
+  }
+  if (SUMS)
+    for (int i = t; i < 2 * a.c; i += a.threads) tot[i] = 0.f;
+  GnWalk walk;
+  if (ring.r0 < ring.r1) walk.find(a, ring.r0);
+  for (int row = ring.r0; row < ring.r1;) {
+    const int end = min(walk.hi, ring.r1);
+    const bool live = walk.live(a);
+    float mu[VEC], r[VEC], s1[VEC] = {}, s2[VEC] = {}, gmu = 0.f, gr_ = 0.f, fr = 0.f, g1 = 0.f, g2 = 0.f;
+    if (live) {
+      const float *st = a.stats + (size_t)walk.s * a.n_group * 2;
 #pragma unroll
       for (int q = 0; q < VEC; ++q) {
-        hat[u][q] = (hat[u][q] - mu[q]) * r[q];
-        z[u][q] = fmaf(hat[u][q], w[q], b[q]);
+        const float2 v = *(const float2 *)(st + 2 * group[q]);
+        mu[q] = v.x;
+        r[q] = v.y;
       }
-    if (GATED && body) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int q = 0; q < VEC; ++q) prods[(u * R + ty) * a.c_out + ch + q] = dz[u][q] * z[u][q];
-    }
-    if (!body || scalars) act_slopes<EXACT, 2 * VEC>(&z[0][0], &slope[0][0], body ? a.scalar_act : a.gate_act);
-    if (GATED) {
-      if (!body) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int q = 0; q < VEC; ++q) gates[(u * R + ty) * a.n_gate + ch - a.c_out + q] = z[u][q];
+      if (GATED) {
+        gmu = st[2 * gg];
+        gr_ = st[2 * gg + 1];
+        fr = st[2 * fg + 1] * fw;
       }
-      __syncthreads();
-    }
+      if (!SUMS) {
+        int first, many;
+        sample_pieces(a, walk, first, many);
+        const int width = lanes_for(many), lane = t & (width - 1);
+        const float *from = a.partial + (size_t)(first + walk.s) * a.n_group * 2;
+        for (int g0 = 0; g0 < a.n_group; g0 += a.threads / width) {
+          const int g = g0 + t / width;
+          float u = 0.f, v = 0.f;
+          if (g < a.n_group)
+            for (int i = lane; i < many; i += width) {
+              const float2 p = *(const float2 *)(from + ((size_t)i * a.n_group + g) * 2);
+              u += p.x;
+              v += p.y;
+            }
+          for (int d = width / 2; d > 0; d >>= 1) u += __shfl_xor_sync(0xffffffffu, u, d), v += __shfl_xor_sync(0xffffffffu, v, d);
+          if (lane == 0 && g < a.n_group) {
+            const float m = 1.0f / ((float)(walk.hi - walk.lo) * (float)a.t.group_copies[g]);
+            gs[2 * g] = u * m;
+            gs[2 * g + 1] = v * m;
+          }
+        }
+        __syncthreads();
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int at = u * R + ty;
-#pragma unroll
-      for (int q = 0; q < VEC; ++q) {
-        if (gate[q] == -1) dz[u][q] *= slope[u][q];
-        else if (GATED && gate[q] >= 0) dz[u][q] *= gates[at * a.n_gate + gate[q]];
-        else if (GATED && !body) {
-          float s = 0.f;
-          for (int i = 0; i < len[q]; ++i) s += prods[at * a.c_out + first[q] + i];
-          dz[u][q] = row0 + at < k.hi ? s * slope[u][q] : 0.f;
+        for (int q = 0; q < VEC; ++q) {
+          s1[q] = centred >> q & 1 ? gs[2 * group[q]] : 0.f;
+          s2[q] = gs[2 * group[q] + 1];
+        }
+        if (GATED) {
+          g1 = gs[2 * gg];
+          g2 = gs[2 * gg + 1];
         }
       }
     }
-    if (GATED) __syncthreads();
-  }
-};
-
-// First pass, backward: sum of dz and of dz xhat of each channel of a chunk, as the groups' sums of a and a xhat and as the
-// chunk's share of the parameters' gradients.
-template <class T, int VEC, bool GATED>
-__global__ void __launch_bounds__(kGnThreads) gn_bwd_sums_kernel(GnArgs a) {
-  after_previous();
-  __shared__ Chunk shared;
-  extern __shared__ float sm[];                       // [R][c], [R][c]; before that the gates and products of GnBack
-  const Chunk k = find_chunk(a, blockIdx.x, &shared);
-  if (k.sample < 0) return;
-  const int R = blockDim.y, ty = threadIdx.y, ch = threadIdx.x * VEC;
-  GnBack<T, VEC, GATED> back;
-  back.setup(a, k, ch, sm);
-  float s1[VEC] = {}, s2[VEC] = {};
-  for (int row0 = k.lo; row0 < k.hi; row0 += 2 * R) {
-    float hat[2][VEC], dz[2][VEC];
-    back.rows(a, k, row0, ch, hat, dz);
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int q = 0; q < VEC; ++q) {
-        s1[q] += dz[u][q];
-        s2[q] = fmaf(dz[u][q], hat[u][q], s2[q]);
+    while (row < end) {
+      const char *stage = ring.tile(a);
+      const T *tile = (const T *)stage, *grad = (const T *)(stage + a.x_bytes);
+      const int first = ring.first, last = min(end, ring.end(a));
+      if (GATED && live) {
+        if (gr < GR)
+          for (int i = row - first + gr; i < last - first; i += GR) {
+            const float hat = ((float)tile[i * a.c + a.c_out + gj] - gmu) * gr_;
+            float z = fmaf(hat, gw, gb), slope, p = 0.f;
+            act_slopes<EXACT, 1>(&z, &slope, a.gate_act);
+            gates[i * a.n_gate + gj] = z;
+            for (int k = 0; k < flen; ++k) p = fmaf((float)tile[i * a.c + gf + k], (float)grad[i * a.c_out + gf + k], p);
+            const float dz = p * fr * slope;
+            if (SUMS) {
+              g1 += dz;
+              g2 = fmaf(dz, hat, g2);
+            } else {
+              ((T *)a.out)[(size_t)(first + i) * a.c + a.c_out + gj] = (T)(gr_ * (fmaf(dz, gw, -g1) - hat * g2));
+            }
+          }
+        __syncthreads();
       }
-  }
-  float *s2_s = sm + R * a.c;
+      if (works && live) {
+        for (int i = row - first + ty; i < last - first; i += 2 * R) {
+          float hat[2][VEC], dz[2][VEC];
+          const bool two = i + R < last - first;
+          const int at[2] = {i, two ? i + R : i};
 #pragma unroll
-  for (int q = 0; q < VEC; ++q) {
-    sm[ty * a.c + ch + q] = s1[q];
-    s2_s[ty * a.c + ch + q] = s2[q];
-  }
-  __syncthreads();
-  const int t = ty * blockDim.x + threadIdx.x, threads = blockDim.x * R;
-  for (int i = t; i < a.c; i += threads) {
-    float u = 0.f, v = 0.f;
-    for (int r = 0; r < R; ++r) u += sm[r * a.c + i], v += s2_s[r * a.c + i];
-    sm[i] = u;
-    s2_s[i] = v;
-  }
-  __syncthreads();
-  for (int f = t; f < a.n_field; f += threads) {
-    float *p = a.fields + (size_t)blockIdx.x * (a.n_field + a.n_scalar);
-    const int first = a.t.field_first[f], len = a.t.field_len[f], sc = a.t.field_scalar[f];
-    float v = 0.f;
-    for (int i = 0; i < len; ++i) v += s2_s[first + i];
-    p[f] = v;
-    if (sc >= 0) p[a.n_field + sc] = sm[first];
-  }
-  const int lane = t & 31, warps = threads >> 5;
-  if (t < warps * 32)
-    for (int g = t >> 5; g < a.n_group; g += warps) {
-      const int first = a.t.group_first[g], len = a.t.group_len[g];
-      float u = 0.f, v = 0.f;
-      for (int i = lane; i < len; i += 32) {
-        const float w = a.weight ? a.weight[a.t.field_of_channel[first + i]] : 1.f;
-        u = fmaf(w, sm[first + i], u);
-        v = fmaf(w, s2_s[first + i], v);
+          for (int u = 0; u < 2; ++u) {
+            load<T, VEC>(tile + at[u] * a.c + ch, hat[u]);
+            load<T, VEC>(grad + at[u] * a.c_out + ch, dz[u]);
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) hat[u][q] = (hat[u][q] - mu[q]) * r[q];
+          }
+          if (scalars) {
+            float z[2][VEC], slope[2][VEC];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int q = 0; q < VEC; ++q) z[u][q] = fmaf(hat[u][q], w[q], b[q]);
+            act_slopes<EXACT, 2 * VEC>(&z[0][0], &slope[0][0], a.scalar_act);
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int q = 0; q < VEC; ++q)
+                if (gate[q] == -1) dz[u][q] *= slope[u][q];
+          }
+          if (GATED) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int q = 0; q < VEC; ++q)
+                if (gate[q] >= 0) dz[u][q] *= gates[at[u] * a.n_gate + gate[q]];
+          }
+          if (SUMS) {
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) {
+              s1[q] += two ? dz[0][q] + dz[1][q] : dz[0][q];
+              s2[q] = fmaf(dz[0][q], hat[0][q], s2[q]);
+              if (two) s2[q] = fmaf(dz[1][q], hat[1][q], s2[q]);
+            }
+          } else {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+#pragma unroll
+              for (int q = 0; q < VEC; ++q) dz[u][q] = r[q] * (fmaf(dz[u][q], w[q], -s1[q]) - hat[u][q] * s2[q]);
+              if (u == 0 || two) store<T, VEC>(out + (size_t)(first + at[u]) * a.c, dz[u]);
+            }
+          }
+        }
       }
-      for (int d = 1; d < 32; d <<= 1) u += __shfl_xor_sync(0xffffffffu, u, d), v += __shfl_xor_sync(0xffffffffu, v, d);
-      if (lane == 0) {
-        float *p = a.partial + ((size_t)blockIdx.x * a.n_group + g) * 2;
-        p[0] = u;
-        p[1] = v;
+      if (!SUMS && !live)
+        for (long long i = (long long)row * a.c + t; i < (long long)last * a.c; i += a.threads) ((T *)a.out)[i] = (T)0.f;
+      ring.release(a, last);
+      if (GATED) gates = gates == gates0 ? gates + a.tile * a.n_gate : gates0;
+      row = last;
+    }
+    if (SUMS && live) {
+      float *second = sums + RS * a.c;
+      for (int i = t; i < 2 * RS * a.c; i += a.threads) sums[i] = 0.f;
+      __syncthreads();
+      if (works) {
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) {
+          sums[ty * a.c + ch + q] = s1[q];
+          second[ty * a.c + ch + q] = s2[q];
+        }
+      }
+      if (GATED && gr < GR) {
+        sums[gr * a.c + a.c_out + gj] = g1;
+        second[gr * a.c + a.c_out + gj] = g2;
+      }
+      __syncthreads();
+      for (int i = t; i < a.c; i += a.threads) {
+        float u = 0.f, v = 0.f;
+        for (int k = 0; k < RS; ++k) u += sums[k * a.c + i], v += second[k * a.c + i];
+        sums[i] = u;
+        second[i] = v;
+        tot[i] += u;
+        tot[a.c + i] += v;
+      }
+      __syncthreads();
+      const int lane = t & 31;
+      for (int g = t >> 5; g < a.n_group; g += a.threads >> 5) {
+        const int from = a.t.group_first[g], len = a.t.group_len[g];
+        float u = 0.f, v = 0.f;
+        for (int i = lane; i < len; i += 32) {
+          const float weight = a.weight ? a.weight[a.t.field_of_channel[from + i]] : 1.f;
+          u = fmaf(weight, sums[from + i], u);
+          v = fmaf(weight, second[from + i], v);
+        }
+        for (int d = 1; d < 32; d <<= 1) u += __shfl_xor_sync(0xffffffffu, u, d), v += __shfl_xor_sync(0xffffffffu, v, d);
+        if (lane == 0) *(float2 *)(a.partial + ((size_t)(block + walk.s) * a.n_group + g) * 2) = {u, v};
       }
     }
-}
-
-// Second pass, backward: dx.  The first blocks add up the parameters' gradients, kGnSum of them each.
-template <class T, int VEC, bool GATED>
-__global__ void __launch_bounds__(kGnThreads) gn_bwd_apply_kernel(GnArgs a, int sum_blocks) {
-  after_previous();
-  __shared__ Chunk shared;
-  extern __shared__ float sm[];                       // [n_group][2], gates and products; or [threads] sums
-  const int R = blockDim.y, ty = threadIdx.y, ch = threadIdx.x * VEC;
-  const int t = ty * blockDim.x + threadIdx.x, threads = blockDim.x * R;
-  const Chunk k = find_chunk(a, (int)blockIdx.x - sum_blocks, &shared);
-  if ((int)blockIdx.x < sum_blocks) {
-    const int cols = a.n_field + a.n_scalar, lanes = min(kGnSum, threads), parts = threads / lanes;
-    for (int c0 = blockIdx.x * kGnSum; c0 < min((int)(blockIdx.x + 1) * kGnSum, cols); c0 += lanes) {
-      const int col = c0 + t % lanes, part = t / lanes;
+    if (live) __syncthreads();
+    if (row < ring.r1) walk.place(a, row);
+  }
+  if (SUMS) {
+    __syncthreads();
+    float *p = a.fields + (size_t)block * (a.n_field + a.n_scalar);
+    for (int f = t; f < a.n_field; f += a.threads) {
+      const int from = a.t.field_first[f], len = a.t.field_len[f], sc = a.t.field_scalar[f];
       float v = 0.f;
-      if (part < parts && col < cols)
-        for (int i = part; i < shared.total; i += parts) v += a.fields[(size_t)i * cols + col];
-      __syncthreads();
-      sm[t] = v;
-      __syncthreads();
-      if (t < lanes && col < cols) {
-        for (int p = 1; p < parts; ++p) v += sm[p * lanes + t];
-        if (col < a.n_field) a.d_weight[col] = v;
-        else a.d_bias[col - a.n_field] = v;
-      }
-    }
-    return;
-  }
-  if (k.sample == -2) return;
-  T *out = (T *)a.out + ch;
-  if (k.sample < 0) {
-    const float zero[VEC] = {};
-    for (int row = k.lo + ty; row < k.hi; row += R) store<T, VEC>(out + (size_t)row * a.c, zero);
-    return;
-  }
-  const int lane = t & 31, warps = threads >> 5;
-  if (t < warps * 32)
-    for (int g = t >> 5; g < a.n_group; g += warps) {
-      float u = 0.f, v = 0.f;
-      for (int i = lane; i < k.chunks && k.first + i < a.max_chunks; i += 32) {
-        const float *p = a.partial + ((size_t)(k.first + i) * a.n_group + g) * 2;
-        u += p[0];
-        v += p[1];
-      }
-      for (int d = 1; d < 32; d <<= 1) u += __shfl_xor_sync(0xffffffffu, u, d), v += __shfl_xor_sync(0xffffffffu, v, d);
-      if (lane == 0) {
-        const float m = 1.0f / ((float)k.rows * (float)a.t.group_copies[g]);
-        sm[2 * g] = u * m;
-        sm[2 * g + 1] = v * m;
-      }
-    }
-  __syncthreads();
-  GnBack<T, VEC, GATED> back;
-  back.setup(a, k, ch, sm + 2 * a.n_group);
-  float s1[VEC], s2[VEC];
-#pragma unroll
-  for (int q = 0; q < VEC; ++q) {
-    const int g = a.t.group_of_channel[ch + q];
-    s1[q] = a.t.scalar_of_channel[ch + q] >= 0 ? sm[2 * g] : 0.f;
-    s2[q] = sm[2 * g + 1];
-  }
-  for (int row0 = k.lo; row0 < k.hi; row0 += 2 * R) {
-    float hat[2][VEC], dz[2][VEC];
-    back.rows(a, k, row0, ch, hat, dz);
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int row = row0 + u * R + ty;
-      if (row >= k.hi) continue;
-#pragma unroll
-      for (int q = 0; q < VEC; ++q) dz[u][q] = back.r[q] * (fmaf(dz[u][q], back.w[q], -s1[q]) - hat[u][q] * s2[q]);
-      store<T, VEC>(out + (size_t)row * a.c, dz[u]);
+      for (int i = 0; i < len; ++i) v += tot[a.c + from + i];
+      p[f] = v;
+      if (sc >= 0) p[a.n_field + sc] = tot[from];
     }
   }
+  ring.close(a);
 }
-
-struct GnShape {
-  int vec, tx, ty, chunk_rows, max_chunks;
-};
 
 int type_bytes(int type) { return type == SSC_PREC_FP32 ? 4 : 2; }
 
-// Chunks: about four blocks to an SM, at least eight rows to a thread.  (Halves and doubles of this were as fast or slower.)
-GnShape gn_shape(int n, int batch, int c, int vec) {
-  GnShape s;
-  s.vec = vec;
-  s.tx = c / vec;
-  s.ty = s.tx >= 256 ? 1 : 256 / s.tx;
-  const long long unit = 4ll * s.ty, want = ((long long)n + sm_count() * 4 - 1) / (sm_count() * 4);
-  long long rows = (want + unit - 1) / unit * unit;
-  if (rows < 2 * unit) rows = 2 * unit;
-  s.chunk_rows = (int)(rows < 1 << 30 ? rows : 1 << 30);
-  s.max_chunks = n / s.chunk_rows + batch + 2;
-  return s;
+// (eight channels of two rows with their gradients are more than a thread's registers)
+int gn_vec(int c, int c_out, int type, bool grads) {
+  int v = grads ? 4 : 16 / type_bytes(type);
+  while (v > 1 && (c % v || c_out % v)) v /= 2;
+  return v;
+}
+constexpr int kGnBlocks = 2;               // to an SM
+
+// Tiles of four rows to a thread, two where gradients come with them (8 to 16 KB, a multiple of 16 bytes); a ring of up to 88 KB.
+void gn_shape(GnArgs &a, int type, int vec, bool grads) {
+  const int bytes = a.c * type_bytes(type);
+  a.threads = a.c / vec > 256 || a.n_gate > 256 ? kGnThreads : 256;
+  const int rows = a.threads / (a.c / vec);
+  const long long slots = (long long)sm_count() * kGnBlocks;
+  int each = grads ? 2 : 4;
+  while ((rows * each * bytes) % 16 || (rows * each * a.c_out * type_bytes(type)) % 16) each *= 2;
+  a.tile = rows * each;
+  a.x_bytes = (uint32_t)align_up((size_t)a.tile * bytes, 128);
+  a.stage_bytes = a.x_bytes + (grads ? (uint32_t)align_up((size_t)a.tile * a.c_out * type_bytes(type), 128) : 0);
+  a.stages = (int)(90112 / a.stage_bytes);
+  if (a.stages > kGnStages) a.stages = kGnStages;
+  if (a.stages < 2) a.stages = 2;
+  const long long tiles = ((long long)a.n + a.tile - 1) / a.tile, per = (tiles + slots - 1) / slots;
+  a.range = (int)(per * a.tile);
+  a.blocks = (int)((tiles + per - 1) / per);
 }
 
-int gn_vec(int c, int c_out, int type, const void *x, const void *y, const void *z, int out_type) {
-  for (int v = 16 / type_bytes(type); v > 1; v /= 2) {
-    if (c % v || c_out % v) continue;
-    const uintptr_t in = (uintptr_t)v * type_bytes(type), out = (uintptr_t)v * type_bytes(out_type);
-    if (((uintptr_t)x | (uintptr_t)z) % in == 0 && (uintptr_t)y % out == 0) return v;
-  }
-  return 1;
-}
-
-// The partial results for any vector width: one channel a thread makes the most blocks.
-size_t gn_scratch(int n, int batch, int c, int n_group, int n_cols) {
-  int most = 0;
-  for (int v = 1; v <= 8; v *= 2)
-    if (c % v == 0 && c / v <= kGnThreads) {
-      const GnShape s = gn_shape(n, batch, c, v);
-      if (s.max_chunks > most) most = s.max_chunks;
-    }
-  return (size_t)most * (2 * (size_t)n_group + (size_t)n_cols) * sizeof(float) + 16;
+size_t gn_scratch(int batch, int n_group, int n_cols) {
+  const size_t blocks = (size_t)sm_count() * kGnBlocks;
+  return ((blocks + batch) * 2 * (size_t)n_group + blocks * (size_t)n_cols) * sizeof(float) + 16;
 }
 
 int gn_fill(GnArgs &a, const int32_t *table, const char *what) {
@@ -605,6 +746,7 @@ int gn_fill(GnArgs &a, const int32_t *table, const char *what) {
   SSC_REQUIRE(a.scalar_act >= 0 && a.scalar_act <= 4 && a.gate_act >= 0 && a.gate_act <= 4, "%s: unknown activation", what);
   SSC_REQUIRE(a.eps > 0.f, "%s: eps must be positive", what);
   SSC_REQUIRE(table && a.offsets && a.stats && (a.n == 0 || (a.x && a.out)), "%s: null pointer", what);
+  SSC_REQUIRE((((uintptr_t)a.x | (uintptr_t)a.gy | (uintptr_t)a.out) & 15) == 0, "%s: rows must start at a multiple of 16 bytes", what);
   const int32_t *p = table;
   a.t.group_of_channel = p; p += a.c;
   a.t.field_of_channel = p; p += a.c;
@@ -617,56 +759,54 @@ int gn_fill(GnArgs &a, const int32_t *table, const char *what) {
   a.t.group_first = p; p += a.n_group;
   a.t.group_len = p; p += a.n_group;
   a.t.group_copies = p;
+  a.alarm = alarm_word();
   return SSC_OK;
 }
 
 template <class T, class TO, int VEC>
-cudaError_t gn_fwd(const GnArgs &a, const GnShape &s, cudaStream_t st) {
-  const dim3 block(s.tx, s.ty), grid(s.max_chunks);
-  const size_t stats = 2 * (size_t)s.ty * a.c * sizeof(float);
-  const size_t room = (2 * (size_t)a.n_group + 8 * (size_t)s.ty * a.n_gate) * sizeof(float);
+cudaError_t gn_fwd(const GnArgs &a, cudaStream_t st) {
+  const dim3 block(a.threads), grid(a.blocks);
+  const size_t ring = (size_t)a.stages * a.stage_bytes, rows = a.threads / (a.c / VEC);
+  const size_t stats = ring + 2 * (rows + 1) * a.c * sizeof(float), room = ring + (2 * (size_t)a.n_group + 2 * (size_t)a.tile * a.n_gate) * sizeof(float);
   auto apply = a.n_gate ? gn_apply_kernel<T, TO, VEC, true> : gn_apply_kernel<T, TO, VEC, false>;
-  cudaError_t e;
-  if (stats > 49152 && (e = allow_smem((const void *)gn_stats_kernel<T, VEC>, stats)) != cudaSuccess) return e;
-  if (room > 49152 && (e = allow_smem((const void *)apply, room)) != cudaSuccess) return e;
-  if ((e = launch_ready(gn_stats_kernel<T, VEC>, grid, block, stats, st, a)) != cudaSuccess) return e;
-  return launch_ready(apply, grid, block, room, st, a);
+  cudaError_t e = allow_smem((const void *)gn_stats_kernel<T, VEC>, stats);
+  if (e == cudaSuccess) e = allow_smem((const void *)apply, room);
+  if (e == cudaSuccess) e = launch_ready(gn_stats_kernel<T, VEC>, grid, block, stats, st, a);
+  return e == cudaSuccess ? launch_ready(apply, grid, block, room, st, a) : e;
 }
 
 template <class T, int VEC>
-cudaError_t gn_bwd(const GnArgs &a, const GnShape &s, cudaStream_t st) {
-  const dim3 block(s.tx, s.ty);
-  const size_t gates = 2 * (size_t)s.ty * (a.n_gate ? a.n_gate + a.c_out : 0), sums = 2 * (size_t)s.ty * a.c;
-  const size_t first = (gates > sums ? gates : sums) * sizeof(float);
-  size_t second = 2 * (size_t)a.n_group + gates;
-  if (second < (size_t)s.tx * s.ty) second = (size_t)s.tx * s.ty;
-  second *= sizeof(float);
-  auto one = a.n_gate ? gn_bwd_sums_kernel<T, VEC, true> : gn_bwd_sums_kernel<T, VEC, false>;
-  auto two = a.n_gate ? gn_bwd_apply_kernel<T, VEC, true> : gn_bwd_apply_kernel<T, VEC, false>;
-  cudaError_t e;
-  if (first > 49152 && (e = allow_smem((const void *)one, first)) != cudaSuccess) return e;
-  if (second > 49152 && (e = allow_smem((const void *)two, second)) != cudaSuccess) return e;
+cudaError_t gn_bwd(const GnArgs &a, cudaStream_t st) {
+  const dim3 block(a.threads);
+  const size_t ring = (size_t)a.stages * a.stage_bytes;
+  size_t rows = a.threads / (a.c_out / VEC);
+  if (a.n_gate && rows < (size_t)kGnGateRows) rows = kGnGateRows;
+  const size_t gates = 2 * (size_t)a.tile * a.n_gate;
+  const size_t first = ring + (gates + 2 * (rows + 1) * a.c) * sizeof(float), second = ring + (gates + 2 * (size_t)a.n_group) * sizeof(float);
+  auto one = a.n_gate ? gn_bwd_kernel<T, VEC, true, true> : gn_bwd_kernel<T, VEC, false, true>;
+  auto two = a.n_gate ? gn_bwd_kernel<T, VEC, true, false> : gn_bwd_kernel<T, VEC, false, false>;
+  cudaError_t e = allow_smem((const void *)one, first);
+  if (e == cudaSuccess) e = allow_smem((const void *)two, second);
   const int sum_blocks = ceil_div(a.n_field + a.n_scalar, kGnSum);
-  if ((e = launch_ready(one, dim3(s.max_chunks), block, first, st, a)) != cudaSuccess) return e;
-  return launch_ready(two, dim3(s.max_chunks + sum_blocks), block, second, st, a, sum_blocks);
+  if (e == cudaSuccess) e = launch_ready(one, dim3(a.blocks), block, first, st, a, 0);
+  return e == cudaSuccess ? launch_ready(two, dim3(a.blocks + sum_blocks), block, second, st, a, sum_blocks) : e;
 }
 
 template <class T, class TO>
-cudaError_t gn_fwd_vec(const GnArgs &a, const GnShape &s, cudaStream_t st) {
-  switch (s.vec) {
-    case 8: if constexpr (sizeof(T) == 2) return gn_fwd<T, TO, 8>(a, s, st);
-    case 4: return gn_fwd<T, TO, 4>(a, s, st);
-    case 2: return gn_fwd<T, TO, 2>(a, s, st);
-    default: return gn_fwd<T, TO, 1>(a, s, st);
+cudaError_t gn_fwd_vec(const GnArgs &a, int vec, cudaStream_t st) {
+  switch (vec) {
+    case 8: if constexpr (sizeof(T) == 2) return gn_fwd<T, TO, 8>(a, st);
+    case 4: return gn_fwd<T, TO, 4>(a, st);
+    case 2: return gn_fwd<T, TO, 2>(a, st);
+    default: return gn_fwd<T, TO, 1>(a, st);
   }
 }
 template <class T>
-cudaError_t gn_bwd_vec(const GnArgs &a, const GnShape &s, cudaStream_t st) {
-  switch (s.vec) {
-    case 8: if constexpr (sizeof(T) == 2) return gn_bwd<T, 8>(a, s, st);
-    case 4: return gn_bwd<T, 4>(a, s, st);
-    case 2: return gn_bwd<T, 2>(a, s, st);
-    default: return gn_bwd<T, 1>(a, s, st);
+cudaError_t gn_bwd_vec(const GnArgs &a, int vec, cudaStream_t st) {
+  switch (vec) {
+    case 4: return gn_bwd<T, 4>(a, st);
+    case 2: return gn_bwd<T, 2>(a, st);
+    default: return gn_bwd<T, 1>(a, st);
   }
 }
 bool known_type(int t) { return t == SSC_PREC_FP32 || t == SSC_PREC_F16 || t == SSC_PREC_BF16; }
@@ -674,34 +814,35 @@ bool known_type(int t) { return t == SSC_PREC_FP32 || t == SSC_PREC_F16 || t == 
 }  // namespace
 }  // namespace ssc
 
-extern "C" size_t ssc_group_norm_scratch_bytes(int n, int batch, int c, int n_group, int n_field, int n_scalar) {
-  if (n < 0 || batch < 1 || c < 1 || n_group < 0 || n_field < 0 || n_scalar < 0) return 0;
-  return ssc::gn_scratch(n, batch, c, n_group, n_field + n_scalar);
+extern "C" size_t ssc_group_norm_scratch_bytes(int batch, int n_group, int n_field, int n_scalar) {
+  if (batch < 1 || n_group < 0 || n_field < 0 || n_scalar < 0) return 0;
+  return ssc::gn_scratch(batch, n_group, n_field + n_scalar);
 }
 
 extern "C" int ssc_group_norm_fwd(const void *x, int type, int n, int c, const int32_t *offsets, int batch, const int32_t *table, int n_field,
                                   int n_scalar, int n_group, int n_gate, const float *weight, const float *bias, float eps, int scalar_act, int gate_act,
-                                  void *out, int out_type, float *stats, void *scratch, size_t scratch_bytes, void *stream) {
+                                  void *out, int out_type, float *stats, int32_t *status, void *scratch, size_t scratch_bytes, void *stream) {
   using namespace ssc;
   SSC_REQUIRE(known_type(type) && known_type(out_type) && (type == out_type || type == SSC_PREC_FP32), "group_norm_fwd: unknown types");
   GnArgs a = {};
   a.x = x; a.out = out; a.n = n; a.c = c; a.c_out = c - n_gate; a.n_gate = n_gate; a.n_group = n_group; a.n_field = n_field; a.n_scalar = n_scalar;
   a.batch = batch; a.offsets = offsets; a.weight = weight; a.bias = bias; a.eps = eps; a.scalar_act = scalar_act; a.gate_act = gate_act; a.stats = stats;
+  a.status = status;
   if (int e = gn_fill(a, table, "group_norm_fwd")) return e;
   if (n == 0) return SSC_OK;
-  const GnShape s = gn_shape(n, batch, c, gn_vec(c, a.c_out, type, x, out, x, out_type));
-  SSC_REQUIRE(s.tx <= kGnThreads, "group_norm_fwd: %d channels, at most %d of this alignment", c, kGnThreads * s.vec);
-  a.chunk_rows = s.chunk_rows;
-  a.max_chunks = s.max_chunks;
-  if (scratch == nullptr || scratch_bytes < 2 * (size_t)s.max_chunks * n_group * sizeof(float)) return fail(SSC_ERR_SCRATCH, "group_norm_fwd: scratch too small");
+  const int vec = gn_vec(c, a.c_out, type, false);
+  SSC_REQUIRE(n_gate <= kGnThreads, "group_norm_fwd: %d gates, at most %d", n_gate, kGnThreads);
+  SSC_REQUIRE(c / vec <= kGnThreads, "group_norm_fwd: %d channels, at most %d of this divisibility", c, kGnThreads * vec);
+  gn_shape(a, type, vec, false);
+  if (scratch == nullptr || ((uintptr_t)scratch & 15) != 0 || scratch_bytes < gn_scratch(batch, n_group, 0)) return fail(SSC_ERR_SCRATCH, "group_norm_fwd: scratch too small");
   a.partial = (float *)scratch;
   const cudaStream_t st = as_stream(stream);
   cudaError_t e;
-  if (type == SSC_PREC_F16) e = gn_fwd_vec<__half, __half>(a, s, st);
-  else if (type == SSC_PREC_BF16) e = gn_fwd_vec<__nv_bfloat16, __nv_bfloat16>(a, s, st);
-  else if (out_type == SSC_PREC_F16) e = gn_fwd_vec<float, __half>(a, s, st);
-  else if (out_type == SSC_PREC_BF16) e = gn_fwd_vec<float, __nv_bfloat16>(a, s, st);
-  else e = gn_fwd_vec<float, float>(a, s, st);
+  if (type == SSC_PREC_F16) e = gn_fwd_vec<__half, __half>(a, vec, st);
+  else if (type == SSC_PREC_BF16) e = gn_fwd_vec<__nv_bfloat16, __nv_bfloat16>(a, vec, st);
+  else if (out_type == SSC_PREC_F16) e = gn_fwd_vec<float, __half>(a, vec, st);
+  else if (out_type == SSC_PREC_BF16) e = gn_fwd_vec<float, __nv_bfloat16>(a, vec, st);
+  else e = gn_fwd_vec<float, float>(a, vec, st);
   if (e != cudaSuccess) return fail(SSC_ERR_CUDA, "group_norm_fwd: %s", cudaGetErrorString(e));
   note_launches(2);
   SSC_CHECK_LAUNCH("group_norm_fwd");
@@ -710,14 +851,14 @@ extern "C" int ssc_group_norm_fwd(const void *x, int type, int n, int c, const i
 
 extern "C" int ssc_group_norm_bwd(const void *x, const void *gy, int type, int n, int c, const int32_t *offsets, int batch, const int32_t *table,
                                   int n_field, int n_scalar, int n_group, int n_gate, const float *weight, const float *bias, float eps, int scalar_act,
-                                  int gate_act, const float *stats, void *gx, float *d_weight, float *d_bias, void *scratch, size_t scratch_bytes,
-                                  void *stream) {
+                                  int gate_act, const float *stats, void *gx, float *d_weight, float *d_bias, int32_t *status, void *scratch,
+                                  size_t scratch_bytes, void *stream) {
   using namespace ssc;
   SSC_REQUIRE(known_type(type), "group_norm_bwd: unknown type");
   GnArgs a = {};
   a.x = x; a.gy = gy; a.out = gx; a.n = n; a.c = c; a.c_out = c - n_gate; a.n_gate = n_gate; a.n_group = n_group; a.n_field = n_field;
   a.n_scalar = n_scalar; a.batch = batch; a.offsets = offsets; a.weight = weight; a.bias = bias; a.eps = eps; a.scalar_act = scalar_act;
-  a.gate_act = gate_act; a.stats = const_cast<float *>(stats); a.d_weight = d_weight; a.d_bias = d_bias;
+  a.gate_act = gate_act; a.stats = const_cast<float *>(stats); a.d_weight = d_weight; a.d_bias = d_bias; a.status = status;
   if (int e = gn_fill(a, table, "group_norm_bwd")) return e;
   SSC_REQUIRE((n == 0 || gy) && d_weight && (n_scalar == 0 || d_bias), "group_norm_bwd: null pointer");
   const cudaStream_t st = as_stream(stream);
@@ -727,15 +868,15 @@ extern "C" int ssc_group_norm_bwd(const void *x, const void *gy, int type, int n
     if (e != cudaSuccess) return fail(SSC_ERR_CUDA, "group_norm_bwd: %s", cudaGetErrorString(e));
     return SSC_OK;
   }
-  const GnShape s = gn_shape(n, batch, c, gn_vec(c, a.c_out, type, x, gx, gy, type));
-  SSC_REQUIRE(s.tx <= kGnThreads, "group_norm_bwd: %d channels, at most %d of this alignment", c, kGnThreads * s.vec);
-  a.chunk_rows = s.chunk_rows;
-  a.max_chunks = s.max_chunks;
-  if (scratch == nullptr || scratch_bytes < (size_t)s.max_chunks * (2 * (size_t)n_group + n_field + n_scalar) * sizeof(float))
+  const int vec = gn_vec(c, a.c_out, type, true);
+  SSC_REQUIRE(n_gate <= kGnThreads, "group_norm_bwd: %d gates, at most %d", n_gate, kGnThreads);
+  SSC_REQUIRE(c / vec <= kGnThreads, "group_norm_bwd: %d channels, at most %d of this divisibility", c, kGnThreads * vec);
+  gn_shape(a, type, vec, true);
+  if (scratch == nullptr || ((uintptr_t)scratch & 15) != 0 || scratch_bytes < gn_scratch(batch, n_group, n_field + n_scalar))
     return fail(SSC_ERR_SCRATCH, "group_norm_bwd: scratch too small");
   a.partial = (float *)scratch;
-  a.fields = a.partial + 2 * (size_t)s.max_chunks * n_group;
-  cudaError_t e = type == SSC_PREC_F16 ? gn_bwd_vec<__half>(a, s, st) : type == SSC_PREC_BF16 ? gn_bwd_vec<__nv_bfloat16>(a, s, st) : gn_bwd_vec<float>(a, s, st);
+  a.fields = a.partial + 2 * ((size_t)a.blocks + batch) * n_group;
+  cudaError_t e = type == SSC_PREC_F16 ? gn_bwd_vec<__half>(a, vec, st) : type == SSC_PREC_BF16 ? gn_bwd_vec<__nv_bfloat16>(a, vec, st) : gn_bwd_vec<float>(a, vec, st);
   if (e != cudaSuccess) return fail(SSC_ERR_CUDA, "group_norm_bwd: %s", cudaGetErrorString(e));
   note_launches(2);
   SSC_CHECK_LAUNCH("group_norm_bwd");

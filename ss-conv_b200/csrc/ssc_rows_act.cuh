@@ -1,36 +1,52 @@
 // Activations of rows of scalars and their slopes: 0 identity, 1 relu, 2 sigmoid, 3 silu, 4 gelu (erf).
 //
-// EXACT: within a few steps of float32.  Otherwise for values that are rounded to 16 bits, by the approximate exponential (two
-// steps and |z| 2^-24 relative) and quotient.  The kind is the same for a whole launch, so the branch on it stands outside the loop over the values: inside
-// it cost five times the arithmetic (group norm with silu of 786432 rows of 128 in bf16: 427 us with it).
+// The special-function unit (sixteen lanes a cycle and SM) bounds sigmoids: an exponential and a reciprocal each would be 46 us for the 100 M values
+// of 786432 rows of 128.  So two of them share a reciprocal: 1 / d0 = d1 / (d0 d1).  The exponential is the approximate one, two
+// steps and |z| 2^-24 relative, in what is added to one.  EXACT: the correctly rounded reciprocal of the product; otherwise, for
+// values that are rounded to 16 bits, the approximate one.  Denominators end at 2^62 (the product stays finite): sigmoids below 2^-62
+// become that.
+// The kind is the same for a whole launch, so the branch on it stands outside the loop over the values: inside
+// it cost five times the arithmetic.
 #pragma once
 #include "ssc_act.cuh"
 
 namespace ssc {
 
-// Denominators beyond the quick reciprocal's end at its limit: results below 2^-125 become that.  (NaN stays.)
-template <bool EXACT>
-__device__ __forceinline__ float sigmoid(float z) {
-  if (!EXACT) return __fdividef(1.0f, 1.0f + __expf(-z));
-  const float d = 1.0f + expf(-z);
-  return quick_reciprocal(d > 0x1p125f ? 0x1p125f : d);
+template <bool EXACT, int N>
+__device__ __forceinline__ void sigmoids(const float *z, float *s) {
+  float d[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) d[i] = fminf(1.0f + __expf(-z[i]), 0x1p62f);      // (a number for NaN too: the neighbour keeps its value)
+#pragma unroll
+  for (int i = 0; i + 1 < N; i += 2) {
+    const float p = d[i] * d[i + 1];
+    float r;
+    if (EXACT) r = quick_reciprocal(p);
+    else asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(p));
+    s[i] = r * d[i + 1];
+    s[i + 1] = r * d[i];
+  }
+  if (N % 2 == 1) s[N - 1] = quick_reciprocal(d[N - 1]);
 }
 __device__ __forceinline__ float normal_share(float z) { return 0.5f * (1.0f + erff(z * 0.70710678118654752f)); }
 
 template <bool EXACT, int N>
 __device__ __forceinline__ void act_values(float *v, int kind) {
+  float s[N];
   switch (kind) {
     case 1:
 #pragma unroll
       for (int i = 0; i < N; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];
       break;
     case 2:
+      sigmoids<EXACT, N>(v, s);
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = sigmoid<EXACT>(v[i]);
+      for (int i = 0; i < N; ++i) v[i] = v[i] == v[i] ? s[i] : v[i];
       break;
     case 3:
+      sigmoids<EXACT, N>(v, s);
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] *= sigmoid<EXACT>(v[i]);
+      for (int i = 0; i < N; ++i) v[i] *= s[i];
       break;
     case 4:
 #pragma unroll
@@ -52,19 +68,20 @@ __device__ __forceinline__ void act_slopes(float *v, float *s, int kind) {
       }
       break;
     case 2:
+      sigmoids<EXACT, N>(v, s);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const float t = sigmoid<EXACT>(v[i]);
-        s[i] = t * (1.f - t);
-        v[i] = t;
+        v[i] = v[i] == v[i] ? s[i] : v[i];
+        s[i] = v[i] * (1.f - v[i]);
       }
       break;
     case 3:
+      sigmoids<EXACT, N>(v, s);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const float t = sigmoid<EXACT>(v[i]);
-        s[i] = t * fmaf(v[i], 1.f - t, 1.f);
-        v[i] *= t;
+        const float a = v[i] * s[i];
+        s[i] = fmaf(a, 1.f - s[i], s[i]);
+        v[i] = a;
       }
       break;
     // (the density (2 pi)^-1/2 exp(-z^2 / 2))

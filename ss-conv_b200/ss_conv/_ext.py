@@ -159,11 +159,11 @@ SIGNATURES = {
                            c_void_p, c_float, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "ssc_gate_bwd": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
                              c_void_p, c_void_p]),
-    "ssc_group_norm_scratch_bytes": (c_size_t, [c_int] * 6),
+    "ssc_group_norm_scratch_bytes": (c_size_t, [c_int] * 4),
     "ssc_group_norm_fwd": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
-                                   c_float, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
+                                   c_float, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "ssc_group_norm_bwd": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p,
-                                   c_void_p, c_float, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+                                   c_void_p, c_float, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "ssc_gated_ff_scratch_bytes": (c_size_t, [c_int] * 6),
     "ssc_gated_ff_fwd": (c_int, [c_void_p] + [c_int] * 5 + [c_void_p] * 5 + [c_int] + [c_void_p] * 3 + [c_size_t, c_void_p]),
     "ssc_gated_ff_bwd": (c_int, [c_void_p] * 2 + [c_int] * 5 + [c_void_p] * 3 + [c_int] + [c_void_p] * 7 + [c_size_t, c_void_p]),
@@ -1721,36 +1721,42 @@ def _on_device_of(call):
     return there
 
 
+def _aligned(t):
+    """t, contiguous and at an address the copy engine takes."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 @_on_device_of
 def group_norm_forward(x, offsets, layout, weight, bias, eps, codes, out_dtype):
     """(result [n, c_out], statistics [samples, groups, 2]); layout: the channel tables (groupnorm._Layout)."""
-    x, offsets = x.contiguous(), offsets.contiguous()
+    x, offsets = _aligned(x), offsets.contiguous()
     weight, bias = (p if p is None else p.detach().contiguous() for p in (weight, bias))
     n, batch, dev = x.shape[0], offsets.shape[0] - 1, x.device
     out = _empty((n, layout.c_out), out_dtype, dev)
     stats = _empty((batch, layout.n_group, 2), torch.float32, dev)
-    nbytes = int(lib().ssc_group_norm_scratch_bytes(n, batch, layout.c, layout.n_group, 0, 0))
+    nbytes = int(lib().ssc_group_norm_scratch_bytes(batch, layout.n_group, 0, 0))
     scratch = _empty(nbytes, torch.uint8, dev)
     _check(lib().ssc_group_norm_fwd(_p(x), ROW_TYPES[x.dtype], n, layout.c, _p(offsets, torch.int32), batch, _p(layout.table(dev)), layout.n_field,
                                     layout.n_scalar, layout.n_group, layout.n_gate, _p(weight, torch.float32), _p(bias, torch.float32), eps,
-                                    codes[0], codes[1], _p(out), ROW_TYPES[out_dtype], _p(stats), _p(scratch), nbytes, _stream()))
+                                    codes[0], codes[1], _p(out), ROW_TYPES[out_dtype], _p(stats), _p(status_word(dev)), _p(scratch), nbytes, _stream()))
     return out, stats
 
 
 @_on_device_of
 def group_norm_backward(x, gy, offsets, layout, weight, bias, eps, codes, stats):
     """(gx, d_weight [fields], d_bias [scalars]) of group_norm_forward at x and the gradient gy of its result."""
-    x, gy, offsets = x.contiguous(), gy.contiguous(), offsets.contiguous()
+    x, gy, offsets = _aligned(x), _aligned(gy), offsets.contiguous()
     weight, bias = (p if p is None else p.detach().contiguous() for p in (weight, bias))
     n, batch, dev = x.shape[0], offsets.shape[0] - 1, x.device
     gx = torch.empty_like(x)
     grads = _empty(layout.n_field + max(layout.n_scalar, 1), torch.float32, dev)
-    nbytes = int(lib().ssc_group_norm_scratch_bytes(n, batch, layout.c, layout.n_group, layout.n_field, layout.n_scalar))
+    nbytes = int(lib().ssc_group_norm_scratch_bytes(batch, layout.n_group, layout.n_field, layout.n_scalar))
     scratch = _empty(nbytes, torch.uint8, dev)
     _check(lib().ssc_group_norm_bwd(_p(x), _p(gy, x.dtype), ROW_TYPES[x.dtype], n, layout.c, _p(offsets, torch.int32), batch, _p(layout.table(dev)),
                                     layout.n_field, layout.n_scalar, layout.n_group, layout.n_gate, _p(weight, torch.float32),
                                     _p(bias, torch.float32), eps, codes[0], codes[1], _p(stats), _p(gx), _p(grads), _p(grads[layout.n_field:]),
-                                    _p(scratch), nbytes, _stream()))
+                                    _p(status_word(dev)), _p(scratch), nbytes, _stream()))
     return gx, grads[:layout.n_field], grads[layout.n_field:layout.n_field + layout.n_scalar]
 
 

@@ -75,6 +75,12 @@ CASES = [
     ([3, 4], [(2048, 0)], 4, None),
     ([900] * 33, [(16, 0)], 4, F.silu),                                 # more samples than lanes
     ([20000, 7], [(24, 0)], 2, torch.sigmoid),
+    ([70, 70], [(500, 0), (1, 1), (1, 0)], 1, GATE),                    # wide rows, one gate
+    ([9, 30], [(4, 0), (300, 1), (300, 0)], 4, (F.silu, torch.sigmoid)),    # more gates than 256
+    ([1] * 700, [(6, 0)], 3, None),
+    ([1, 500000], [(40, 0)], 5, F.silu),                                # rings that go round several times
+    ([150000, 2, 150001], [(8, 0), (4, 1), (4, 0)], 2, GATE),
+    ([3] * 40 + [0] * 40 + [500], [(5, 0), (1, 2), (1, 0)], 1, GATE),   # many pieces to a block, rows of no multiple of anything
 ]
 
 

@@ -40,14 +40,14 @@ def test_library_refuses_bad_arguments_of_the_norm():
     def forward(type=0, out_type=0, n=0, c=8, batch=1, fields=8, scalars=8, groups=2, gates=0, act=0, eps=1e-5, table=64):
         # (addresses that nothing reads: the call ends before its first launch)
         return L.ssc_group_norm_fwd(64, type, n, c, 64, batch, table, fields, scalars, groups, gates, None, None, eps, act, 0, 64, out_type, 64,
-                                    None, 0, None)
+                                    None, None, 0, None)
 
     assert forward() == 0                                               # no rows: nothing to do
     for bad in (dict(type=1), dict(type=2, out_type=0), dict(n=-1), dict(c=0), dict(batch=0), dict(fields=9), dict(scalars=9), dict(groups=0),
                 dict(gates=8), dict(act=5), dict(eps=0.0), dict(table=None)):
         assert forward(**bad) == 1, bad
     assert forward(n=5) == 3 and b"scratch" in L.ssc_last_error()
-    assert L.ssc_group_norm_scratch_bytes(-1, 1, 8, 2, 8, 8) == 0
+    assert L.ssc_group_norm_scratch_bytes(0, 2, 8, 8) == 0
 
 
 def test_feedforward_refusals():
