@@ -28,7 +28,7 @@ def _nvcc():
 
 
 def _newest_input():
-    files = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if not f.endswith(".cpp")] + [os.path.join(HERE, "..", "include", "ssconv_b200.h")]
+    files = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if not f.endswith(".cpp") and f != "ssc_host_rows.h"] + [os.path.join(HERE, "..", "include", "ssconv_b200.h")]
     return max(os.path.getmtime(f) for f in files if os.path.exists(f))
 
 
@@ -47,20 +47,21 @@ def bindings_current(inputs):
 
 def build_bindings(force=False):
     """ss_conv/_host.so: needs the headers of Python and torch, no GPU toolkit."""
-    inputs = [os.path.join(CSRC, "ssc_host.cpp"), os.path.join(HERE, "..", "include", "ssconv_b200.h")]
+    sources = [os.path.join(CSRC, "ssc_host.cpp"), os.path.join(CSRC, "ssc_host_rows.cpp")]
+    inputs = sources + [os.path.join(CSRC, "ssc_host_rows.h"), os.path.join(HERE, "..", "include", "ssconv_b200.h")]
     if not force and bindings_current(inputs):
         return BINDINGS
     import sysconfig
     import torch
     base = os.path.join(os.path.dirname(torch.__file__), "include")
     cuda = os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "include")
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", inputs[0], "-o", BINDINGS, "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared"] + sources + ["-o", BINDINGS, "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
            "-I" + base, "-I" + os.path.join(base, "torch", "csrc", "api", "include"), "-I" + sysconfig.get_paths()["include"], "-I" + cuda,
            "-L" + os.path.dirname(LIB), "-lssconv_b200", "-Wl,-rpath,$ORIGIN",
-           "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10"]
+           "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError("g++ failed on ssc_host.cpp:\n" + r.stderr[-6000:])
+        raise RuntimeError("g++ failed on the bindings:\n" + r.stderr[-6000:])
     os.makedirs(os.path.dirname(MADE_FOR), exist_ok=True)
     with open(MADE_FOR, "w") as f:
         f.write(_versions())

@@ -14,6 +14,7 @@
 #include <utility>
 
 #include "../../include/ssconv_b200.h"
+#include "ssc_host_rows.h"
 
 namespace {
 
@@ -220,6 +221,9 @@ PyObject *head(PyObject *, PyObject *const *args, Py_ssize_t n) {
 PyMethodDef methods[] = {{"ptr", (PyCFunction)(void (*)())ptr, METH_FASTCALL, "device pointer of a contiguous CUDA tensor"},
                          {"empty", (PyCFunction)(void (*)())empty, METH_FASTCALL, "torch.empty(shape, dtype, device)"},
                          {"head", (PyCFunction)(void (*)())head, METH_FASTCALL, "tensor[:n]"},
+                         {"group_norm", (PyCFunction)(void (*)())ssc_py_group_norm, METH_FASTCALL, "group norm of ragged samples, recorded by autograd"},
+                         {"gated_ff", (PyCFunction)(void (*)())ssc_py_gated_ff, METH_FASTCALL, "gated feed-forward of rows, recorded by autograd"},
+                         {"row_operators", (PyCFunction)(void (*)())ssc_py_row_operators, METH_FASTCALL, "the functions behind the two"},
                          SSC_FUNCTIONS{nullptr, nullptr, 0, nullptr}};
 #undef X
 

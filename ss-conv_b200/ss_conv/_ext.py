@@ -10,7 +10,6 @@ variants of convolution and pools); only the functions the reference's own Pytho
 (indice_field_maxpool_*, voxelize_idx, point_recover_*) and the 2-D rulebooks raise NotImplementedError.
 """
 import ctypes
-import functools
 import os
 import threading
 
@@ -1706,84 +1705,44 @@ def gate_backward(x, gy, c_out, gate_of_channel, field_start, field_len, scalar_
     return gx
 
 
-# ================================================================ group norm
-ROW_TYPES = {torch.float32: PREC_FP32, torch.float16: PREC_F16, torch.bfloat16: PREC_BF16}
+# ================================================================ row operators: group norm, gated feed-forward
+
+def _row_operator(name):
+    """The autograd node `name` of the bindings (csrc/ssc_host_rows.cpp); with another build of the library behind it where
+    SSCONV_B200_LIB names one."""
+    global _rows_bound
+    L = lib()
+    if _host is None:
+        raise RuntimeError("the row operators need the bindings _host.so (%s): run `python ss-conv_b200/build.py`" % (_host_error,))
+    if L is not _host and not _rows_bound:
+        _host.row_operators(*(ctypes.cast(getattr(L, f), c_void_p).value for f in (
+            "ssc_last_error", "ssc_group_norm_scratch_bytes", "ssc_group_norm_fwd", "ssc_group_norm_bwd", "ssc_gated_ff_scratch_bytes",
+            "ssc_gated_ff_fwd", "ssc_gated_ff_bwd")))
+        _rows_bound = True
+    return getattr(_host, name)
 
 
-def _on_device_of(call):
-    """The call with its first argument's device as the current one: launches and streams are the current device's."""
-    @functools.wraps(call)
-    def there(t, *args):
-        if t.device.index == torch._C._cuda_getDevice():
-            return call(t, *args)
-        with torch.cuda.device(t.device):
-            return call(t, *args)
-    return there
+_rows_bound = False
 
 
-def _aligned(t):
-    """t, contiguous and at an address the copy engine takes."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+def _row_status(x):
+    return status_word(x.device) if x.is_cuda else None
 
 
-@_on_device_of
-def group_norm_forward(x, offsets, layout, weight, bias, eps, codes, out_dtype):
-    """(result [n, c_out], statistics [samples, groups, 2]); layout: the channel tables (groupnorm._Layout)."""
-    x, offsets = _aligned(x), offsets.contiguous()
-    weight, bias = (p if p is None else p.detach().contiguous() for p in (weight, bias))
-    n, batch, dev = x.shape[0], offsets.shape[0] - 1, x.device
-    out = _empty((n, layout.c_out), out_dtype, dev)
-    stats = _empty((batch, layout.n_group, 2), torch.float32, dev)
-    nbytes = int(lib().ssc_group_norm_scratch_bytes(batch, layout.n_group, 0, 0))
-    scratch = _empty(nbytes, torch.uint8, dev)
-    _check(lib().ssc_group_norm_fwd(_p(x), ROW_TYPES[x.dtype], n, layout.c, _p(offsets, torch.int32), batch, _p(layout.table(dev)), layout.n_field,
-                                    layout.n_scalar, layout.n_group, layout.n_gate, _p(weight, torch.float32), _p(bias, torch.float32), eps,
-                                    codes[0], codes[1], _p(out), ROW_TYPES[out_dtype], _p(stats), _p(status_word(dev)), _p(scratch), nbytes, _stream()))
-    return out, stats
-
-
-@_on_device_of
-def group_norm_backward(x, gy, offsets, layout, weight, bias, eps, codes, stats):
-    """(gx, d_weight [fields], d_bias [scalars]) of group_norm_forward at x and the gradient gy of its result."""
-    x, gy, offsets = _aligned(x), _aligned(gy), offsets.contiguous()
-    weight, bias = (p if p is None else p.detach().contiguous() for p in (weight, bias))
-    n, batch, dev = x.shape[0], offsets.shape[0] - 1, x.device
-    gx = torch.empty_like(x)
-    grads = _empty(layout.n_field + max(layout.n_scalar, 1), torch.float32, dev)
-    nbytes = int(lib().ssc_group_norm_scratch_bytes(batch, layout.n_group, layout.n_field, layout.n_scalar))
-    scratch = _empty(nbytes, torch.uint8, dev)
-    _check(lib().ssc_group_norm_bwd(_p(x), _p(gy, x.dtype), ROW_TYPES[x.dtype], n, layout.c, _p(offsets, torch.int32), batch, _p(layout.table(dev)),
-                                    layout.n_field, layout.n_scalar, layout.n_group, layout.n_gate, _p(weight, torch.float32),
-                                    _p(bias, torch.float32), eps, codes[0], codes[1], _p(stats), _p(gx), _p(grads), _p(grads[layout.n_field:]),
-                                    _p(status_word(dev)), _p(scratch), nbytes, _stream()))
-    return gx, grads[:layout.n_field], grads[layout.n_field:layout.n_field + layout.n_scalar]
-
-
-# ================================================================ gated feed-forward
-@_on_device_of
-def gated_ff_forward(x, w_in, w_out, b_in, b_out, residual, act):
-    """(act(x w_in[0]' + b_in[0]) * (x w_in[1]' + b_in[1])) w_out' + b_out (+ residual); contiguous tensors of one type."""
-    n, (c_out, hidden), dev, kind = x.shape[0], w_out.shape, x.device, ROW_TYPES[x.dtype]
-    out = _empty((n, c_out), x.dtype, dev)
-    nbytes = int(lib().ssc_gated_ff_scratch_bytes(kind, n, x.shape[1], hidden, c_out, 0))
-    scratch = _empty(nbytes, torch.uint8, dev)
-    _check(lib().ssc_gated_ff_fwd(_p(x), kind, n, x.shape[1], hidden, c_out, _p(w_in), _p(w_out), _p(b_in), _p(b_out), _p(residual), act,
-                                  _p(out), _p(status_word(dev)), _p(scratch), nbytes, _stream()))
+def group_norm(x, offsets, layout, weight, bias, eps, codes, out_dtype=None):
+    """act(norm(x)) [n, c_out], recorded by autograd; layout: the channel tables (groupnorm._Layout)."""
+    out = _row_operator("group_norm")(x, weight, bias, offsets, layout.table(x.device), _row_status(x), layout.sizes, eps, *codes, out_dtype or x.dtype)
+    if _alarm is not None and _alarm.value:
+        _raise_on_alarm()
     return out
 
 
-@_on_device_of
-def gated_ff_backward(x, gy, w_in, w_out, b_in, act, need):
-    """(gx, gw_in, gw_out, gb_in, gb_out), None where `need` says so."""
-    n, (c_out, hidden), dev, kind = x.shape[0], w_out.shape, x.device, ROW_TYPES[x.dtype]
-    shapes = (x.shape, w_in.shape, w_out.shape, (2, hidden), (c_out,))
-    grads = [_empty(tuple(s), x.dtype, dev) if k else None for s, k in zip(shapes, need)]
-    nbytes = int(lib().ssc_gated_ff_scratch_bytes(kind, n, x.shape[1], hidden, c_out, 1))
-    scratch = _empty(nbytes, torch.uint8, dev)
-    _check(lib().ssc_gated_ff_bwd(_p(x), _p(gy, x.dtype), kind, n, x.shape[1], hidden, c_out, _p(w_in), _p(w_out), _p(b_in), act,
-                                  *(_p(g) for g in grads), _p(status_word(dev)), _p(scratch), nbytes, _stream()))
-    return grads
+def gated_ff(x, w_in, w_out, b_in, b_out, residual, act):
+    """(act(x w_in[0]' + b_in[0]) * (x w_in[1]' + b_in[1])) w_out' + b_out (+ residual), recorded by autograd."""
+    out = _row_operator("gated_ff")(x, w_in, w_out, b_in, b_out, residual, _row_status(x), act)
+    if _alarm is not None and _alarm.value:
+        _raise_on_alarm()
+    return out
 
 
 def scatter_add_rate(out, rows, steps, lanes_per_row=8, warps_per_sm=16):

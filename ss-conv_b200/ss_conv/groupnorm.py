@@ -10,7 +10,6 @@ import itertools
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from . import _ext
 from .activation import _act_code
@@ -71,6 +70,7 @@ class _Layout(object):
         spread = lambda v: [x for x, d in zip(v, dims) for _ in range(d)]  # noqa: E731
         self.rows = (spread(group_of_field) + spread(range(self.n_field)) + spread(slots) + gates + first + dims + slots
                      + gate_field + group_first + group_len + copies)
+        self.sizes = (self.c, self.n_field, self.n_scalar, self.n_group, self.n_gate)
         self.tables = {}
 
     def table(self, device):
@@ -87,44 +87,13 @@ def _layout(Rs, groups, gated, scalar_act):
     return _Layout(Rs, groups, gated, scalar_act)
 
 
-class _GroupNormFn(torch.autograd.Function):
-    """Saves the rows and the statistics; everything between is computed again on the way back."""
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, offsets, layout, eps, codes):
-        y, stats = _ext.group_norm_forward(x, offsets, layout, weight, bias, eps, codes, x.dtype)
-        ctx.save_for_backward(x, weight, bias, offsets, stats)
-        ctx.layout, ctx.eps, ctx.codes = layout, eps, codes
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, gy):
-        x, weight, bias, offsets, stats = ctx.saved_tensors
-        gx, gw, gb = _ext.group_norm_backward(x, gy, offsets, ctx.layout, weight, bias, ctx.eps, ctx.codes, stats)
-        need = ctx.needs_input_grad
-        return gx, gw if need[1] else None, gb if need[2] else None, None, None, None, None
-
-
-def _normed(x, offsets, layout, weight, bias, eps, codes, out_dtype=None):
-    if not x.is_cuda:
-        raise RuntimeError("ssconv_b200 runs on CUDA tensors only (got a %s tensor)" % x.device.type)
-    if x.dim() != 2 or x.shape[1] != layout.c:
-        raise ValueError("features must be [n, %d] (got %s)" % (layout.c, tuple(x.shape)))
-    if x.dtype not in _ext.ROW_TYPES:
-        raise TypeError("features must be float32, float16 or bfloat16 (got %s)" % x.dtype)
-    if offsets.dim() != 1 or offsets.shape[0] < 2 or offsets.dtype != torch.int32 or offsets.device != x.device:
-        raise ValueError("offsets must be int32 [samples + 1] on %s (got %s %s on %s)" % (x.device, offsets.dtype, tuple(offsets.shape),
-                                                                                      offsets.device))
-    for name, p, size in (("weight", weight, layout.n_field), ("bias", bias, layout.n_scalar)):
-        if p is not None and (p.shape != (size,) or p.device != x.device or not p.is_floating_point()):
-            raise ValueError("%s must hold %d floating point values on %s (got %s %s on %s)" % (name, size, x.device, p.dtype,
-                                                                                            tuple(p.shape), p.device))
-    weight, bias = (p if p is None or p.dtype == torch.float32 else p.float() for p in (weight, bias))
-    if torch.is_grad_enabled() and (x.requires_grad or any(p is not None and p.requires_grad for p in (weight, bias))):
-        y = _GroupNormFn.apply(x, weight, bias, offsets, layout, eps, codes)
-        return y if out_dtype in (None, x.dtype) else y.to(out_dtype)
-    return _ext.group_norm_forward(x, offsets, layout, weight, bias, eps, codes, out_dtype or x.dtype)[0]
+@functools.lru_cache(maxsize=256)
+def _plan(Rs, groups, activation):
+    """(channel tables, activation codes) of group_norm's arguments."""
+    scalar, gate = activation if isinstance(activation, tuple) else (activation, activation)
+    gated = gate is not None and any(l > 0 and m > 0 for m, l in Rs)
+    codes = (act_code(scalar), act_code(gate) if gated else 0)
+    return _layout(Rs, int(groups), gated, codes[0] != 0), codes
 
 
 def group_norm(features, offsets, Rs, num_groups=1, weight=None, bias=None, eps=1e-5, activation=None):
@@ -136,13 +105,10 @@ def group_norm(features, offsets, Rs, num_groups=1, weight=None, bias=None, eps=
     Activation; with a gate and fields of order l > 0 the last entry of Rs holds one gate scalar for each of them, and
     the result has the channels before it.  relu, sigmoid, silu, gelu or None.  Statistics and parameters are float32, the
     result has the type of the rows; rows of no sample (outside the offsets) come out as zeros."""
-    scalar, gate = activation if isinstance(activation, tuple) else (activation, activation)
-    Rs = tuple((int(m), int(l)) for m, l in Rs)
-    gated = gate is not None and any(l > 0 and m > 0 for m, l in Rs)
-    codes = (act_code(scalar), act_code(gate) if gated else 0)
     if not eps > 0:
         raise ValueError("eps must be positive (got %r)" % (eps,))
-    return _normed(features, offsets, _layout(Rs, int(num_groups), gated, codes[0] != 0), weight, bias, float(eps), codes)
+    layout, codes = _plan(tuple(map(tuple, Rs)), num_groups, activation)
+    return _ext.group_norm(features, offsets, layout, weight, bias, eps, codes)
 
 
 class GroupNorm(nn.Module):
@@ -152,10 +118,7 @@ class GroupNorm(nn.Module):
     def __init__(self, Rs, num_groups=1, eps=1e-5, affine=True, activation=None):
         super().__init__()
         self.Rs, self.num_groups, self.eps, self.affine, self.activation = [(int(m), int(l)) for m, l in Rs], int(num_groups), eps, affine, activation
-        scalar, gate = activation if isinstance(activation, tuple) else (activation, activation)
-        gated = gate is not None and any(l > 0 and m > 0 for m, l in self.Rs)
-        act_code(scalar), act_code(gate) if gated else None
-        layout = _layout(tuple(self.Rs), self.num_groups, gated, scalar is not None)
+        layout = _plan(tuple(self.Rs), self.num_groups, activation)[0]
         if affine:
             self.weight = nn.Parameter(torch.ones(layout.n_field))
             self.bias = nn.Parameter(torch.zeros(layout.n_scalar))
@@ -191,7 +154,7 @@ class GroupNorm(nn.Module):
             out = f.dtype
             if out == torch.float32 and not torch.is_grad_enabled():
                 out = _ext._stored_type(f.shape[0], layout.c, layout.c_out, layout.c_out, _ext.get_feature_storage()) or out
-            return _normed(f, offsets, layout, self.weight, self.bias, float(self.eps), codes, out)
+            return _ext.group_norm(f, offsets, layout, self.weight, self.bias, self.eps, codes, out)
 
         return self._apply_to(input, rows)
 

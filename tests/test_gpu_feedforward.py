@@ -135,6 +135,32 @@ def test_some_gradients_alone_and_differences(cuda):
         assert abs(num.item() - flat[at].item()) <= 1e-2 * max(1.0, abs(flat[at].item())), name
 
 
+def test_every_choice_of_gradients(cuda):
+    """Arguments that are absent, and those that ask for no gradient, in all combinations: each gradient is its own argument's."""
+    import itertools
+    from ss_conv.feedforward import gated_feedforward
+    t, gy = inputs(70, 16, 24, 8, torch.float32, True, True, 9)
+    names = list(t)
+    full = {k: v.to(cuda).requires_grad_(True) for k, v in t.items()}
+    for there in itertools.product((False, True), repeat=3):
+        absent = [n for n, on in zip(("b_in", "b_out", "residual"), there) if not on]
+        use = {k: (None if k in absent else v) for k, v in full.items()}
+        y = gated_feedforward(use["x"], use["w_in"], use["w_out"], use["b_in"], use["b_out"], F.silu, use["residual"])
+        have = [k for k in names if use[k] is not None]
+        want = dict(zip(have, torch.autograd.grad(y, [use[k] for k in have], gy.to(cuda))))
+        for asks in itertools.product((False, True), repeat=len(have)):
+            if not any(asks):
+                continue
+            ask = [k for k, on in zip(have, asks) if on]
+            leaf = {k: None if use[k] is None else use[k].detach().requires_grad_(k in ask) for k in names}
+            y = gated_feedforward(leaf["x"], leaf["w_in"], leaf["w_out"], leaf["b_in"], leaf["b_out"], F.silu, leaf["residual"])
+            for k, g in zip(ask, torch.autograd.grad(y, [leaf[k] for k in ask], gy.to(cuda))):
+                assert torch.equal(g, want[k]), (absent, ask, k)
+    y = gated_feedforward(full["x"], full["w_in"], full["w_out"])
+    with pytest.raises(RuntimeError, match="gradients of gradients"):
+        torch.autograd.grad(y.sum(), [full["x"]], create_graph=True)
+
+
 def test_not_finite_rows_stay_their_own(cuda):
     from ss_conv.feedforward import gated_feedforward
     for n in (8, 300):

@@ -186,6 +186,27 @@ def test_same_bits_every_time_and_in_any_batch(cuda):
     assert all(torch.equal(a, b) for a, b in zip(*runs))
 
 
+def test_parameters_one_by_one(cuda):
+    """Without weight or bias, with either frozen: each gradient is its own parameter's; parameters in 16 bits."""
+    from ss_conv.groupnorm import group_norm
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(50, 12, generator=g).to(cuda)
+    off = torch.tensor([0, 20, 50], dtype=torch.int32, device=cuda)
+    w, b = (torch.randn(12, generator=g).to(cuda).requires_grad_(True) for _ in range(2))
+    gy = torch.randn(50, 12, generator=g).to(cuda)
+    call = lambda w, b: group_norm(x, off, [(12, 0)], 3, w, b, activation=F.silu)  # noqa: E731
+    gw, gb = torch.autograd.grad(call(w, b), [w, b], gy)
+    assert torch.equal(torch.autograd.grad(call(w.detach(), b), [b], gy)[0], gb)
+    assert torch.equal(torch.autograd.grad(call(w, b.detach()), [w], gy)[0], gw)
+    ones, zeros = torch.ones(12, device=cuda).requires_grad_(True), torch.zeros(12, device=cuda).requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(call(None, b), [b], gy)[0], torch.autograd.grad(call(ones, b), [b], gy)[0])
+    assert torch.equal(torch.autograd.grad(call(w, None), [w], gy)[0], torch.autograd.grad(call(w, zeros), [w], gy)[0])
+    half = w.detach().half().requires_grad_(True)
+    assert torch.autograd.grad(call(half, b), [half], gy)[0].dtype == torch.float16
+    with pytest.raises(RuntimeError, match="gradients of gradients"):
+        torch.autograd.grad(call(w, b).sum(), [w], create_graph=True)
+
+
 def test_strided_rows_a_side_stream_and_a_graph(cuda):
     from ss_conv.groupnorm import group_norm
     g = torch.Generator().manual_seed(9)
