@@ -26,7 +26,11 @@ constexpr int kTileM = 128;
 constexpr int kStageBoxes = 6;                // two of A, up to four of B
 constexpr uint32_t kStageBytes = kStageBoxes * kBoxBytes;
 constexpr int kStages = 4;
-constexpr int kThreads = 384;                 // TMA, products, tensor memory, one idle warp, eight for the accumulators
+// Warps: TMA, products, tensor memory, an idle one, then those for the accumulators: sixteen (eight where float32 sums need the registers).
+template <class T>
+constexpr int kSides = sizeof(T) == 4 ? 2 : 4;              // shares of a tile's columns
+template <class T>
+constexpr int kThreads = 128 + 128 * kSides<T>;
 constexpr uint32_t kSmemBytes = kStages * kStageBytes + 1024;
 
 enum Epilogue { kGate, kBack, kRows, kPart };
@@ -56,7 +60,7 @@ struct FfParams {
   void *out, *out2;                            // kGate: h; kBack: h, dg|du; kRows: result; kPart: float [splits][rows of all][cols]
   int pitch;                                   // of out
   size_t plane, plane2;                        // elements from one plane to the next (of out, of a matrix of out2)
-  int vec;                                     // rows of out (and residual) are aligned to 16 bytes
+  int vec;                                     // rows of out (and residual) are aligned to 32 bytes
   int accumulate;                              // kPart: add to what is there
   int32_t *status, *alarm;
 };
@@ -73,16 +77,21 @@ __device__ __forceinline__ uint32_t operand_lo(uint32_t addr, int mn) { return (
 
 __constant__ const int8_t kPlaneA[6] = {2, 0, 1, 1, 0, 0}, kPlaneB[6] = {0, 2, 1, 0, 1, 0};
 
+// A whole sector of L2 in one store: two halves of 16 bytes cost four times as much (gate and up of 65536 rows 256 -> 1024 in bf16: 119 us).
+__device__ __forceinline__ void store32(void *p, const uint32_t *v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
 template <class T>
 __device__ __forceinline__ void put16(T *p, const float *v, int left, int vec) {
   if (vec && left >= 16) {
-    constexpr int N = 16 / sizeof(T);
+    constexpr int N = 32 / sizeof(T);
 #pragma unroll
     for (int i = 0; i < 16; i += N) {
       struct alignas(16) { T v[N]; } k;
 #pragma unroll
       for (int q = 0; q < N; ++q) k.v[q] = (T)v[i + q];
-      *(int4 *)(p + i) = *(const int4 *)&k;
+      store32(p + i, (const uint32_t *)&k);
     }
   } else {
 #pragma unroll
@@ -207,7 +216,7 @@ __device__ __forceinline__ void finish(const FfParams &p, int split, int half_m,
 }
 
 template <int EPI, class T>
-__global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_constant__ FfMaps maps, const FfParams p) {
+__global__ void __launch_bounds__(kThreads<T>, 1) ff_gemm_kernel(const __grid_constant__ FfMaps maps, const FfParams p) {
   after_previous();
   extern __shared__ uint8_t raw[];
   __shared__ alignas(8) uint64_t bars[2 * kStages + 5];
@@ -223,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(acc_full + 8 * b, 1);
-      mbar_init(acc_empty + 8 * b, 8);
+      mbar_init(acc_empty + 8 * b, 4 * kSides<T>);
     }
     mbar_init(done, 1);
     abort_flag = 0;
@@ -240,60 +249,60 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
 
   if (warp == 0) {
     // operands
-    const bool one = elect_one();
-    uint32_t step = 0;
+    uint32_t slot = 0, phase = 1, step = 0;
     bool ok = true;
     for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
       const Tile k = tile_of(p, t);
       const int half_m = k.m >= p.m_half ? 1 : 0, m0 = (k.m - half_m * p.m_half) * kTileM, n0 = k.n * p.step_n;
       const int parts = parts_of(p, k);
-      for (int part = 0; part < parts && ok; ++part)
-        for (int g = 0; g < p.n_seg && ok; ++g) {
+      for (int part = 0; part < parts; ++part)
+        for (int g = 0; g < p.n_seg; ++g) {
           const Segment &s = p.seg[g];
           const int kb0 = split_begin(s.blocks, k.split, p.splits), blocks = split_begin(s.blocks, k.split + 1, p.splits) - kb0;
           if (part >= part_count(blocks, p.pairs)) continue;
           const uint32_t bytes = (2 + s.boxes_b) * kBoxBytes;
           const int per = s.b_half == kByBox ? s.boxes_b / 2 : s.boxes_b, end = part_begin(blocks, p.pairs, part + 1);
+          const CUtensorMap *map_a = &maps.a[g], *map_b = &maps.b[g];
           int i = part_begin(blocks, p.pairs, part), pair = blocks > 0 ? i / blocks : 0, kb = kb0 + i - pair * blocks;
-          for (; i < end; ++i, ++step) {
-            const uint32_t slot = step % kStages, turn = step / kStages;
-            ok = mbar_wait_uniform(empty + 8 * slot, (turn & 1) ^ 1, &abort_flag);
-            if (!ok) break;
-            if (one) {
-              const int pa = p.pairs == 1 ? 0 : kPlaneA[pair], pb = p.pairs == 1 ? 0 : kPlaneB[pair];
-              const uint32_t at = ring + slot * kStageBytes, bar = full + 8 * slot;
+          for (; i < end && ok; ++i, ++step) {
+            ok = mbar_wait_straight(empty + 8 * slot, phase, &abort_flag);
+            const int pa = p.pairs == 1 ? 0 : kPlaneA[pair], pb = p.pairs == 1 ? 0 : kPlaneB[pair];
+            const uint32_t at = ring + slot * kStageBytes, bar = full + 8 * slot;
+            const int by_k = kb >= s.half_blocks ? 1 : 0, kk = (kb - by_k * s.half_blocks) * kBox;
+            const int za = pa * s.a_planes + (s.a_half == kByK ? by_k : s.a_half == kByM ? half_m : 0), zb = pb * s.b_planes + (s.b_half == kByK ? by_k : 0);
+            if (ok && elect_one()) {
               mbar_expect_tx(bar, bytes);
-              const int by_k = kb >= s.half_blocks ? 1 : 0, kk = (kb - by_k * s.half_blocks) * kBox;
-              const int za = pa * s.a_planes + (s.a_half == kByK ? by_k : s.a_half == kByM ? half_m : 0);
-              for (int j = 0; j < 2; ++j) {
-                const int m = m0 + j * kBox;
-                tma_box(at + j * kBoxBytes, &maps.a[g], s.a_mn ? m : kk, s.a_mn ? kk : m, za, bar);
+              if (s.a_mn) {
+                tma_box(at, map_a, m0, kk, za, bar);
+                tma_box(at + kBoxBytes, map_a, m0 + kBox, kk, za, bar);
+              } else {
+                tma_box(at, map_a, kk, m0, za, bar);
+                tma_box(at + kBoxBytes, map_a, kk, m0 + kBox, za, bar);
               }
               for (int j = 0; j < s.boxes_b; ++j) {
-                const int h = j / per, n = n0 + (j - h * per) * kBox, zb = pb * s.b_planes + (s.b_half == kByK ? by_k : h);
-                tma_box(at + (2 + j) * kBoxBytes, &maps.b[g], s.b_mn ? n : kk, s.b_mn ? kk : n, zb, bar);
+                const int h = j >= per ? 1 : 0, n = n0 + (j - h * per) * kBox;
+                tma_box(at + (2 + j) * kBoxBytes, map_b, s.b_mn ? n : kk, s.b_mn ? kk : n, zb + h, bar);
               }
             }
+            if (++slot == kStages) slot = 0, phase ^= 1;
             if (++kb == kb0 + blocks) kb = kb0, ++pair;
           }
         }
     }
-    if (!ok)      // copies in flight arrive before the block leaves
+    if (abort_flag)      // copies in flight arrive before the block leaves
       for (uint32_t s = step > kStages ? step - kStages : 0; s < step; ++s) mbar_wait_drain(full + 8 * (s % kStages), (s / kStages) & 1);
   } else if (warp == 1) {
     // products
-    const bool one = elect_one();
-    uint32_t step = 0, turn = 0;
+    uint32_t slot = 0, phase = 0, turn = 0;
     bool ok = true;
     for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
       const Tile k = tile_of(p, t);
       const int parts = parts_of(p, k);
       for (int part = 0; part < parts && ok; ++part, ++turn) {
         const uint32_t buf = turn & 1;
-        ok = mbar_wait_uniform(acc_empty + 8 * buf, ((turn >> 1) & 1) ^ 1, &abort_flag);
-        if (!ok) break;
+        ok = mbar_wait_straight(acc_empty + 8 * buf, ((turn >> 1) & 1) ^ 1, &abort_flag);
         tc_fence_after();
-        for (int g = 0; g < p.n_seg && ok; ++g) {
+        for (int g = 0; g < p.n_seg; ++g) {
           const Segment &s = p.seg[g];
           const int blocks = split_begin(s.blocks, k.split + 1, p.splits) - split_begin(s.blocks, k.split, p.splits);
           if (part >= part_count(blocks, p.pairs)) continue;
@@ -302,23 +311,20 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
           const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)s.a_mn << 15) | ((uint32_t)s.b_mn << 16) |
                                  ((uint32_t)(s.boxes_b * kBox >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24);
           const uint32_t d = tmem + buf * 256 + s.col, ua = s.a_mn ? 128 : 2, ub = s.b_mn ? 128 : 2;
-          for (int i = 0; i < steps; ++i, ++step) {
-            const uint32_t slot = step % kStages;
-            ok = mbar_wait_uniform(full + 8 * slot, (step / kStages) & 1, &abort_flag);
-            if (!ok) break;
+          const uint32_t a0 = operand_lo(ring, s.a_mn), b0 = operand_lo(ring + 2 * kBoxBytes, s.b_mn);
+          for (int i = 0; i < steps && ok; ++i) {
+            ok = mbar_wait_straight(full + 8 * slot, phase, &abort_flag);
             tc_fence_after();
-            const uint32_t at = ring + slot * kStageBytes;
-            const uint32_t a = operand_lo(at, s.a_mn), b = operand_lo(at + 2 * kBoxBytes, s.b_mn);
-            if (one) {
+            const uint32_t a = a0 + slot * (kStageBytes >> 4), b = b0 + slot * (kStageBytes >> 4);
+            if (ok && elect_one()) {
 #pragma unroll
-              for (uint32_t q = 0; q < 4; ++q) mma_f16_ss(d, a + q * ua, b + q * ub, idesc, i > 0 || q > 0 ? 1u : 0u);
+              for (uint32_t q = 0; q < 4; ++q) mma_f16_ss(d, a + q * ua, b + q * ub, idesc, (i | (int)q) != 0 ? 1u : 0u);
               mma_commit(empty + 8 * slot);
             }
-            __syncwarp();
+            if (++slot == kStages) slot = 0, phase ^= 1;
           }
         }
-        if (ok && one) mma_commit(acc_full + 8 * buf);
-        __syncwarp();
+        if (ok && elect_one()) mma_commit(acc_full + 8 * buf);
       }
     }
   } else if (warp >= 4) {
@@ -331,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
     for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
       const Tile k = tile_of(p, t);
       const int half_m = k.m >= p.m_half ? 1 : 0, m0 = (k.m - half_m * p.m_half) * kTileM, n0 = k.n * p.step_n;
-      const int row = m0 + 32 * quad + lane, each = p.step_n / 2;
+      const int row = m0 + 32 * quad + lane, each = p.step_n / kSides<T>;
       if constexpr (sizeof(T) == 4) {
         float sum[kSets][kGroups][16];
 #pragma unroll
@@ -591,7 +597,7 @@ int make_map(CUtensorMap *map, const Matrix &m, bool f16) {
   return SSC_OK;
 }
 
-int pitch_of(int cols) { return (cols + 7) & ~7; }
+int pitch_of(int cols) { return (cols + 15) & ~15; }     // rows of whole sectors
 int planes_for(int type) { return type == SSC_PREC_FP32 ? 3 : 1; }
 
 // Scratch is handed out piece by piece; a null base counts the bytes.
@@ -617,7 +623,7 @@ struct Ff {
 template <class T>
 Matrix operand(Ff &f, Scratch &s, const void *p, long long rows, int cols, int each) {
   const int pitch = pitch_of(cols), planes = planes_for(f.type);
-  if (sizeof(T) == 2 && pitch == cols && ((uintptr_t)p & 15) == 0) return {p, rows / each, cols, cols, each};
+  if (sizeof(T) == 2 && cols % 8 == 0 && ((uintptr_t)p & 15) == 0) return {p, rows / each, cols, cols, each};
   void *to = s.take((size_t)rows * pitch * 2 * planes);
   if (s.base != nullptr) {
     const long long threads = rows * (pitch / 8);
@@ -641,7 +647,7 @@ int launch_gemm(Ff &f, const FfMaps &maps, FfParams &p) {
   SSC_REQUIRE(tiles < 1ll << 30, "gated_ff: too many tiles");
   const int sms = sm_count();
   cudaError_t e = allow_smem((const void *)ff_gemm_kernel<EPI, T>, kSmemBytes);
-  if (e == cudaSuccess) e = launch_ready(ff_gemm_kernel<EPI, T>, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(kThreads), kSmemBytes, f.st, maps, p);
+  if (e == cudaSuccess) e = launch_ready(ff_gemm_kernel<EPI, T>, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(kThreads<T>), kSmemBytes, f.st, maps, p);
   if (e != cudaSuccess) return fail(SSC_ERR_CUDA, "gated_ff: %s", cudaGetErrorString(e));
   ++f.launches;
   return SSC_OK;
@@ -685,7 +691,7 @@ int rows_product(Ff &f, const Matrix &a, const Matrix &b, int b_mn, bool halves,
   p.bias = bias;
   p.residual = residual;
   p.out = out;
-  p.vec = cols % (16 / (int)sizeof(T)) == 0 && (((uintptr_t)out | (uintptr_t)residual) & 15) == 0;
+  p.vec = cols % (32 / (int)sizeof(T)) == 0 && (((uintptr_t)out | (uintptr_t)residual) & 31) == 0;
   return launch_gemm<kRows, T>(f, maps, p);
 }
 
@@ -773,7 +779,7 @@ int filter_product(Ff &f, const Matrix &a, const Matrix &b, int halves, int m, i
   p.tiles_n = ceil_div(cols, p.step_n);
   p.splits = splits;
   p.out = part;
-  p.vec = cols % 4 == 0;
+  p.vec = cols % 8 == 0;
   p.accumulate = accumulate;
   return launch_gemm<kPart, T>(f, maps, p);
 }
