@@ -6,8 +6,8 @@
 // cost time up to 700 channels, and two roundings); then dx = dg Wg + du Wu, dWin = [dg, du]' x and dWo = dy' h, whose long sums
 // are split over the rows and added in a fixed order.
 //
-// All of them are one kernel: tiles of 128 rows in tensor memory, operands by TMA, a warp that issues the products and eight
-// that empty the accumulators, two of which are in turn.  Operands are 16-bit; float32 rows are the sum of
+// All of them are one kernel: pairs of CTAs with tiles of 256 rows in tensor memory, half of each operand in either CTA, operands by TMA, a warp
+// that issues the products and others that empty the accumulators, two of which are in turn.  Operands are 16-bit; float32 rows are the sum of
 // three bfloat16 planes (24 bits), and a product the sum of the six products of planes that reach 2^-24, the small ones first.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -22,15 +22,14 @@ namespace {
 
 constexpr int kBox = 64;                      // TMA boxes: 64 x 64 elements, 128-byte rows
 constexpr uint32_t kBoxBytes = kBox * kBox * 2;
-constexpr int kTileM = 128;
-constexpr int kStageBoxes = 6;                // two of A, up to four of B
-constexpr uint32_t kStageBytes = kStageBoxes * kBoxBytes;
-constexpr int kStages = 4;
-// Warps: TMA, products, tensor memory, an idle one, then those for the accumulators: sixteen (eight where float32 sums need the registers).
-template <class T>
-constexpr int kSides = sizeof(T) == 4 ? 2 : 4;              // shares of a tile's columns
-template <class T>
-constexpr int kThreads = 128 + 128 * kSides<T>;
+constexpr int kTileM = 256;                   // of a pair of CTAs, half of it each
+constexpr uint32_t kStageBytes = 4 * kBoxBytes;     // two boxes of A, up to two of B
+constexpr int kStages = 6;
+// Warps: TMA, products, tensor memory, an idle one, then those for the accumulators: sixteen, eight where sums in registers (LONG) need the room.
+template <bool LONG>
+constexpr int kSides = LONG ? 2 : 4;                        // shares of a tile's columns
+template <bool LONG>
+constexpr int kThreads = 128 + 128 * kSides<LONG>;
 constexpr uint32_t kSmemBytes = kStages * kStageBytes + 1024;
 
 enum Epilogue { kGate, kBack, kRows, kPart };
@@ -42,21 +41,21 @@ struct Segment {
   int a_planes, b_planes;    // matrices of one plane: 1 or 2
   int blocks;                // of 64 along the summed index
   int half_blocks;           // kByK: blocks of the first matrix
-  int boxes_b;
-  int col;                   // accumulator column
+  uint32_t idesc;            // of the product: types, which operand lies which way round, 256 rows and the columns
+  int boxes_b;               // of each CTA: half of the product's columns (kByBox: of one matrix in each)
 };
 struct FfMaps {
   CUtensorMap a[2], b[2];
 };
 struct FfParams {
   Segment seg[2];
-  int n_seg, pairs, f16;
+  int n_seg, pairs;
   int tiles_m, tiles_n, splits, m_half;        // tiles; m_half: tiles of the first matrix (kByM)
   int step_n;                                  // columns of the result to a tile
   int rows, cols;                              // of the result (one matrix)
   int act;
   const void *bias;                            // of the result's columns; kGate / kBack: [2][hidden]
-  const void *residual;
+  const void *residual;                        // kRows: rows of T; kBack of float32: dh [rows][pitch]
   void *out, *out2;                            // kGate: h; kBack: h, dg|du; kRows: result; kPart: float [splits][rows of all][cols]
   int pitch;                                   // of out
   size_t plane, plane2;                        // elements from one plane to the next (of out, of a matrix of out2)
@@ -65,11 +64,13 @@ struct FfParams {
   int32_t *status, *alarm;
 };
 
+// A box into this CTA's shared memory; its bytes count on a barrier of either CTA.
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map),
-               "r"(x), "r"(y), "r"(z), "r"(bar)
+  asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+               "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
                : "memory");
 }
+__device__ __forceinline__ void arrive_there(uint32_t bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 
 // Operands of a stage: rows of 128 bytes, 128-byte swizzle.  Summed index contiguous: groups of eight rows 1024 bytes
 // apart, 32 bytes a step of 16.  Rows contiguous: blocks of 64 rows a box apart, eight steps of the summed index 1024 bytes.
@@ -141,18 +142,40 @@ __device__ __forceinline__ void put_hidden(void *base, size_t at, size_t plane, 
 __device__ __forceinline__ void tmem_floats(float *v, uint32_t addr) { tmem_ld16((uint32_t *)v, addr); }
 __device__ __forceinline__ void tmem_arrived() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
-struct Tile {
-  int m, n, split;      // tile numbers
+// The tiles of a pair of CTAs, stepped through without a division: the roles that walk are single warps, whose every instruction is
+// waited for (with divisions for tiles and shares, products of K = 256 spent half of their time between tiles).
+struct Walk {
+  int n, m, split;      // column tile, row tile, share
+  int dn, dm, ds;
+  __device__ __forceinline__ explicit Walk(const FfParams &p) {
+    const int t = blockIdx.x >> 1, by = gridDim.x >> 1;
+    split_up(p, t, n, m, split);
+    split_up(p, by, dn, dm, ds);
+  }
+  static __device__ __forceinline__ void split_up(const FfParams &p, int t, int &n, int &m, int &split) {
+    n = t % p.tiles_n;
+    t /= p.tiles_n;
+    m = t % p.tiles_m;
+    split = t / p.tiles_m;
+  }
+  __device__ __forceinline__ bool more(const FfParams &p) const { return split < p.splits; }
+  __device__ __forceinline__ void next(const FfParams &p) {
+    n += dn;
+    m += dm;
+    split += ds;
+    if (n >= p.tiles_n) n -= p.tiles_n, ++m;
+    if (m >= p.tiles_m) m -= p.tiles_m, ++split;
+  }
 };
-__device__ __forceinline__ Tile tile_of(const FfParams &p, int t) {
-  Tile k;
-  k.n = t % p.tiles_n;
-  t /= p.tiles_n;
-  k.m = t % p.tiles_m;
-  k.split = t / p.tiles_m;
-  return k;
+// The blocks of 64 of a segment's sum in a share.
+__device__ __forceinline__ void share_of_sum(const FfParams &p, int g, int split, int &first, int &blocks) {
+  first = 0;
+  blocks = p.seg[g].blocks;
+  if (p.splits > 1) {
+    first = (int)((uint32_t)blocks * (uint32_t)split / (uint32_t)p.splits);
+    blocks = (int)((uint32_t)blocks * (uint32_t)(split + 1) / (uint32_t)p.splits) - first;
+  }
 }
-__device__ __forceinline__ int split_begin(int blocks, int split, int splits) { return (int)((long long)blocks * split / splits); }
 
 // The steps of a tile's sum: `blocks` of 64 for each pair of planes.  Tensor memory's additions cut off instead of rounding, which
 // adds up (1.5e-6 of gx over 1024 terms): float32 results leave tensor memory after every kLeave blocks of the last
@@ -163,11 +186,22 @@ __device__ __forceinline__ int part_begin(int blocks, int pairs, int part) {
   return part == 0 ? 0 : min((pairs - 1) * blocks + part * (pairs == 1 ? blocks : kLeave), pairs * blocks);
 }
 
-__device__ __forceinline__ int parts_of(const FfParams &p, const Tile &k) {
+__device__ __forceinline__ int parts_of(const FfParams &p, int split) {
+  if (p.pairs == 1) return 1;
   int most = 1;
-  for (int g = 0; g < p.n_seg; ++g)
-    most = max(most, part_count(split_begin(p.seg[g].blocks, k.split + 1, p.splits) - split_begin(p.seg[g].blocks, k.split, p.splits), p.pairs));
+  for (int g = 0; g < p.n_seg; ++g) {
+    int first, blocks;
+    share_of_sum(p, g, split, first, blocks);
+    most = max(most, part_count(blocks, p.pairs));
+  }
   return most;
+}
+
+// dh of float32 rows, which has been multiplied before.
+__device__ __forceinline__ void stored_dh(const FfParams &p, int row, int n, float *d) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) d[i] = 0.f;
+  if (row < p.rows) add16<float>(d, (const float *)p.residual + (size_t)row * p.pitch + n, p.cols - n, 1);
 }
 
 // 16 columns from column n on of a row of the result: v (kGate: gate, u: up; kBack: d = dh too).
@@ -215,8 +249,9 @@ __device__ __forceinline__ void finish(const FfParams &p, int split, int half_m,
   }
 }
 
-template <int EPI, class T>
-__global__ void __launch_bounds__(kThreads<T>, 1) ff_gemm_kernel(const __grid_constant__ FfMaps maps, const FfParams p) {
+// LONG: float32 sums that leave tensor memory in between (part_count).
+template <int EPI, class T, bool LONG>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads<LONG>, 1) ff_gemm_kernel(const __grid_constant__ FfMaps maps, const FfParams p) {
   after_previous();
   extern __shared__ uint8_t raw[];
   __shared__ alignas(8) uint64_t bars[2 * kStages + 5];
@@ -224,121 +259,139 @@ __global__ void __launch_bounds__(kThreads<T>, 1) ff_gemm_kernel(const __grid_co
   __shared__ volatile int abort_flag;
   const uint32_t ring = (smem_u32(raw) + 1023u) & ~1023u;
   const uint32_t full = smem_u32(bars), empty = full + 8 * kStages, acc_full = empty + 8 * kStages, acc_empty = acc_full + 16, done = acc_empty + 16;
-  const int warp = warp_id(), tiles = p.tiles_m * p.tiles_n * p.splits;
+  const int warp = warp_id(), rank = blockIdx.x & 1;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(full + 8 * s, 1);
+      mbar_init(full + 8 * s, 1);                       // the first CTA's: both CTAs' boxes count there
       mbar_init(empty + 8 * s, 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(acc_full + 8 * b, 1);
-      mbar_init(acc_empty + 8 * b, 4 * kSides<T>);
+      mbar_init(acc_empty + 8 * b, 8 * kSides<LONG>);   // the first CTA's: both CTAs' warps
     }
     mbar_init(done, 1);
     abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 2) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_base)) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_base)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
+  cluster_sync();                                       // the other CTA's barriers stand
   tc_fence_after();
   const uint32_t tmem = tmem_base;
+  // Accumulators: two of 256 columns in turn.  kBack with three products: gate and up in the first 256 columns, dh in the others, in turn, so that
+  // the next tile's dh is multiplied while this tile's values are taken out.
+  constexpr bool kThree = EPI == kBack && sizeof(T) == 2;
 
   if (warp == 0) {
     // operands
+    const uint32_t full_there = peer_address(full, 0);
     uint32_t slot = 0, phase = 1, step = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      const Tile k = tile_of(p, t);
-      const int half_m = k.m >= p.m_half ? 1 : 0, m0 = (k.m - half_m * p.m_half) * kTileM, n0 = k.n * p.step_n;
-      const int parts = parts_of(p, k);
+    for (Walk k(p); k.more(p) && ok; k.next(p)) {
+      const int half_m = k.m >= p.m_half ? 1 : 0, m0 = (k.m - half_m * p.m_half) * kTileM + rank * (kTileM / 2);
+      const int parts = parts_of(p, k.split);
       for (int part = 0; part < parts; ++part)
         for (int g = 0; g < p.n_seg; ++g) {
           const Segment &s = p.seg[g];
-          const int kb0 = split_begin(s.blocks, k.split, p.splits), blocks = split_begin(s.blocks, k.split + 1, p.splits) - kb0;
+          int kb0, blocks;
+          share_of_sum(p, g, k.split, kb0, blocks);
           if (part >= part_count(blocks, p.pairs)) continue;
-          const uint32_t bytes = (2 + s.boxes_b) * kBoxBytes;
-          const int per = s.b_half == kByBox ? s.boxes_b / 2 : s.boxes_b, end = part_begin(blocks, p.pairs, part + 1);
+          const int n0 = k.n * p.step_n + (s.b_half == kByBox ? 0 : rank * s.boxes_b * kBox), end = part_begin(blocks, p.pairs, part + 1);
           const CUtensorMap *map_a = &maps.a[g], *map_b = &maps.b[g];
-          int i = part_begin(blocks, p.pairs, part), pair = blocks > 0 ? i / blocks : 0, kb = kb0 + i - pair * blocks;
-          for (; i < end && ok; ++i, ++step) {
-            ok = mbar_wait_straight(empty + 8 * slot, phase, &abort_flag);
+          const uint32_t bytes = 2 * (2 + s.boxes_b) * kBoxBytes;
+          int pair = part == 0 ? 0 : p.pairs - 1, i = part_begin(blocks, p.pairs, part), kb = i - pair * blocks;
+          while (i < end && ok) {
+            // a run of blocks of one pair of planes in one matrix
+            const int by_k = kb0 + kb >= s.half_blocks ? 1 : 0;
+            const int run = min(min(end - i, blocks - kb), by_k ? 1 << 30 : s.half_blocks - kb0 - kb);
             const int pa = p.pairs == 1 ? 0 : kPlaneA[pair], pb = p.pairs == 1 ? 0 : kPlaneB[pair];
-            const uint32_t at = ring + slot * kStageBytes, bar = full + 8 * slot;
-            const int by_k = kb >= s.half_blocks ? 1 : 0, kk = (kb - by_k * s.half_blocks) * kBox;
-            const int za = pa * s.a_planes + (s.a_half == kByK ? by_k : s.a_half == kByM ? half_m : 0), zb = pb * s.b_planes + (s.b_half == kByK ? by_k : 0);
-            if (ok && elect_one()) {
-              mbar_expect_tx(bar, bytes);
-              if (s.a_mn) {
-                tma_box(at, map_a, m0, kk, za, bar);
-                tma_box(at + kBoxBytes, map_a, m0 + kBox, kk, za, bar);
-              } else {
-                tma_box(at, map_a, kk, m0, za, bar);
-                tma_box(at + kBoxBytes, map_a, kk, m0 + kBox, za, bar);
+            const int za = pa * s.a_planes + (s.a_half == kByK ? by_k : s.a_half == kByM ? half_m : 0);
+            const int zb = pb * s.b_planes + (s.b_half == kByK ? by_k : s.b_half == kByBox ? rank : 0);
+            int kk = (kb0 + kb - by_k * s.half_blocks) * kBox;
+            for (int j = 0; j < run && ok; ++j, kk += kBox, ++step) {
+              ok = mbar_wait_straight(empty + 8 * slot, phase, &abort_flag);
+              const uint32_t at = ring + slot * kStageBytes, bar = full_there + 8 * slot;
+              if (ok && elect_one()) {
+                if (rank == 0) mbar_expect_tx(full + 8 * slot, bytes);
+                if (s.a_mn) {
+                  tma_box(at, map_a, m0, kk, za, bar);
+                  tma_box(at + kBoxBytes, map_a, m0 + kBox, kk, za, bar);
+                } else {
+                  tma_box(at, map_a, kk, m0, za, bar);
+                  tma_box(at + kBoxBytes, map_a, kk, m0 + kBox, za, bar);
+                }
+                if (s.b_mn) {
+                  tma_box(at + 2 * kBoxBytes, map_b, n0, kk, zb, bar);
+                  if (s.boxes_b == 2) tma_box(at + 3 * kBoxBytes, map_b, n0 + kBox, kk, zb, bar);
+                } else {
+                  tma_box(at + 2 * kBoxBytes, map_b, kk, n0, zb, bar);
+                  if (s.boxes_b == 2) tma_box(at + 3 * kBoxBytes, map_b, kk, n0 + kBox, zb, bar);
+                }
               }
-              for (int j = 0; j < s.boxes_b; ++j) {
-                const int h = j >= per ? 1 : 0, n = n0 + (j - h * per) * kBox;
-                tma_box(at + (2 + j) * kBoxBytes, map_b, s.b_mn ? n : kk, s.b_mn ? kk : n, zb + h, bar);
-              }
+              if (++slot == kStages) slot = 0, phase ^= 1;
             }
-            if (++slot == kStages) slot = 0, phase ^= 1;
-            if (++kb == kb0 + blocks) kb = kb0, ++pair;
+            i += run;
+            kb += run;
+            if (kb == blocks) kb = 0, ++pair;
           }
         }
     }
-    if (abort_flag)      // copies in flight arrive before the block leaves
+    if (abort_flag && rank == 0)      // copies in flight, the other CTA's too, arrive before the blocks leave
       for (uint32_t s = step > kStages ? step - kStages : 0; s < step; ++s) mbar_wait_drain(full + 8 * (s % kStages), (s / kStages) & 1);
-  } else if (warp == 1) {
+  } else if (warp == 1 && rank == 0) {
     // products
     uint32_t slot = 0, phase = 0, turn = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      const Tile k = tile_of(p, t);
-      const int parts = parts_of(p, k);
+    for (Walk k(p); k.more(p) && ok; k.next(p)) {
+      const int parts = parts_of(p, k.split);
       for (int part = 0; part < parts && ok; ++part, ++turn) {
         const uint32_t buf = turn & 1;
-        ok = mbar_wait_straight(acc_empty + 8 * buf, ((turn >> 1) & 1) ^ 1, &abort_flag);
+        ok = mbar_wait_straight_cluster(acc_empty + 8 * buf, ((turn >> 1) & 1) ^ 1, &abort_flag);
         tc_fence_after();
         for (int g = 0; g < p.n_seg; ++g) {
           const Segment &s = p.seg[g];
-          const int blocks = split_begin(s.blocks, k.split + 1, p.splits) - split_begin(s.blocks, k.split, p.splits);
+          int first, blocks;
+          share_of_sum(p, g, k.split, first, blocks);
           if (part >= part_count(blocks, p.pairs)) continue;
+          if (kThree && g == 1 && turn > 0) {           // gate and up of the tile before have been taken out
+            ok = ok && mbar_wait_straight_cluster(acc_empty + 8 * (buf ^ 1), ((turn - 1) >> 1) & 1, &abort_flag);
+            tc_fence_after();
+          }
           const int steps = part_begin(blocks, p.pairs, part + 1) - part_begin(blocks, p.pairs, part);
-          const uint32_t type = p.f16 ? 0u : 1u;
-          const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)s.a_mn << 15) | ((uint32_t)s.b_mn << 16) |
-                                 ((uint32_t)(s.boxes_b * kBox >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24);
-          const uint32_t d = tmem + buf * 256 + s.col, ua = s.a_mn ? 128 : 2, ub = s.b_mn ? 128 : 2;
+          const uint32_t idesc = s.idesc, d = tmem + (kThree ? (g == 0 ? 256 + buf * 128 : 0) : buf * 256), ua = s.a_mn ? 128 : 2, ub = s.b_mn ? 128 : 2;
           const uint32_t a0 = operand_lo(ring, s.a_mn), b0 = operand_lo(ring + 2 * kBoxBytes, s.b_mn);
           for (int i = 0; i < steps && ok; ++i) {
-            ok = mbar_wait_straight(full + 8 * slot, phase, &abort_flag);
+            ok = mbar_wait_straight_cluster(full + 8 * slot, phase, &abort_flag);
             tc_fence_after();
             const uint32_t a = a0 + slot * (kStageBytes >> 4), b = b0 + slot * (kStageBytes >> 4);
             if (ok && elect_one()) {
 #pragma unroll
-              for (uint32_t q = 0; q < 4; ++q) mma_f16_ss(d, a + q * ua, b + q * ub, idesc, (i | (int)q) != 0 ? 1u : 0u);
-              mma_commit(empty + 8 * slot);
+              for (uint32_t q = 0; q < 4; ++q) mma_pair<true>(d, a + q * ua, b + q * ub, idesc, (i | (int)q) != 0 ? 1u : 0u);
+              mma_commit_pair(empty + 8 * slot);
             }
             if (++slot == kStages) slot = 0, phase ^= 1;
           }
         }
-        if (ok && elect_one()) mma_commit(acc_full + 8 * buf);
+        if (ok && elect_one()) mma_commit_pair(acc_full + 8 * buf);
       }
     }
   } else if (warp >= 4) {
-    // accumulators: a thread has a row and half of a tile's columns, kGroups times 16 of them from kSets products
-    constexpr int kSets = EPI == kGate ? 2 : EPI == kBack ? 3 : 1, kGroups = EPI == kGate ? 4 : EPI == kBack ? 2 : 8;
+    // accumulators: a thread has a row and a share of a tile's columns, kGroups times 16 of them from kSets products
+    constexpr int kSets = EPI == kGate ? 2 : kThree ? 3 : EPI == kBack ? 2 : 1, kGroups = kSets == 2 ? 4 : 8;
     const int quad = warp & 3, side = (warp - 4) >> 2, lane = threadIdx.x & 31;
-    const uint32_t lanes = (uint32_t)(32 * quad) << 16;
+    const uint32_t lanes = (uint32_t)(32 * quad) << 16, empty_there = peer_address(acc_empty, 0);
     uint32_t turn = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      const Tile k = tile_of(p, t);
-      const int half_m = k.m >= p.m_half ? 1 : 0, m0 = (k.m - half_m * p.m_half) * kTileM, n0 = k.n * p.step_n;
-      const int row = m0 + 32 * quad + lane, each = p.step_n / kSides<T>;
-      if constexpr (sizeof(T) == 4) {
+    for (Walk k(p); k.more(p) && ok; k.next(p)) {
+      const int half_m = k.m >= p.m_half ? 1 : 0, m0 = (k.m - half_m * p.m_half) * kTileM + rank * (kTileM / 2), n0 = k.n * p.step_n;
+      const int row = m0 + 32 * quad + lane, each = p.step_n / kSides<LONG>;
+      int first, blocks;
+      share_of_sum(p, 0, k.split, first, blocks);
+      if constexpr (LONG) {
         float sum[kSets][kGroups][16];
 #pragma unroll
         for (int s = 0; s < kSets; ++s)
@@ -346,60 +399,66 @@ __global__ void __launch_bounds__(kThreads<T>, 1) ff_gemm_kernel(const __grid_co
           for (int g = 0; g < kGroups; ++g)
 #pragma unroll
             for (int i = 0; i < 16; ++i) sum[s][g][i] = 0.f;
-        const int parts = parts_of(p, k);
+        const int parts = parts_of(p, k.split);
         for (int part = 0; part < parts && ok; ++part, ++turn) {
           const uint32_t buf = turn & 1, acc = tmem + buf * 256 + lanes;
           ok = mbar_wait_uniform(acc_full + 8 * buf, (turn >> 1) & 1, &abort_flag);
           if (!ok) break;
           tc_fence_after();
+          if (blocks > 0) {                             // (else an empty share)
 #pragma unroll
-          for (int s = 0; s < kSets; ++s) {
-            const Segment &from = p.seg[EPI == kBack && s == 2 ? 1 : 0];
-            const int blocks = split_begin(from.blocks, k.split + 1, p.splits) - split_begin(from.blocks, k.split, p.splits);
-            if (blocks == 0 || part >= part_count(blocks, p.pairs)) continue;
+            for (int s = 0; s < kSets; ++s)
 #pragma unroll
-            for (int g = 0; g < kGroups; ++g)
-              if (16 * g < each) {
-                float v[16];
-                tmem_floats(v, acc + s * p.step_n + side * each + 16 * g);
-                tmem_arrived();
+              for (int g = 0; g < kGroups; ++g)
+                if (16 * g < each) {
+                  float v[16];
+                  tmem_floats(v, acc + s * p.step_n + side * each + 16 * g);
+                  tmem_arrived();
 #pragma unroll
-                for (int i = 0; i < 16; ++i) sum[s][g][i] += v[i];
-              }
+                  for (int i = 0; i < 16; ++i) sum[s][g][i] += v[i];
+                }
           }
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(acc_empty + 8 * buf);
+          if (lane == 0) arrive_there(empty_there + 8 * buf);
         }
         if (!ok) break;
 #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
           const int n = n0 + side * each + 16 * g;
-          if (16 * g < each && n < p.cols)
-            finish<EPI, T>(p, k.split, half_m, row, n, sum[0][g], sum[kSets > 1 ? 1 : 0][g], sum[kSets > 2 ? 2 : 0][g]);
+          if (16 * g < each && n < p.cols) {
+            float d[16];
+            if (EPI == kBack) stored_dh(p, row, n, d);
+            finish<EPI, T>(p, k.split, half_m, row, n, sum[0][g], sum[kSets > 1 ? 1 : 0][g], d);
+          }
         }
       } else {
-        const uint32_t buf = turn & 1, acc = tmem + buf * 256 + lanes;
+        const uint32_t buf = turn & 1, acc = tmem + (kThree ? 0 : buf * 256) + lanes;
         ok = mbar_wait_uniform(acc_full + 8 * buf, (turn >> 1) & 1, &abort_flag);
         if (!ok) break;
         tc_fence_after();
-        const bool none = split_begin(p.seg[0].blocks, k.split, p.splits) == split_begin(p.seg[0].blocks, k.split + 1, p.splits);
         for (int c = side * each; c < (side + 1) * each; c += 16) {
           const int n = n0 + c;
           if (n >= p.cols) break;
           float v[kSets][16];
 #pragma unroll
-          for (int s = 0; s < kSets; ++s) tmem_floats(v[s], acc + s * p.step_n + c);
+          for (int s = 0; s < kSets; ++s) tmem_floats(v[s], kThree && s == 2 ? tmem + 256 + buf * 128 + lanes + c : acc + s * p.step_n + c);
           tmem_arrived();
-          if (EPI == kPart && none) {
+          if (EPI == kPart && blocks == 0) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) v[0][i] = 0.f;      // (an empty share)
           }
-          finish<EPI, T>(p, k.split, half_m, row, n, v[0], v[kSets > 1 ? 1 : 0], v[kSets > 2 ? 2 : 0]);
+          if (EPI == kBack && !kThree) {
+            float d[16];
+            stored_dh(p, row, n, d);
+            finish<EPI, T>(p, k.split, half_m, row, n, v[0], v[kSets > 1 ? 1 : 0], d);
+          } else {
+            finish<EPI, T>(p, k.split, half_m, row, n, v[0], v[kSets > 1 ? 1 : 0], v[kSets > 2 ? 2 : 0]);
+          }
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(acc_empty + 8 * buf);
+        if (lane == 0) arrive_there(empty_there + 8 * buf);
         ++turn;
       }
     }
@@ -408,15 +467,16 @@ __global__ void __launch_bounds__(kThreads<T>, 1) ff_gemm_kernel(const __grid_co
   __syncthreads();
   tc_fence_after();
   if (abort_flag) {
-    if (warp == 1) {      // products that are still running end before tensor memory is given back
-      if (elect_one()) mma_commit(done);
+    if (warp == 1 && rank == 0) {      // products that are still running end before tensor memory is given back
+      if (elect_one()) mma_commit_pair(done);
       __syncwarp();
       mbar_wait_drain(done, 0);
     }
     if (threadIdx.x == 0) report_expired(p.status, p.alarm);
-    __syncthreads();
   }
-  if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  cluster_sync();                                       // neither leaves while the other may still signal it
+  if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  cluster_sync();
 }
 
 // Rows [rows][cols] of float32 as three bfloat16 planes, or 16-bit rows that TMA cannot read as they are (a width or an address
@@ -639,15 +699,28 @@ size_t operand_bytes(int type, long long rows, int cols) { return align_up((size
 template <int EPI, class T>
 int launch_gemm(Ff &f, const FfMaps &maps, FfParams &p) {
   p.pairs = planes_for(f.type) == 3 ? 6 : 1;
-  p.f16 = f.type == SSC_PREC_F16;
+  for (Segment &s : p.seg) {
+    const uint32_t type = f.type == SSC_PREC_F16 ? 0u : 1u;
+    s.idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)s.a_mn << 15) | ((uint32_t)s.b_mn << 16) | ((uint32_t)(2 * s.boxes_b * kBox >> 3) << 17) |
+              ((uint32_t)(kTileM >> 4) << 24);
+  }
   p.act = f.act;
   p.status = f.status;
   p.alarm = alarm_word();
   const long long tiles = (long long)p.tiles_m * p.tiles_n * p.splits;
   SSC_REQUIRE(tiles < 1ll << 30, "gated_ff: too many tiles");
-  const int sms = sm_count();
-  cudaError_t e = allow_smem((const void *)ff_gemm_kernel<EPI, T>, kSmemBytes);
-  if (e == cudaSuccess) e = launch_ready(ff_gemm_kernel<EPI, T>, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(kThreads<T>), kSmemBytes, f.st, maps, p);
+  const unsigned pairs = (unsigned)(sm_count() / 2), grid = 2 * (tiles < (long long)pairs ? (unsigned)tiles : pairs);
+  bool parts = false;
+  for (int g = 0; g < p.n_seg; ++g) parts |= p.pairs > 1 && ceil_div(p.seg[g].blocks, p.splits) > kLeave;
+  auto kernel = ff_gemm_kernel<EPI, T, false>;
+  int threads = kThreads<false>;
+  if constexpr (sizeof(T) == 4)
+    if (parts) {
+      kernel = ff_gemm_kernel<EPI, T, true>;
+      threads = kThreads<true>;
+    }
+  cudaError_t e = allow_smem((const void *)kernel, kSmemBytes);
+  if (e == cudaSuccess) e = launch_ready(kernel, dim3(grid), dim3(threads), kSmemBytes, f.st, maps, p);
   if (e != cudaSuccess) return fail(SSC_ERR_CUDA, "gated_ff: %s", cudaGetErrorString(e));
   ++f.launches;
   return SSC_OK;
@@ -662,18 +735,18 @@ Segment segment(int k, int boxes_b) {
   return s;
 }
 
-// Result tiles of 64, 128 or 256 columns: the widest that is not mostly empty.
-int tile_columns(int cols) { return cols <= 64 ? 64 : cols <= 128 ? 128 : 256; }
+// Result tiles of 128 or 256 columns.
+int tile_columns(int cols) { return cols <= 128 ? 128 : 256; }
 
 // C [rows][cols] = A B' (+ bias, residual) as rows of T; B as stored (b_mn: [k][cols]).
 template <class T>
-int rows_product(Ff &f, const Matrix &a, const Matrix &b, int b_mn, bool halves, int k, int cols, const void *bias, const void *residual, void *out) {
+int rows_product(Ff &f, const Matrix &a, const Matrix &b, int b_mn, bool halves, int k, int cols, const void *bias, const void *residual, void *out, int pitch = 0) {
   FfMaps maps = {};
   FfParams p = {};
   if (int e = make_map(&maps.a[0], a, f.type == SSC_PREC_F16)) return e;
   if (int e = make_map(&maps.b[0], b, f.type == SSC_PREC_F16)) return e;
   p.step_n = tile_columns(cols);
-  p.seg[0] = segment(k, p.step_n / kBox);
+  p.seg[0] = segment(k, p.step_n / (2 * kBox));
   p.seg[0].b_mn = b_mn;
   if (halves) {
     p.seg[0].a_half = p.seg[0].b_half = kByK;
@@ -683,7 +756,8 @@ int rows_product(Ff &f, const Matrix &a, const Matrix &b, int b_mn, bool halves,
   }
   p.n_seg = 1;
   p.rows = (int)a.rows;
-  p.cols = p.pitch = cols;
+  p.cols = cols;
+  p.pitch = pitch ? pitch : cols;
   p.tiles_m = ceil_div(p.rows, kTileM);
   p.m_half = 1 << 30;
   p.tiles_n = ceil_div(cols, p.step_n);
@@ -691,7 +765,7 @@ int rows_product(Ff &f, const Matrix &a, const Matrix &b, int b_mn, bool halves,
   p.bias = bias;
   p.residual = residual;
   p.out = out;
-  p.vec = cols % (32 / (int)sizeof(T)) == 0 && (((uintptr_t)out | (uintptr_t)residual) & 31) == 0;
+  p.vec = p.pitch % (32 / (int)sizeof(T)) == 0 && (((uintptr_t)out | (uintptr_t)residual) & 31) == 0;
   return launch_gemm<kRows, T>(f, maps, p);
 }
 
@@ -701,8 +775,8 @@ int gate_product(Ff &f, const Matrix &x, const Matrix &w_in, const void *b_in, v
   FfParams p = {};
   if (int e = make_map(&maps.a[0], x, f.type == SSC_PREC_F16)) return e;
   if (int e = make_map(&maps.b[0], w_in, f.type == SSC_PREC_F16)) return e;
-  p.step_n = f.hidden <= 64 ? 64 : 128;
-  p.seg[0] = segment(f.c, 2 * p.step_n / kBox);
+  p.step_n = 128;
+  p.seg[0] = segment(f.c, p.step_n / kBox);
   p.seg[0].b_half = kByBox;
   p.seg[0].b_planes = 2;
   p.n_seg = 1;
@@ -719,24 +793,26 @@ int gate_product(Ff &f, const Matrix &x, const Matrix &w_in, const void *b_in, v
   return launch_gemm<kGate, T>(f, maps, p);
 }
 
-// h, dg and du: gate and up again, and dy Wo.
+// h, dg and du: gate and up again, and dh = dy Wo; float32 sums of three products are more than the registers, there dh has been multiplied before.
 template <class T>
-int back_product(Ff &f, const Matrix &x, const Matrix &w_in, const Matrix &gy, const Matrix &w_out, const void *b_in, void *h, void *dgu) {
+int back_product(Ff &f, const Matrix &x, const Matrix &w_in, const Matrix &gy, const Matrix &w_out, const void *b_in, const float *dh, void *h, void *dgu) {
   FfMaps maps = {};
   FfParams p = {};
   const bool f16 = f.type == SSC_PREC_F16;
-  if (int e = make_map(&maps.a[0], x, f16)) return e;
-  if (int e = make_map(&maps.b[0], w_in, f16)) return e;
-  if (int e = make_map(&maps.a[1], gy, f16)) return e;
-  if (int e = make_map(&maps.b[1], w_out, f16)) return e;
-  p.step_n = 64;
-  p.seg[0] = segment(f.c, 2);
-  p.seg[0].b_half = kByBox;
-  p.seg[0].b_planes = 2;
-  p.seg[1] = segment(f.c_out, 1);
-  p.seg[1].b_mn = 1;
-  p.seg[1].col = 2 * p.step_n;
-  p.n_seg = 2;
+  const int g = sizeof(T) == 2 ? 1 : 0;
+  if (int e = make_map(&maps.a[g], x, f16)) return e;
+  if (int e = make_map(&maps.b[g], w_in, f16)) return e;
+  p.step_n = 128;
+  p.seg[g] = segment(f.c, 2);
+  p.seg[g].b_half = kByBox;
+  p.seg[g].b_planes = 2;
+  p.n_seg = g + 1;
+  if (g == 1) {
+    if (int e = make_map(&maps.a[0], gy, f16)) return e;
+    if (int e = make_map(&maps.b[0], w_out, f16)) return e;
+    p.seg[0] = segment(f.c_out, 1);
+    p.seg[0].b_mn = 1;
+  }
   p.rows = (int)x.rows;
   p.cols = f.hidden;
   p.pitch = pitch_of(f.hidden);
@@ -746,6 +822,7 @@ int back_product(Ff &f, const Matrix &x, const Matrix &w_in, const Matrix &gy, c
   p.tiles_n = ceil_div(f.hidden, p.step_n);
   p.splits = 1;
   p.bias = b_in;
+  p.residual = dh;
   p.out = h;
   p.out2 = dgu;
   return launch_gemm<kBack, T>(f, maps, p);
@@ -754,7 +831,7 @@ int back_product(Ff &f, const Matrix &x, const Matrix &w_in, const Matrix &gy, c
 // Shares of a long sum: enough tiles for every SM, at least eight blocks of 64 to a share.
 int filter_splits(long long rows, int halves, int m, int cols) {
   const int tiles = halves * ceil_div(m, kTileM) * ceil_div(cols, tile_columns(cols)), blocks = ceil_div(rows, kBox);
-  int s = sm_count() / (tiles > 0 ? tiles : 1);
+  int s = sm_count() / 2 / (tiles > 0 ? tiles : 1);
   if (s > blocks / 8) s = blocks / 8;
   return s < 1 ? 1 : s;
 }
@@ -766,7 +843,7 @@ int filter_product(Ff &f, const Matrix &a, const Matrix &b, int halves, int m, i
   if (int e = make_map(&maps.a[0], a, f.type == SSC_PREC_F16)) return e;
   if (int e = make_map(&maps.b[0], b, f.type == SSC_PREC_F16)) return e;
   p.step_n = tile_columns(cols);
-  p.seg[0] = segment((int)a.rows, p.step_n / kBox);
+  p.seg[0] = segment((int)a.rows, p.step_n / (2 * kBox));
   p.seg[0].a_mn = p.seg[0].b_mn = 1;
   p.seg[0].a_planes = halves;
   p.seg[0].a_half = halves == 2 ? kByM : kNone;
@@ -795,7 +872,7 @@ constexpr int kColumnShares = 32;
 long long rows_at_once(const Ff &f, bool backward) {
   const long long per = (long long)pitch_of(f.hidden) * 2 * planes_for(f.type) * (backward ? 3 : 1) + (long long)(pitch_of(f.c) + pitch_of(f.c_out)) * 2 * planes_for(f.type);
   long long rows = (1ll << 30) / per / kTileM * kTileM;
-  if (rows < 32 * kTileM) rows = 32 * kTileM;
+  if (rows < 16 * kTileM) rows = 16 * kTileM;
   return rows < f.n ? rows : f.n;
 }
 
@@ -843,6 +920,7 @@ int backward(Ff &f, Scratch s, const void *x, const void *gy, const void *w_in, 
   const size_t size_in = 2 * (size_t)f.hidden * f.c, size_out = (size_t)f.c_out * f.hidden;
   const int split_in = filter_splits(most, 2, f.hidden, f.c), split_out = filter_splits(most, 1, f.c_out, f.hidden);
   void *h = s.take((size_t)most * pitch * 2 * planes), *dgu = s.take((size_t)most * pitch * 4 * planes);
+  float *dh = planes == 3 ? (float *)s.take((size_t)most * pitch * sizeof(float)) : nullptr;
   float *part_in = (float *)s.take(split_in * size_in * sizeof(float)), *part_out = (float *)s.take(split_out * size_out * sizeof(float));
   float *cols_in = (float *)s.take((size_t)kColumnShares * 2 * f.hidden * sizeof(float)), *cols_out = (float *)s.take((size_t)kColumnShares * f.c_out * sizeof(float));
   cudaError_t e = cudaSuccess;
@@ -851,7 +929,9 @@ int backward(Ff &f, Scratch s, const void *x, const void *gy, const void *w_in, 
     Scratch here = s;
     const int more = r > 0;
     const Matrix xm = operand<T>(f, here, (const T *)x + r * f.c, rows, f.c, 1), gm = operand<T>(f, here, (const T *)gy + r * f.c_out, rows, f.c_out, 1);
-    if (int k = back_product<T>(f, xm, wi, gm, wo, b_in, h, dgu)) return k;
+    if (dh)
+      if (int k = rows_product<T>(f, gm, wo, 1, false, f.c_out, f.hidden, nullptr, nullptr, dh, pitch)) return k;
+    if (int k = back_product<T>(f, xm, wi, gm, wo, b_in, dh, h, dgu)) return k;
     const Matrix hm = {h, rows, f.hidden, pitch, planes}, dm = {dgu, rows, f.hidden, pitch, 2 * planes};
     if (gx)
       if (int k = rows_product<T>(f, dm, wi, 1, true, f.hidden, f.c, nullptr, nullptr, (T *)gx + r * f.c)) return k;
@@ -894,7 +974,7 @@ size_t scratch_bytes_for(const Ff &f, bool back) {
   size_t b = 256 + operand_bytes(f.type, 2ll * f.hidden, f.c) + operand_bytes(f.type, f.c_out, f.hidden) + operand_bytes(f.type, most, f.c);
   if (!back) return b + hidden;
   const size_t size_in = 2 * (size_t)f.hidden * f.c, size_out = (size_t)f.c_out * f.hidden;
-  b += operand_bytes(f.type, most, f.c_out) + 3 * hidden + 512;
+  b += operand_bytes(f.type, most, f.c_out) + 3 * hidden + 512 + (f.type == SSC_PREC_FP32 ? align_up((size_t)most * pitch_of(f.hidden) * sizeof(float), 256) : 0);
   b += align_up(filter_splits(most, 2, f.hidden, f.c) * size_in * 4, 256) + align_up(filter_splits(most, 1, f.c_out, f.hidden) * size_out * 4, 256);
   return b + align_up((size_t)kColumnShares * 8 * f.hidden, 256) + align_up((size_t)kColumnShares * 4 * f.c_out, 256);
 }
