@@ -13,6 +13,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "ssc_common.cuh"
 #include "ssc_rows_act.cuh"
 #include "ssc_tc_ptx.cuh"
@@ -20,19 +22,23 @@
 namespace ssc {
 namespace {
 
+enum Epilogue { kGate, kBack, kRows, kPart };
 constexpr int kBox = 64;                      // TMA boxes: 64 x 64 elements, 128-byte rows
 constexpr uint32_t kBoxBytes = kBox * kBox * 2;
 constexpr int kTileM = 256;                   // of a pair of CTAs, half of it each
 constexpr uint32_t kStageBytes = 4 * kBoxBytes;     // two boxes of A, up to two of B
-constexpr int kStages = 6;
+template <int EPI>
+constexpr int kStages = EPI == kBack ? 4 : 5;
+template <int EPI>
+constexpr uint32_t kOutBytes = EPI == kBack ? 98304 : 65536;      // rows on their way out, a share for each of the warps that empty accumulators
 // Warps: TMA, products, tensor memory, an idle one, then those for the accumulators: sixteen, eight where sums in registers (LONG) need the room.
 template <bool LONG>
 constexpr int kSides = LONG ? 2 : 4;                        // shares of a tile's columns
 template <bool LONG>
 constexpr int kThreads = 128 + 128 * kSides<LONG>;
-constexpr uint32_t kSmemBytes = kStages * kStageBytes + 1024;
+template <int EPI>
+constexpr uint32_t kSmemBytes = kStages<EPI> * kStageBytes + kOutBytes<EPI> + 1024;
 
-enum Epilogue { kGate, kBack, kRows, kPart };
 enum Half { kNone, kByK, kByBox, kByM };      // what chooses between the two matrices of an operand (gate and up)
 
 struct Segment {
@@ -46,6 +52,7 @@ struct Segment {
 };
 struct FfMaps {
   CUtensorMap a[2], b[2];
+  CUtensorMap out[2];        // of out and out2, where rows can be stored by boxes
 };
 struct FfParams {
   Segment seg[2];
@@ -58,7 +65,8 @@ struct FfParams {
   const void *residual;                        // kRows: rows of T; kBack of float32: dh [rows][pitch]
   void *out, *out2;                            // kGate: h; kBack: h, dg|du; kRows: result; kPart: float [splits][rows of all][cols]
   int pitch;                                   // of out
-  size_t plane, plane2;                        // elements from one plane to the next (of out, of a matrix of out2)
+  size_t plane;                                // kPart: elements of a share
+  int boxes;                                   // out (and out2) are stored by boxes (maps.out), else from registers
   int vec;                                     // rows of out (and residual) are aligned to 32 bytes
   int accumulate;                              // kPart: add to what is there
   int32_t *status, *alarm;
@@ -124,21 +132,61 @@ __device__ __forceinline__ void planes_of(float v, float &a, float &b, float &c)
   b = fabsf(a) < INFINITY ? __bfloat162float(__float2bfloat16_rn(r)) : 0.f;
   c = fabsf(a) < INFINITY ? r - b : 0.f;
 }
-// 16 columns of an intermediate: rows of T, or the planes of float32 ones.  (pitch and buffers are aligned)
-template <class T>
-__device__ __forceinline__ void put_hidden(void *base, size_t at, size_t plane, const float *v, int left) {
-  if (sizeof(T) == 2) {
-    put16<T>((T *)base + at, v, left, 1);
-  } else {
-    float a[16], b[16], c[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) planes_of(v[i], a[i], b[i], c[i]);
-    __nv_bfloat16 *p = (__nv_bfloat16 *)base + at;
-    put16<__nv_bfloat16>(p, a, left, 1);
-    put16<__nv_bfloat16>(p + plane, b, left, 1);
-    put16<__nv_bfloat16>(p + 2 * plane, c, left, 1);
+
+// A warp's way out of 32 rows of up to 32 columns: each lane puts its row's 16 columns into the warp's shared memory, one lane sends the box off.  Rows
+// from registers cost as much time as the products did (131072 rows 512 -> 2048 in bf16: 549 us, 394 without them).
+// Boxes of 32 columns: rows of 64 bytes (16-bit) or 128 (float32), or of 16 columns, 32 bytes; swizzled as the copy engine has it, which
+// keeps lanes on different banks.
+struct Outbox {
+  uint32_t at;             // the warp's shared memory: slots taken in turn
+  uint32_t slot, slots, slot_bytes;
+  __device__ __forceinline__ void open(uint32_t where, uint32_t size, uint32_t each) {
+    at = where;
+    slot_bytes = each;
+    slots = size / each;
+    slot = 0;
   }
-}
+  // Room for one more box (the whole warp): what was sent last may still be read, the slots before it not.
+  __device__ __forceinline__ uint32_t room() {
+    if ((threadIdx.x & 31) == 0) {
+      if (slots == 1) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      else if (slots < 4) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+      else asm volatile("cp.async.bulk.wait_group.read 3;" ::: "memory");
+    }
+    __syncwarp();
+    const uint32_t here = at + slot * slot_bytes;
+    if (++slot == slots) slot = 0;
+    return here;
+  }
+  // 16 columns (half 0 or 1 of the box) of the lane's row.
+  template <class V, int COLS = 32>
+  __device__ __forceinline__ void put(uint32_t box, int half, const float *v) {
+    const uint32_t lane = threadIdx.x & 31;
+    constexpr int N = 16 / sizeof(V);
+    constexpr uint32_t row_bytes = COLS * sizeof(V), mask = row_bytes / 16 - 1;
+    const uint32_t row = box + lane * row_bytes, turn = lane / (128 / row_bytes) & mask;
+#pragma unroll
+    for (int i = 0; i < 16 / N; ++i) {
+      struct alignas(16) { V v[N]; } k;
+#pragma unroll
+      for (int q = 0; q < N; ++q) k.v[q] = (V)v[i * N + q];
+      const uint32_t *w = (const uint32_t *)&k, to = row + (((uint32_t)(half * (16 / N) + i) ^ turn) << 4);
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+    }
+  }
+  __device__ __forceinline__ void send(uint32_t box, const CUtensorMap *map, int x, int y, int z) {
+    fence_async_smem();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) {
+      asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(x), "r"(y), "r"(z), "r"(box) : "memory");
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+  }
+  __device__ __forceinline__ void close() {
+    if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
+  }
+};
 __device__ __forceinline__ void tmem_floats(float *v, uint32_t addr) { tmem_ld16((uint32_t *)v, addr); }
 __device__ __forceinline__ void tmem_arrived() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
@@ -201,51 +249,129 @@ __device__ __forceinline__ int parts_of(const FfParams &p, int split) {
 __device__ __forceinline__ void stored_dh(const FfParams &p, int row, int n, float *d) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) d[i] = 0.f;
-  if (row < p.rows) add16<float>(d, (const float *)p.residual + (size_t)row * p.pitch + n, p.cols - n, 1);
+  if (row < p.rows && n < p.cols) add16<float>(d, (const float *)p.residual + (size_t)row * p.pitch + n, p.cols - n, 1);
 }
 
-// 16 columns from column n on of a row of the result: v (kGate: gate, u: up; kBack: d = dh too).
-template <int EPI, class T>
-__device__ __forceinline__ void finish(const FfParams &p, int split, int half_m, int row, int n, float *v, float *u, float *d) {
-  const int left = p.cols - n;
-  if (EPI == kGate || EPI == kBack) {
-    if (p.bias) {
-      add16<T>(v, (const T *)p.bias + n, left, 0);
-      add16<T>(u, (const T *)p.bias + p.cols + n, left, 0);
+// A plane of 32 columns of hidden rows (16-bit, or one of the three of float32 rows) goes out as a box.
+template <class T>
+__device__ __forceinline__ void send_hidden(Outbox &box, const CUtensorMap *map, const float (*v)[16], int n, int row0, int z, int planes_apart) {
+  if (sizeof(T) == 2) {
+    const uint32_t at = box.room();
+    box.put<T>(at, 0, v[0]);
+    box.put<T>(at, 1, v[1]);
+    box.send(at, map, n, row0, z);
+  } else {
+#pragma unroll
+    for (int plane = 0; plane < 3; ++plane) {
+      const uint32_t at = box.room();
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float w[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float a, b, c;
+          planes_of(v[h][i], a, b, c);
+          w[i] = plane == 0 ? a : plane == 1 ? b : c;
+        }
+        box.put<__nv_bfloat16>(at, h, w);
+      }
+      box.send(at, map, n, row0, z + plane * planes_apart);
     }
   }
+}
+
+// 16 columns (half `half` of a box) of a warp's rows, row0 the first of them: gate v, up u, dh d.
+template <class T>
+__device__ __forceinline__ void finish_back(const FfParams &p, const FfMaps &maps, Outbox &box, int row0, int n, int half, float *v, float *u, float *d) {
+  const int left = p.cols - n;
+  if (p.bias && left > 0) {
+    add16<T>(v, (const T *)p.bias + n, left, 0);
+    add16<T>(u, (const T *)p.bias + p.cols + n, left, 0);
+  }
+  float s[16], h[16];
+  act_slopes<sizeof(T) == 4, 16>(v, s, p.act);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) h[i] = v[i];
+  multiply<16>(h, u);           // act(g) u
+  multiply<16>(u, s);
+  multiply<16>(u, d);           // dh u act'(g)
+  multiply<16>(v, d);           // dh act(g)
+  if constexpr (sizeof(T) == 2) {
+    if (half == 0) {            // three boxes at a time
+      if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      __syncwarp();
+    }
+    box.put<T>(box.at, half, h);
+    box.put<T>(box.at + 2048, half, u);
+    box.put<T>(box.at + 4096, half, v);
+    if (half == 1) {
+      box.send(box.at, &maps.out[0], n - 16, row0, 0);
+      box.send(box.at + 2048, &maps.out[1], n - 16, row0, 0);
+      box.send(box.at + 4096, &maps.out[1], n - 16, row0, 1);
+    }
+  } else if (left > 0) {
+#pragma unroll
+    for (int o = 0; o < 3; ++o) {
+      const float *from = o == 0 ? h : o == 1 ? u : v;
+#pragma unroll
+      for (int plane = 0; plane < 3; ++plane) {
+        float w[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float a, b, c;
+          planes_of(from[i], a, b, c);
+          w[i] = plane == 0 ? a : plane == 1 ? b : c;
+        }
+        const uint32_t at = box.room();
+        box.put<__nv_bfloat16, 16>(at, 0, w);
+        box.send(at, o == 0 ? &maps.out[0] : &maps.out[1], n, row0, o == 0 ? plane : 2 * plane + o - 1);
+      }
+    }
+  }
+}
+
+// 32 columns from column n on of a warp's rows of the result, two times 16: v (kGate: gate, u: up).
+template <int EPI, class T>
+__device__ __forceinline__ void finish(const FfParams &p, const FfMaps &maps, Outbox &box, int split, int half_m, int row0, int n, float (*v)[16], float (*u)[16]) {
+  const int row = row0 + (threadIdx.x & 31);
   if (EPI == kGate) {
-    act_values<sizeof(T) == 4, 16>(v, p.act);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] *= u[i];
-    if (row < p.rows) put_hidden<T>(p.out, (size_t)row * p.pitch + n, p.plane, v, left);
-  } else if (EPI == kBack) {
-    float s[16], h[16];
-    act_slopes<sizeof(T) == 4, 16>(v, s, p.act);
+    for (int q = 0; q < 2; ++q) {
+      const int left = p.cols - n - 16 * q;
+      if (p.bias && left > 0) {
+        add16<T>(v[q], (const T *)p.bias + n + 16 * q, left, 0);
+        add16<T>(u[q], (const T *)p.bias + p.cols + n + 16 * q, left, 0);
+      }
+      act_values<sizeof(T) == 4, 16>(v[q], p.act);
+      multiply<16>(v[q], u[q]);
+    }
+    send_hidden<T>(box, &maps.out[0], v, n, row0, 0, 1);
+    return;
+  }
+  if (EPI == kRows) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float a = v[i];
-      h[i] = a * u[i];
-      v[i] = d[i] * u[i] * s[i];
-      u[i] = d[i] * a;
+    for (int q = 0; q < 2; ++q) {
+      const int left = p.cols - n - 16 * q;
+      if (left <= 0) continue;
+      if (p.bias) add16<T>(v[q], (const T *)p.bias + n + 16 * q, left, 0);
+      if (p.residual && row < p.rows) add16<T>(v[q], (const T *)p.residual + (size_t)row * p.pitch + n + 16 * q, left, p.vec);
     }
-    if (row < p.rows) {
-      const size_t at = (size_t)row * p.pitch + n;
-      put_hidden<T>(p.out, at, p.plane, h, left);
-      put_hidden<T>(p.out2, at, 2 * p.plane2, v, left);
-      put_hidden<T>(p.out2, p.plane2 + at, 2 * p.plane2, u, left);
-    }
-  } else if (EPI == kRows) {
-    if (p.bias) add16<T>(v, (const T *)p.bias + n, left, 0);
-    if (row < p.rows) {
-      const size_t at = (size_t)row * p.pitch + n;
-      if (p.residual) add16<T>(v, (const T *)p.residual + at, left, p.vec);
-      put16<T>((T *)p.out + at, v, left, p.vec);
-    }
+  }
+  using V = std::conditional_t<EPI == kPart, float, T>;
+  if (p.boxes) {
+    const uint32_t at = box.room();
+    box.put<V>(at, 0, v[0]);
+    box.put<V>(at, 1, v[1]);
+    box.send(at, &maps.out[0], n, row0, EPI == kPart ? split * (p.m_half < p.tiles_m ? 2 : 1) + half_m : 0);
   } else if (row < p.rows) {
-    float *o = (float *)p.out + (size_t)split * p.plane + ((size_t)half_m * p.rows + row) * p.pitch + n;
-    if (p.accumulate) add16<float>(v, o, left, p.vec);
-    put16<float>(o, v, left, p.vec);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int left = p.cols - n - 16 * q;
+      if (left <= 0) continue;
+      V *o = (V *)p.out + (EPI == kPart ? (size_t)split * p.plane : 0) + ((size_t)half_m * p.rows + row) * p.pitch + n + 16 * q;
+      if (EPI == kPart && p.accumulate) add16<V>(v[q], o, left, p.vec);
+      put16<V>(o, v[q], left, p.vec);
+    }
   }
 }
 
@@ -254,14 +380,14 @@ template <int EPI, class T, bool LONG>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads<LONG>, 1) ff_gemm_kernel(const __grid_constant__ FfMaps maps, const FfParams p) {
   after_previous();
   extern __shared__ uint8_t raw[];
-  __shared__ alignas(8) uint64_t bars[2 * kStages + 5];
+  __shared__ alignas(8) uint64_t bars[2 * kStages<EPI> + 5];
   __shared__ uint32_t tmem_base;
   __shared__ volatile int abort_flag;
   const uint32_t ring = (smem_u32(raw) + 1023u) & ~1023u;
-  const uint32_t full = smem_u32(bars), empty = full + 8 * kStages, acc_full = empty + 8 * kStages, acc_empty = acc_full + 16, done = acc_empty + 16;
+  const uint32_t full = smem_u32(bars), empty = full + 8 * kStages<EPI>, acc_full = empty + 8 * kStages<EPI>, acc_empty = acc_full + 16, done = acc_empty + 16;
   const int warp = warp_id(), rank = blockIdx.x & 1;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < kStages<EPI>; ++s) {
       mbar_init(full + 8 * s, 1);                       // the first CTA's: both CTAs' boxes count there
       mbar_init(empty + 8 * s, 1);
     }
@@ -332,7 +458,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads<LONG>, 1) f
                   if (s.boxes_b == 2) tma_box(at + 3 * kBoxBytes, map_b, kk, n0 + kBox, zb, bar);
                 }
               }
-              if (++slot == kStages) slot = 0, phase ^= 1;
+              if (++slot == kStages<EPI>) slot = 0, phase ^= 1;
             }
             i += run;
             kb += run;
@@ -341,7 +467,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads<LONG>, 1) f
         }
     }
     if (abort_flag && rank == 0)      // copies in flight, the other CTA's too, arrive before the blocks leave
-      for (uint32_t s = step > kStages ? step - kStages : 0; s < step; ++s) mbar_wait_drain(full + 8 * (s % kStages), (s / kStages) & 1);
+      for (uint32_t s = step > kStages<EPI> ? step - kStages<EPI> : 0; s < step; ++s) mbar_wait_drain(full + 8 * (s % kStages<EPI>), (s / kStages<EPI>) & 1);
   } else if (warp == 1 && rank == 0) {
     // products
     uint32_t slot = 0, phase = 0, turn = 0;
@@ -373,32 +499,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads<LONG>, 1) f
               for (uint32_t q = 0; q < 4; ++q) mma_pair<true>(d, a + q * ua, b + q * ub, idesc, (i | (int)q) != 0 ? 1u : 0u);
               mma_commit_pair(empty + 8 * slot);
             }
-            if (++slot == kStages) slot = 0, phase ^= 1;
+            if (++slot == kStages<EPI>) slot = 0, phase ^= 1;
           }
         }
         if (ok && elect_one()) mma_commit_pair(acc_full + 8 * buf);
       }
     }
   } else if (warp >= 4) {
-    // accumulators: a thread has a row and a share of a tile's columns, kGroups times 16 of them from kSets products
-    constexpr int kSets = EPI == kGate ? 2 : kThree ? 3 : EPI == kBack ? 2 : 1, kGroups = kSets == 2 ? 4 : 8;
+    // accumulators: a thread has a row and a share of a tile's columns, kGroups times 32 of them from kSets products
+    constexpr int kSets = EPI == kGate ? 2 : kThree ? 3 : EPI == kBack ? 2 : 1, kGroups = kSets == 2 ? 2 : 4;      // of 32
     const int quad = warp & 3, side = (warp - 4) >> 2, lane = threadIdx.x & 31;
     const uint32_t lanes = (uint32_t)(32 * quad) << 16, empty_there = peer_address(acc_empty, 0);
+    constexpr uint32_t kShare = kOutBytes<EPI> / (4 * kSides<LONG>);
+    Outbox box;
+    box.open(ring + kStages<EPI> * kStageBytes + (warp - 4) * kShare, kShare, EPI == kBack && sizeof(T) == 4 ? 1024 : EPI == kPart || (EPI == kRows && sizeof(T) == 4) ? 4096 : 2048);
     uint32_t turn = 0;
     bool ok = true;
     for (Walk k(p); k.more(p) && ok; k.next(p)) {
       const int half_m = k.m >= p.m_half ? 1 : 0, m0 = (k.m - half_m * p.m_half) * kTileM + rank * (kTileM / 2), n0 = k.n * p.step_n;
-      const int row = m0 + 32 * quad + lane, each = p.step_n / kSides<LONG>;
+      const int row0 = m0 + 32 * quad, each = p.step_n / kSides<LONG>;
       int first, blocks;
       share_of_sum(p, 0, k.split, first, blocks);
       if constexpr (LONG) {
-        float sum[kSets][kGroups][16];
+        float sum[kSets][kGroups][2][16];
 #pragma unroll
-        for (int s = 0; s < kSets; ++s)
-#pragma unroll
-          for (int g = 0; g < kGroups; ++g)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) sum[s][g][i] = 0.f;
+        for (int i = 0; i < kSets * kGroups * 32; ++i) (&sum[0][0][0][0])[i] = 0.f;
         const int parts = parts_of(p, k.split);
         for (int part = 0; part < parts && ok; ++part, ++turn) {
           const uint32_t buf = turn & 1, acc = tmem + buf * 256 + lanes;
@@ -409,13 +534,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads<LONG>, 1) f
 #pragma unroll
             for (int s = 0; s < kSets; ++s)
 #pragma unroll
-              for (int g = 0; g < kGroups; ++g)
+              for (int g = 0; g < 2 * kGroups; ++g)
                 if (16 * g < each) {
                   float v[16];
                   tmem_floats(v, acc + s * p.step_n + side * each + 16 * g);
                   tmem_arrived();
 #pragma unroll
-                  for (int i = 0; i < 16; ++i) sum[s][g][i] += v[i];
+                  for (int i = 0; i < 16; ++i) sum[s][g / 2][g % 2][i] += v[i];
                 }
           }
           tc_fence_before();
@@ -425,11 +550,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads<LONG>, 1) f
         if (!ok) break;
 #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
-          const int n = n0 + side * each + 16 * g;
-          if (16 * g < each && n < p.cols) {
-            float d[16];
-            if (EPI == kBack) stored_dh(p, row, n, d);
-            finish<EPI, T>(p, k.split, half_m, row, n, sum[0][g], sum[kSets > 1 ? 1 : 0][g], d);
+          const int n = n0 + side * each + 32 * g;
+          if (32 * g < each && n < p.cols) {
+            if constexpr (EPI == kBack) {
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                float d[16];
+                stored_dh(p, row0 + lane, n + 16 * q, d);
+                finish_back<T>(p, maps, box, row0, n + 16 * q, q, sum[0][g][q], sum[1][g][q], d);
+              }
+            } else {
+              finish<EPI, T>(p, maps, box, k.split, half_m, row0, n, sum[0][g], sum[kSets > 1 ? 1 : 0][g]);
+            }
           }
         }
       } else {
@@ -437,31 +569,53 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads<LONG>, 1) f
         ok = mbar_wait_uniform(acc_full + 8 * buf, (turn >> 1) & 1, &abort_flag);
         if (!ok) break;
         tc_fence_after();
-        for (int c = side * each; c < (side + 1) * each; c += 16) {
+        for (int c = side * each; c < (side + 1) * each; c += 32) {
           const int n = n0 + c;
           if (n >= p.cols) break;
-          float v[kSets][16];
+          const bool last = c + 32 >= (side + 1) * each || n + 32 >= p.cols;      // behind it the accumulator is free
+          if constexpr (EPI == kBack) {
 #pragma unroll
-          for (int s = 0; s < kSets; ++s) tmem_floats(v[s], kThree && s == 2 ? tmem + 256 + buf * 128 + lanes + c : acc + s * p.step_n + c);
-          tmem_arrived();
-          if (EPI == kPart && blocks == 0) {
+            for (int q = 0; q < 2; ++q) {
+              float v[3][16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[0][i] = 0.f;      // (an empty share)
-          }
-          if (EPI == kBack && !kThree) {
-            float d[16];
-            stored_dh(p, row, n, d);
-            finish<EPI, T>(p, k.split, half_m, row, n, v[0], v[kSets > 1 ? 1 : 0], d);
+              for (int s = 0; s < kSets; ++s) tmem_floats(v[s], (s == 2 ? tmem + 256 + buf * 128 + lanes : acc + s * p.step_n) + c + 16 * q);
+              tmem_arrived();
+              if (q == 1 && last) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_there(empty_there + 8 * buf);
+              }
+              if (!kThree) stored_dh(p, row0 + lane, n + 16 * q, v[2]);
+              finish_back<T>(p, maps, box, row0, n + 16 * q, q, v[0], v[1], v[2]);
+            }
           } else {
-            finish<EPI, T>(p, k.split, half_m, row, n, v[0], v[kSets > 1 ? 1 : 0], v[kSets > 2 ? 2 : 0]);
+            float v[kSets][2][16];
+#pragma unroll
+            for (int s = 0; s < kSets; ++s)
+#pragma unroll
+              for (int q = 0; q < 2; ++q) tmem_floats(v[s][q], acc + s * p.step_n + c + 16 * q);
+            tmem_arrived();
+            if (last) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) arrive_there(empty_there + 8 * buf);
+            }
+            if (EPI == kPart && blocks == 0) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) (&v[0][0][0])[i] = 0.f;      // (an empty share)
+            }
+            finish<EPI, T>(p, maps, box, k.split, half_m, row0, n, v[0], v[kSets > 1 ? 1 : 0]);
           }
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) arrive_there(empty_there + 8 * buf);
+        if (n0 + side * each >= p.cols) {                             // (no columns here)
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_there(empty_there + 8 * buf);
+        }
         ++turn;
       }
     }
+    box.close();
   }
   tc_fence_before();
   __syncthreads();
@@ -657,7 +811,21 @@ int make_map(CUtensorMap *map, const Matrix &m, bool f16) {
   return SSC_OK;
 }
 
+// Where boxes of 32 rows and 32 (or 16) columns go; false: rows of this width or at this address cannot be (no error).
+bool make_out_map(CUtensorMap *map, const void *p, long long rows, int cols, int pitch, int planes, int type, int width = 32) {
+  const int size = type == SSC_PREC_FP32 ? 4 : 2;
+  const EncodeFn fn = encode_fn();
+  if (fn == nullptr || ((uintptr_t)p & 15) != 0 || pitch * size % 16 != 0) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+  const cuuint64_t strides[2] = {(cuuint64_t)pitch * size, (cuuint64_t)pitch * size * (cuuint64_t)rows};
+  const cuuint32_t box[3] = {(cuuint32_t)width, 32, 1}, each[3] = {1, 1, 1};
+  const CUtensorMapDataType kind = type == SSC_PREC_FP32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == SSC_PREC_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return fn(map, kind, 3, const_cast<void *>(p), dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, width * size == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : width * size == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B,
+            CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int pitch_of(int cols) { return (cols + 15) & ~15; }     // rows of whole sectors
+int hidden_type(int type) { return type == SSC_PREC_F16 ? SSC_PREC_F16 : SSC_PREC_BF16; }
 int planes_for(int type) { return type == SSC_PREC_FP32 ? 3 : 1; }
 
 // Scratch is handed out piece by piece; a null base counts the bytes.
@@ -719,8 +887,8 @@ int launch_gemm(Ff &f, const FfMaps &maps, FfParams &p) {
       kernel = ff_gemm_kernel<EPI, T, true>;
       threads = kThreads<true>;
     }
-  cudaError_t e = allow_smem((const void *)kernel, kSmemBytes);
-  if (e == cudaSuccess) e = launch_ready(kernel, dim3(grid), dim3(threads), kSmemBytes, f.st, maps, p);
+  cudaError_t e = allow_smem((const void *)kernel, kSmemBytes<EPI>);
+  if (e == cudaSuccess) e = launch_ready(kernel, dim3(grid), dim3(threads), kSmemBytes<EPI>, f.st, maps, p);
   if (e != cudaSuccess) return fail(SSC_ERR_CUDA, "gated_ff: %s", cudaGetErrorString(e));
   ++f.launches;
   return SSC_OK;
@@ -766,6 +934,7 @@ int rows_product(Ff &f, const Matrix &a, const Matrix &b, int b_mn, bool halves,
   p.residual = residual;
   p.out = out;
   p.vec = p.pitch % (32 / (int)sizeof(T)) == 0 && (((uintptr_t)out | (uintptr_t)residual) & 31) == 0;
+  p.boxes = make_out_map(&maps.out[0], out, p.rows, cols, p.pitch, 1, f.type);
   return launch_gemm<kRows, T>(f, maps, p);
 }
 
@@ -783,13 +952,13 @@ int gate_product(Ff &f, const Matrix &x, const Matrix &w_in, const void *b_in, v
   p.rows = (int)x.rows;
   p.cols = f.hidden;
   p.pitch = pitch_of(f.hidden);
-  p.plane = (size_t)p.rows * p.pitch;
   p.tiles_m = ceil_div(p.rows, kTileM);
   p.m_half = 1 << 30;
   p.tiles_n = ceil_div(f.hidden, p.step_n);
   p.splits = 1;
   p.bias = b_in;
   p.out = h;
+  if (!make_out_map(&maps.out[0], h, p.rows, f.hidden, p.pitch, planes_for(f.type), hidden_type(f.type))) return fail(SSC_ERR_CUDA, "gated_ff: no tensor map for the hidden rows");
   return launch_gemm<kGate, T>(f, maps, p);
 }
 
@@ -816,7 +985,6 @@ int back_product(Ff &f, const Matrix &x, const Matrix &w_in, const Matrix &gy, c
   p.rows = (int)x.rows;
   p.cols = f.hidden;
   p.pitch = pitch_of(f.hidden);
-  p.plane = p.plane2 = (size_t)p.rows * p.pitch;
   p.tiles_m = ceil_div(p.rows, kTileM);
   p.m_half = 1 << 30;
   p.tiles_n = ceil_div(f.hidden, p.step_n);
@@ -825,6 +993,10 @@ int back_product(Ff &f, const Matrix &x, const Matrix &w_in, const Matrix &gy, c
   p.residual = dh;
   p.out = h;
   p.out2 = dgu;
+  const int width = sizeof(T) == 2 ? 32 : 16;      // (float32: nine planes of 16 columns at a time)
+  if (!make_out_map(&maps.out[0], h, p.rows, f.hidden, p.pitch, planes_for(f.type), hidden_type(f.type), width) ||
+      !make_out_map(&maps.out[1], dgu, p.rows, f.hidden, p.pitch, 2 * planes_for(f.type), hidden_type(f.type), width))
+    return fail(SSC_ERR_CUDA, "gated_ff: no tensor map for the hidden rows");
   return launch_gemm<kBack, T>(f, maps, p);
 }
 
@@ -858,6 +1030,7 @@ int filter_product(Ff &f, const Matrix &a, const Matrix &b, int halves, int m, i
   p.out = part;
   p.vec = cols % 8 == 0;
   p.accumulate = accumulate;
+  p.boxes = !accumulate && make_out_map(&maps.out[0], part, m, cols, cols, halves * splits, SSC_PREC_FP32);
   return launch_gemm<kPart, T>(f, maps, p);
 }
 

@@ -9,24 +9,43 @@
 // it cost five times the arithmetic.
 #pragma once
 #include "ssc_act.cuh"
+#include "ssc_common.cuh"
 
 namespace ssc {
 
+// 2^v; results below 2^-126 are zero (the instruction that keeps them takes three more).
+__device__ __forceinline__ float exp2_quick(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
 template <bool EXACT, int N>
 __device__ __forceinline__ void sigmoids(const float *z, float *s) {
-  float d[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) d[i] = fminf(1.0f + __expf(-z[i]), 0x1p62f);      // (a number for NaN too: the neighbour keeps its value)
+  const f32x2 one = pair_of(1.0f, 1.0f), log2e = pair_of(-1.44269504f, -1.44269504f);
 #pragma unroll
   for (int i = 0; i + 1 < N; i += 2) {
-    const float p = d[i] * d[i + 1];
+    const float2 x = halves(mul_pair(pair_of(z[i], z[i + 1]), log2e));
+    const float2 e = halves(add_pair(pair_of(exp2_quick(x.x), exp2_quick(x.y)), one));
+    const float d0 = fminf(e.x, 0x1p62f), d1 = fminf(e.y, 0x1p62f);      // (a number for NaN too: the neighbour keeps its value)
+    const float p = d0 * d1;
     float r;
     if (EXACT) r = quick_reciprocal(p);
     else asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(p));
-    s[i] = r * d[i + 1];
-    s[i + 1] = r * d[i];
+    s[i] = r * d1;
+    s[i + 1] = r * d0;
   }
-  if (N % 2 == 1) s[N - 1] = quick_reciprocal(d[N - 1]);
+  if (N % 2 == 1) s[N - 1] = quick_reciprocal(fminf(1.0f + exp2_quick(-1.44269504f * z[N - 1]), 0x1p62f));
+}
+// a[i] *= b[i]
+template <int N>
+__device__ __forceinline__ void multiply(float *a, const float *b) {
+#pragma unroll
+  for (int i = 0; i + 1 < N; i += 2) {
+    const float2 p = halves(mul_pair(pair_of(a[i], a[i + 1]), pair_of(b[i], b[i + 1])));
+    a[i] = p.x;
+    a[i + 1] = p.y;
+  }
+  if (N % 2 == 1) a[N - 1] *= b[N - 1];
 }
 __device__ __forceinline__ float normal_share(float z) { return 0.5f * (1.0f + erff(z * 0.70710678118654752f)); }
 
@@ -45,8 +64,7 @@ __device__ __forceinline__ void act_values(float *v, int kind) {
       break;
     case 3:
       sigmoids<EXACT, N>(v, s);
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] *= s[i];
+      multiply<N>(v, s);
       break;
     case 4:
 #pragma unroll
@@ -77,12 +95,9 @@ __device__ __forceinline__ void act_slopes(float *v, float *s, int kind) {
       break;
     case 3:
       sigmoids<EXACT, N>(v, s);
+      multiply<N>(v, s);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float a = v[i] * s[i];
-        s[i] = fmaf(a, 1.f - s[i], s[i]);
-        v[i] = a;
-      }
+      for (int i = 0; i < N; ++i) s[i] = fmaf(v[i], 1.f - s[i], s[i]);
       break;
     // (the density (2 pi)^-1/2 exp(-z^2 / 2))
     case 4:
