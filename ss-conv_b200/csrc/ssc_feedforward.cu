@@ -158,9 +158,9 @@ struct Outbox {
     if (++slot == slots) slot = 0;
     return here;
   }
-  // 16 columns (half 0 or 1 of the box) of the lane's row.
+  // 16 columns (part 0, 1 ... of the box) of the lane's row.
   template <class V, int COLS = 32>
-  __device__ __forceinline__ void put(uint32_t box, int half, const float *v) {
+  __device__ __forceinline__ void put(uint32_t box, int part, const float *v) {
     const uint32_t lane = threadIdx.x & 31;
     constexpr int N = 16 / sizeof(V);
     constexpr uint32_t row_bytes = COLS * sizeof(V), mask = row_bytes / 16 - 1;
@@ -170,7 +170,7 @@ struct Outbox {
       struct alignas(16) { V v[N]; } k;
 #pragma unroll
       for (int q = 0; q < N; ++q) k.v[q] = (V)v[i * N + q];
-      const uint32_t *w = (const uint32_t *)&k, to = row + (((uint32_t)(half * (16 / N) + i) ^ turn) << 4);
+      const uint32_t *w = (const uint32_t *)&k, to = row + (((uint32_t)(part * (16 / N) + i) ^ turn) << 4);
       asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
     }
   }
@@ -633,6 +633,212 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads<LONG>, 1) f
   cluster_sync();
 }
 
+// Gate and up of rows that are narrow enough to stay in shared memory: a pair of CTAs keeps its 256 rows of x and goes through the hidden columns,
+// 64 at a time, with the weights alone coming by.  That halves what is fetched from L2, and accumulators of 128 columns leave room for four
+// in turn with a group of warps for each, so that products, special functions and stores of different tiles run side by side.  65536 rows 256 -> 1024
+// in bf16: by tiles of 128 hidden columns with rows fetched for each 104 us.  (All sixteen warps on one tile after the other wait for one chain of
+// instructions, 117 us; rows of 32 bytes on their way out keep the copy engine busy, 86; dh as a third product leaves room for neither four
+// accumulators nor wide boxes, 180 instead of 169.)
+struct HiddenParams {
+  int rows, cols;                  // cols: hidden
+  int blocks;                      // of 64 along c
+  int pairs;                       // of planes: 1 or 6
+  int tiles_m, tiles_n, chunks;    // 256 rows; 64 columns; shares of the columns a pair goes through with one set of rows
+  int act, stages;
+  const void *bias;
+  uint32_t idesc;
+  int32_t *status, *alarm;
+};
+struct HiddenMaps {
+  CUtensorMap x, w_in, h;          // h: boxes of 64 columns (32: planes)
+};
+constexpr int kKeep = 6;           // blocks of 128 x 64 that stay, at most; the ring needs the rest
+constexpr uint32_t kBlockBytes = 2 * kBoxBytes;
+// A step brings two blocks of Win': what the two warps that issue do around a step costs as much as the products of one block.
+constexpr uint32_t kStepBytes = 2 * kBoxBytes;
+constexpr int kHiddenStages = 6;   // at most
+constexpr uint32_t kHiddenOut = 65536, kHiddenRoom = 230400;
+constexpr int kHiddenThreads = 640;
+// Pairs of planes (kPlaneA): the last one that a plane of A is in.
+__constant__ const int8_t kLastPair[3] = {5, 3, 0};
+
+template <class T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHiddenThreads, 1) ff_hidden_kernel(const __grid_constant__ HiddenMaps maps, const HiddenParams p) {
+  after_previous();
+  constexpr int kBufs = 4, kBufCols = 128;
+  extern __shared__ uint8_t raw[];
+  __shared__ alignas(8) uint64_t bars[2 * kHiddenStages + 2 * kKeep + 2 * kBufs + 1];
+  __shared__ uint32_t tmem_base;
+  __shared__ volatile int abort_flag;
+  const uint32_t outs = (smem_u32(raw) + 1023u) & ~1023u, keep = outs + kHiddenOut, ring = keep + p.blocks * (p.pairs == 1 ? 1 : 3) * kBlockBytes;
+  const uint32_t full = smem_u32(bars), empty = full + 8 * kHiddenStages, kept = empty + 8 * kHiddenStages, free_ = kept + 8 * kKeep, acc_full = free_ + 8 * kKeep,
+                 acc_empty = acc_full + 8 * kBufs, done = acc_empty + 8 * kBufs;
+  const int warp = warp_id(), rank = blockIdx.x & 1, units = p.tiles_m * p.chunks, stride = gridDim.x >> 1, S = p.stages;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2 * kHiddenStages + 2 * kKeep + kBufs; ++i) mbar_init(full + 8 * i, 1);
+    for (int b = 0; b < kBufs; ++b) mbar_init(acc_empty + 8 * b, 8);      // (the first CTA's: both CTAs' warps)
+    mbar_init(done, 1);
+    abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_base)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base;
+
+  if (warp == 0) {
+    // operands: a block of rows comes with the step that needs it first
+    const uint32_t full_there = peer_address(full, 0), kept_there = peer_address(kept, 0);
+    int slot = 0, step = 0;
+    uint32_t phase = 1, unit = 0;
+    bool ok = true;
+    for (int u = blockIdx.x >> 1; u < units && ok; u += stride, ++unit) {
+      const int m = u / p.chunks, c = u - m * p.chunks, m0 = m * kTileM + rank * (kTileM / 2);
+      const int n_begin = c * p.tiles_n / p.chunks, n_end = (c + 1) * p.tiles_n / p.chunks;
+      for (int n = n_begin; n < n_end && ok; ++n)
+        for (int pair = 0; pair < p.pairs && ok; ++pair) {
+          const int pa = p.pairs == 1 ? 0 : kPlaneA[pair], pb = p.pairs == 1 ? 0 : kPlaneB[pair];
+          const bool fetch = n == n_begin && pair < 3;
+          for (int kb = 0; kb < p.blocks && ok; kb += 2, ++step) {
+            const int many = min(2, p.blocks - kb);
+            if (fetch)
+              for (int j = 0; j < many; ++j) {
+                const int at = pa * p.blocks + kb + j;
+                ok = ok && mbar_wait_straight(free_ + 8 * at, (unit & 1) ^ 1, &abort_flag);
+                if (ok && elect_one()) {
+                  if (rank == 0) mbar_expect_tx(kept + 8 * at, 2 * kBlockBytes);
+                  tma_box(keep + at * kBlockBytes, &maps.x, (kb + j) * kBox, m0, pa, kept_there + 8 * at);
+                  tma_box(keep + at * kBlockBytes + kBoxBytes, &maps.x, (kb + j) * kBox, m0 + kBox, pa, kept_there + 8 * at);
+                }
+              }
+            ok = ok && mbar_wait_straight(empty + 8 * slot, phase, &abort_flag);
+            if (ok && elect_one()) {
+              const uint32_t to = ring + slot * kStepBytes, bar = full_there + 8 * slot;
+              if (rank == 0) mbar_expect_tx(full + 8 * slot, many * 2 * kBoxBytes);
+              tma_box(to, &maps.w_in, kb * kBox, n * 64, 2 * pb + rank, bar);
+              if (many == 2) tma_box(to + kBoxBytes, &maps.w_in, (kb + 1) * kBox, n * 64, 2 * pb + rank, bar);
+            }
+            if (++slot == S) slot = 0, phase ^= 1;
+          }
+        }
+    }
+    if (abort_flag && rank == 0) {      // copies in flight, the other CTA's too, arrive before the blocks leave
+      for (int s = max(step - S, 0); s < step; ++s) mbar_wait_drain(full + 8 * (s % S), (s / S) & 1);
+      for (int i = 0; i < p.blocks * (p.pairs == 1 ? 1 : 3); ++i) mbar_wait_drain(kept + 8 * i, (unit & 1) ^ 1);
+    }
+  } else if (warp == 1 && rank == 0) {
+    // products
+    int slot = 0;
+    uint32_t phase = 0, turn = 0, unit = 0;
+    bool ok = true;
+    for (int u = blockIdx.x >> 1; u < units && ok; u += stride, ++unit) {
+      const int c = u % p.chunks, n_begin = c * p.tiles_n / p.chunks, n_end = (c + 1) * p.tiles_n / p.chunks;
+      for (int n = n_begin; n < n_end && ok; ++n, ++turn) {
+        const uint32_t buf = turn % kBufs, d = tmem + buf * kBufCols;
+        ok = mbar_wait_straight_cluster(acc_empty + 8 * buf, ((turn / kBufs) & 1) ^ 1, &abort_flag);
+        tc_fence_after();
+        for (int pair = 0; pair < p.pairs; ++pair) {
+          const int pa = p.pairs == 1 ? 0 : kPlaneA[pair];
+          const bool fetch = n == n_begin && pair < 3, leave = n == n_end - 1 && (p.pairs == 1 || kLastPair[pa] == pair);
+          for (int kb = 0; kb < p.blocks && ok; kb += 2) {
+            const int many = min(2, p.blocks - kb), at = pa * p.blocks + kb;
+            if (fetch)
+              for (int j = 0; j < many; ++j) ok = ok && mbar_wait_straight_cluster(kept + 8 * (at + j), unit & 1, &abort_flag);
+            ok = ok && mbar_wait_straight_cluster(full + 8 * slot, phase, &abort_flag);
+            tc_fence_after();
+            const uint32_t a = operand_lo(keep + at * kBlockBytes, 0), b = operand_lo(ring + slot * kStepBytes, 0);
+            if (ok && elect_one()) {
+              for (int j = 0; j < many; ++j)
+#pragma unroll
+                for (uint32_t q = 0; q < 4; ++q)
+                  mma_pair<true>(d, a + j * (kBlockBytes >> 4) + q * 2, b + j * (kBoxBytes >> 4) + q * 2, p.idesc, (pair | kb | j | (int)q) != 0 ? 1u : 0u);
+              mma_commit_pair(empty + 8 * slot);
+              if (leave)
+                for (int j = 0; j < many; ++j) mma_commit_pair(free_ + 8 * (at + j));
+            }
+            if (++slot == S) slot = 0, phase ^= 1;
+          }
+        }
+        if (ok && elect_one()) mma_commit_pair(acc_full + 8 * buf);
+      }
+    }
+  } else if (warp >= 4) {
+    // accumulators: four warps for each of them, 32 rows and 64 columns to a warp
+    const int quad = warp & 3, group = (warp - 4) >> 2, lane = threadIdx.x & 31;
+    const uint32_t acc = tmem + group * kBufCols + ((uint32_t)(32 * quad) << 16), empty_there = peer_address(acc_empty + 8 * group, 0);
+    constexpr int kWide = sizeof(T) == 2 ? 64 : 32;      // columns of a box
+    Outbox box;
+    box.open(outs + (warp - 4) * (kHiddenOut / 16), kHiddenOut / 16, 32 * 2 * kWide);
+    int turn = 0;
+    bool ok = true;
+    for (int u = blockIdx.x >> 1; u < units && ok; u += stride) {
+      const int m = u / p.chunks, c = u - m * p.chunks, row0 = m * kTileM + rank * (kTileM / 2) + 32 * quad;
+      const int n_begin = c * p.tiles_n / p.chunks, n_end = (c + 1) * p.tiles_n / p.chunks;
+      for (int nt = n_begin; nt < n_end && ok; ++nt, ++turn) {
+        if (turn % kBufs != group) continue;
+        ok = mbar_wait_uniform(acc_full + 8 * group, (turn / kBufs) & 1, &abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t at = 0;
+#pragma unroll
+        for (int q = 0; q < 4; q += 2) {
+          const int n = nt * 64 + q * 16;
+          float v[2][16], w[2][16];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            tmem_floats(v[i], acc + (q + i) * 16);
+            tmem_floats(w[i], acc + 64 + (q + i) * 16);
+          }
+          tmem_arrived();
+          if (q == 2) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_there(empty_there);
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int left = p.cols - n - 16 * i;
+            if (p.bias && left > 0) {
+              add16<T>(v[i], (const T *)p.bias + n + 16 * i, left, 0);
+              add16<T>(w[i], (const T *)p.bias + p.cols + n + 16 * i, left, 0);
+            }
+            act_values<sizeof(T) == 4, 16>(v[i], p.act);
+            multiply<16>(v[i], w[i]);
+          }
+          if constexpr (sizeof(T) == 2) {
+            if (q == 0) at = box.room();
+            box.put<T, 64>(at, q, v[0]);
+            box.put<T, 64>(at, q + 1, v[1]);
+            if (q == 2) box.send(at, &maps.h, nt * 64, row0, 0);
+          } else if (n < p.cols) {
+            send_hidden<T>(box, &maps.h, v, n, row0, 0, 1);
+          }
+        }
+      }
+    }
+    box.close();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (abort_flag) {
+    if (warp == 1 && rank == 0) {      // products that are still running end before tensor memory is given back
+      if (elect_one()) mma_commit_pair(done);
+      __syncwarp();
+      mbar_wait_drain(done, 0);
+    }
+    if (threadIdx.x == 0) report_expired(p.status, p.alarm);
+  }
+  cluster_sync();                                       // neither leaves while the other may still signal it
+  if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  cluster_sync();
+}
+
 // Rows [rows][cols] of float32 as three bfloat16 planes, or 16-bit rows that TMA cannot read as they are (a width or an address
 // that is no multiple of 16 bytes), to rows of `pitch` elements.
 template <class T>
@@ -864,14 +1070,15 @@ Matrix operand(Ff &f, Scratch &s, const void *p, long long rows, int cols, int e
 // (what operand() may take of the scratch; whether an address is aligned is not known when sizes are asked for)
 size_t operand_bytes(int type, long long rows, int cols) { return align_up((size_t)rows * pitch_of(cols) * 2 * planes_for(type), 256); }
 
+uint32_t instruction(const Ff &f, int a_mn, int b_mn, int columns) {
+  const uint32_t type = f.type == SSC_PREC_F16 ? 0u : 1u;
+  return (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(columns >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24);
+}
+
 template <int EPI, class T>
 int launch_gemm(Ff &f, const FfMaps &maps, FfParams &p) {
   p.pairs = planes_for(f.type) == 3 ? 6 : 1;
-  for (Segment &s : p.seg) {
-    const uint32_t type = f.type == SSC_PREC_F16 ? 0u : 1u;
-    s.idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)s.a_mn << 15) | ((uint32_t)s.b_mn << 16) | ((uint32_t)(2 * s.boxes_b * kBox >> 3) << 17) |
-              ((uint32_t)(kTileM >> 4) << 24);
-  }
+  for (Segment &s : p.seg) s.idesc = instruction(f, s.a_mn, s.b_mn, 2 * s.boxes_b * kBox);
   p.act = f.act;
   p.status = f.status;
   p.alarm = alarm_word();
@@ -938,8 +1145,49 @@ int rows_product(Ff &f, const Matrix &a, const Matrix &b, int b_mn, bool halves,
   return launch_gemm<kRows, T>(f, maps, p);
 }
 
+// Gate and up with the rows staying in shared memory.
+template <class T>
+int hidden_product(Ff &f, const Matrix &x, const Matrix &w_in, const void *b_in, void *h) {
+  HiddenMaps maps = {};
+  HiddenParams p = {};
+  const bool f16 = f.type == SSC_PREC_F16;
+  if (int e = make_map(&maps.x, x, f16)) return e;
+  if (int e = make_map(&maps.w_in, w_in, f16)) return e;
+  p.rows = (int)x.rows;
+  p.cols = f.hidden;
+  if (!make_out_map(&maps.h, h, p.rows, f.hidden, pitch_of(f.hidden), planes_for(f.type), hidden_type(f.type), sizeof(T) == 2 ? 64 : 32))
+    return fail(SSC_ERR_CUDA, "gated_ff: no tensor map for the hidden rows");
+  p.blocks = ceil_div(f.c, kBox);
+  p.pairs = planes_for(f.type) == 3 ? 6 : 1;
+  p.tiles_m = ceil_div(p.rows, kTileM);
+  p.tiles_n = ceil_div(f.hidden, 64);
+  p.act = f.act;
+  p.bias = b_in;
+  p.idesc = instruction(f, 0, 0, 128);
+  p.status = f.status;
+  p.alarm = alarm_word();
+  const uint32_t fixed = kHiddenOut + (uint32_t)(p.blocks * planes_for(f.type)) * kBlockBytes + 1024;
+  p.stages = (int)((kHiddenRoom - fixed) / kStepBytes);
+  if (p.stages > kHiddenStages) p.stages = kHiddenStages;
+  // as many shares of the columns as make the longest pair's way shortest; rows fetched once more cost about a tile
+  const long long pairs = sm_count() / 2;
+  long long best = -1;
+  for (int c = 1; c <= p.tiles_n && c <= 64; ++c) {
+    const long long way = ((long long)p.tiles_m * c + pairs - 1) / pairs * (ceil_div(p.tiles_n, c) + 1);
+    if (best < 0 || way < best) best = way, p.chunks = c;
+  }
+  const long long units = (long long)p.tiles_m * p.chunks;
+  const size_t room = fixed + (size_t)p.stages * kStepBytes;
+  cudaError_t e = allow_smem((const void *)ff_hidden_kernel<T>, room);
+  if (e == cudaSuccess) e = launch_ready(ff_hidden_kernel<T>, dim3((unsigned)(2 * (units < pairs ? units : pairs))), dim3(kHiddenThreads), room, f.st, maps, p);
+  if (e != cudaSuccess) return fail(SSC_ERR_CUDA, "gated_ff: %s", cudaGetErrorString(e));
+  ++f.launches;
+  return SSC_OK;
+}
+
 template <class T>
 int gate_product(Ff &f, const Matrix &x, const Matrix &w_in, const void *b_in, void *h) {
+  if (planes_for(f.type) * ceil_div(f.c, kBox) <= kKeep) return hidden_product<T>(f, x, w_in, b_in, h);
   FfMaps maps = {};
   FfParams p = {};
   if (int e = make_map(&maps.a[0], x, f.type == SSC_PREC_F16)) return e;
