@@ -86,28 +86,6 @@ __device__ __forceinline__ uint32_t operand_lo(uint32_t addr, int mn) { return (
 
 __constant__ const int8_t kPlaneA[6] = {2, 0, 1, 1, 0, 0}, kPlaneB[6] = {0, 2, 1, 0, 1, 0};
 
-// A whole sector of L2 in one store: two halves of 16 bytes cost four times as much (gate and up of 65536 rows 256 -> 1024 in bf16: 119 us).
-__device__ __forceinline__ void store32(void *p, const uint32_t *v) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
-}
-template <class T>
-__device__ __forceinline__ void put16(T *p, const float *v, int left, int vec) {
-  if (vec && left >= 16) {
-    constexpr int N = 32 / sizeof(T);
-#pragma unroll
-    for (int i = 0; i < 16; i += N) {
-      struct alignas(16) { T v[N]; } k;
-#pragma unroll
-      for (int q = 0; q < N; ++q) k.v[q] = (T)v[i + q];
-      store32(p + i, (const uint32_t *)&k);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (i < left) p[i] = (T)v[i];
-  }
-}
 template <class T>
 __device__ __forceinline__ void add16(float *v, const T *p, int left, int vec) {
   if (vec && left >= 16) {
@@ -173,6 +151,12 @@ struct Outbox {
       const uint32_t *w = (const uint32_t *)&k, to = row + (((uint32_t)(part * (16 / N) + i) ^ turn) << 4);
       asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
     }
+  }
+  // One value of a box of 32 float32 columns.
+  static __device__ __forceinline__ float get(uint32_t box, uint32_t row, uint32_t col) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(box + row * 128 + ((((col >> 2) ^ row) & 7) << 4) + (col & 3) * 4) : "memory");
+    return v;
   }
   __device__ __forceinline__ void send(uint32_t box, const CUtensorMap *map, int x, int y, int z) {
     fence_async_smem();
@@ -348,30 +332,41 @@ __device__ __forceinline__ void finish(const FfParams &p, const FfMaps &maps, Ou
     send_hidden<T>(box, &maps.out[0], v, n, row0, 0, 1);
     return;
   }
-  if (EPI == kRows) {
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int left = p.cols - n - 16 * q;
-      if (left <= 0) continue;
-      if (p.bias) add16<T>(v[q], (const T *)p.bias + n + 16 * q, left, 0);
-      if (p.residual && row < p.rows) add16<T>(v[q], (const T *)p.residual + (size_t)row * p.pitch + n + 16 * q, left, p.vec);
-    }
-  }
   using V = std::conditional_t<EPI == kPart, float, T>;
   if (p.boxes) {
+    if (EPI == kRows) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int left = p.cols - n - 16 * q;
+        if (left <= 0) continue;
+        if (p.bias) add16<T>(v[q], (const T *)p.bias + n + 16 * q, left, 0);
+        if (p.residual && row < p.rows) add16<T>(v[q], (const T *)p.residual + (size_t)row * p.pitch + n + 16 * q, left, p.vec);
+      }
+    }
     const uint32_t at = box.room();
     box.put<V>(at, 0, v[0]);
     box.put<V>(at, 1, v[1]);
     box.send(at, &maps.out[0], n, row0, EPI == kPart ? split * (p.m_half < p.tiles_m ? 2 : 1) + half_m : 0);
-  } else if (row < p.rows) {
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int left = p.cols - n - 16 * q;
-      if (left <= 0) continue;
-      V *o = (V *)p.out + (EPI == kPart ? (size_t)split * p.plane : 0) + ((size_t)half_m * p.rows + row) * p.pitch + n + 16 * q;
-      if (EPI == kPart && p.accumulate) add16<V>(v[q], o, left, p.vec);
-      put16<V>(o, v[q], left, p.vec);
+  } else {
+    // a lane to a column: rows that are no multiple of 16 bytes, one value at a time
+    const uint32_t lane = threadIdx.x & 31;
+    box.put<float>(box.at, 0, v[0]);
+    box.put<float>(box.at, 1, v[1]);
+    __syncwarp();
+    const int col = n + (int)lane, many = min(32, p.rows - row0);
+    if (col < p.cols) {
+      const float bias = EPI == kRows && p.bias ? (float)((const T *)p.bias)[col] : 0.f;
+      V *o = (V *)p.out + (EPI == kPart ? (size_t)split * p.plane : 0) + ((size_t)half_m * p.rows + row0) * p.pitch + col;
+      const T *add = EPI == kRows && p.residual ? (const T *)p.residual + (size_t)row0 * p.pitch + col : nullptr;
+#pragma unroll 8
+      for (int r = 0; r < many; ++r) {
+        float x = Outbox::get(box.at, r, lane) + bias;
+        if (add) x += (float)add[(size_t)r * p.pitch];
+        if (EPI == kPart && p.accumulate) x += (float)o[(size_t)r * p.pitch];
+        o[(size_t)r * p.pitch] = (V)x;
+      }
     }
+    __syncwarp();
   }
 }
 
@@ -875,20 +870,35 @@ __global__ void __launch_bounds__(256) ff_planes_kernel(const T *__restrict__ sr
   }
 }
 
-// out[i] = sum over `parts` of part[k * stride + i], in order.
+// Sums of shares, in order: out[i] = sum over `parts` of part[k * total + i], for up to five arrays in one launch.
+struct SumJob {
+  const float *part;
+  void *out;
+  int parts;
+  size_t total;               // values
+  unsigned first;             // block
+};
+struct SumJobs {
+  SumJob job[5];
+  int many;
+};
 template <class T>
-__global__ void __launch_bounds__(256) ff_sum_kernel(const float *__restrict__ part, int parts, size_t stride, size_t total, T *__restrict__ out) {
+__global__ void __launch_bounds__(256) ff_sum_kernel(const SumJobs jobs) {
   after_previous();
-  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= total) return;
+  int j = 0;
+  while (j + 1 < jobs.many && blockIdx.x >= jobs.job[j + 1].first) ++j;
+  const SumJob &s = jobs.job[j];
+  const size_t i = (size_t)(blockIdx.x - s.first) * 256 + threadIdx.x;
+  if (i >= s.total) return;
   float v = 0.f;
-  for (int k = 0; k < parts; ++k) v += part[(size_t)k * stride + i];
-  out[i] = (T)v;
+#pragma unroll 8
+  for (int k = 0; k < s.parts; ++k) v += s.part[(size_t)k * s.total + i];
+  ((T *)s.out)[i] = (T)v;
 }
 
-// Column sums of rows [rows][pitch] (planes of float32 ones added up), a block's share of the rows: part[blockIdx.y][cols].
+// Column sums of one or two matrices [rows][pitch] (planes of float32 ones added up), a block's share of the rows: part[blockIdx.y][matrices * cols].
 template <class T>
-__global__ void __launch_bounds__(256) ff_columns_kernel(const T *__restrict__ src, long long rows, int cols, int pitch, int planes, size_t plane,
+__global__ void __launch_bounds__(256) ff_columns_kernel(const T *__restrict__ src, long long rows, int cols, int pitch, int planes, size_t plane, size_t matrix,
                                                          float *__restrict__ part, int accumulate) {
   after_previous();
   __shared__ float sm[8][32];
@@ -896,13 +906,16 @@ __global__ void __launch_bounds__(256) ff_columns_kernel(const T *__restrict__ s
   const long long lo = rows * blockIdx.y / gridDim.y, hi = rows * (blockIdx.y + 1) / gridDim.y;
   float v = 0.f;
   if (col < cols)
-    for (int k = planes - 1; k >= 0; --k)
-      for (long long r = lo + w; r < hi; r += 8) v += (float)src[k * plane + r * pitch + col];
+    for (int k = planes - 1; k >= 0; --k) {
+      const T *from = src + blockIdx.z * matrix + k * plane + col;
+#pragma unroll 4
+      for (long long r = lo + w; r < hi; r += 8) v += (float)from[r * pitch];
+    }
   sm[w][lane] = v;
   __syncthreads();
   if (w == 0 && col < cols) {
     for (int i = 1; i < 8; ++i) v += sm[i][lane];
-    float *o = part + (size_t)blockIdx.y * cols + col;
+    float *o = part + ((size_t)blockIdx.y * gridDim.z + blockIdx.z) * cols + col;
     *o = accumulate ? *o + v : v;
   }
 }
@@ -910,26 +923,42 @@ __global__ void __launch_bounds__(256) ff_columns_kernel(const T *__restrict__ s
 // Few rows: the weights are read once and bound the time; a warp to an output, rows in shared memory, sums in float32 and h
 // never rounded.  kR rows at a time.
 constexpr int kR = 8;
+// acc[r] += sum over this lane's part of w[i] xs[r][i], all lanes' sums in the end.  xs: rows of `stride` floats, 16-byte aligned.
 template <class T>
 __device__ __forceinline__ void dot_rows(const T *__restrict__ w, const float *__restrict__ xs, int k, int stride, int live, float *acc, int vec) {
   constexpr int N = 16 / sizeof(T);
   const int lane = threadIdx.x & 31;
   if (vec) {
-    for (int i = lane * N; i < k; i += 32 * N) {
-      struct alignas(16) { T v[N]; } q;
-      *(int4 *)&q = *(const int4 *)(w + i);
+    constexpr int U = 4;                        // pieces of the weights in flight
+    for (int i0 = lane * N; i0 < k; i0 += 32 * N * U) {
+      int4 q[U];
 #pragma unroll
-      for (int r = 0; r < kR; ++r)
-        if (r < live) {
+      for (int u = 0; u < U; ++u) q[u] = i0 + u * 32 * N < k ? *(const int4 *)(w + i0 + u * 32 * N) : make_int4(0, 0, 0, 0);
 #pragma unroll
-          for (int e = 0; e < N; ++e) acc[r] = fmaf((float)q.v[e], xs[r * stride + i + e], acc[r]);
-        }
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * 32 * N;
+        if (i >= k) continue;
+        struct alignas(16) { T v[N]; } piece;
+        *(int4 *)&piece = q[u];
+#pragma unroll
+        for (int r = 0; r < kR; ++r)
+          if (r < live) {
+#pragma unroll
+            for (int e = 0; e < N; e += 4) {
+              const float4 x = *(const float4 *)(xs + (size_t)r * stride + i + e);
+              acc[r] = fmaf((float)piece.v[e], x.x, acc[r]);
+              acc[r] = fmaf((float)piece.v[e + 1], x.y, acc[r]);
+              acc[r] = fmaf((float)piece.v[e + 2], x.z, acc[r]);
+              acc[r] = fmaf((float)piece.v[e + 3], x.w, acc[r]);
+            }
+          }
+      }
     }
   } else {
     for (int i = lane; i < k; i += 32)
 #pragma unroll
       for (int r = 0; r < kR; ++r)
-        if (r < live) acc[r] = fmaf((float)w[i], xs[r * stride + i], acc[r]);
+        if (r < live) acc[r] = fmaf((float)w[i], xs[(size_t)r * stride + i], acc[r]);
   }
 #pragma unroll
   for (int r = 0; r < kR; ++r)
@@ -938,9 +967,9 @@ __device__ __forceinline__ void dot_rows(const T *__restrict__ w, const float *_
 
 template <class T>
 __global__ void __launch_bounds__(256) ff_few_hidden_kernel(const T *__restrict__ x, int rows, int c, int hidden, const T *__restrict__ w_in, const T *__restrict__ b_in,
-                                                            int act, float *__restrict__ h, int vec) {
+                                                            int act, float *__restrict__ h, int h_stride, int vec) {
   after_previous();
-  extern __shared__ float xs[];                 // [kR][c rounded up to 8]
+  extern __shared__ __align__(16) float xs[];   // [kR][c rounded up to 8]
   const int r0 = blockIdx.y * kR, live = min(kR, rows - r0), stride = (c + 7) & ~7;
   for (int i = threadIdx.x; i < live * c; i += 256) {
     const int r = i / c;
@@ -959,19 +988,19 @@ __global__ void __launch_bounds__(256) ff_few_hidden_kernel(const T *__restrict_
       const float bg = b_in ? (float)b_in[j] : 0.f, bu = b_in ? (float)b_in[hidden + j] : 0.f;
       float a = g[r] + bg;
       act_values<true, 1>(&a, act);
-      h[(size_t)(r0 + r) * hidden + j] = a * (u[r] + bu);
+      h[(size_t)(r0 + r) * h_stride + j] = a * (u[r] + bu);
     }
 }
 
 template <class T>
-__global__ void __launch_bounds__(256) ff_few_out_kernel(const float *__restrict__ h, int rows, int hidden, int c_out, const T *__restrict__ w_out, const T *__restrict__ b_out,
+__global__ void __launch_bounds__(256) ff_few_out_kernel(const float *__restrict__ h, int h_stride, int rows, int hidden, int c_out, const T *__restrict__ w_out, const T *__restrict__ b_out,
                                                          const T *__restrict__ residual, T *__restrict__ y, int vec) {
   after_previous();
   const int r0 = blockIdx.y * kR, live = min(kR, rows - r0);
   const int o = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (o >= c_out) return;
   float v[kR] = {};
-  dot_rows<T>(w_out + (size_t)o * hidden, h + (size_t)r0 * hidden, hidden, hidden, live, v, vec);
+  dot_rows<T>(w_out + (size_t)o * hidden, h + (size_t)r0 * h_stride, hidden, h_stride, live, v, vec);
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int r = 0; r < kR; ++r)
@@ -1282,10 +1311,9 @@ int filter_product(Ff &f, const Matrix &a, const Matrix &b, int halves, int m, i
   return launch_gemm<kPart, T>(f, maps, p);
 }
 
-template <class T>
-cudaError_t sum_parts(Ff &f, const float *part, int parts, size_t total, void *out) {
-  ++f.launches;
-  return launch_ready(ff_sum_kernel<T>, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, f.st, part, parts, total, total, (T *)out);
+void add_job(SumJobs &jobs, unsigned &blocks, const float *part, int parts, size_t total, void *out) {
+  jobs.job[jobs.many++] = {part, out, parts, total, blocks};
+  blocks += (unsigned)((total + 255) / 256);
 }
 constexpr int kColumnShares = 32;
 
@@ -1303,15 +1331,16 @@ bool few(const Ff &f) { return f.n <= (f.type == SSC_PREC_FP32 ? 64 : 16) && f.c
 template <class T>
 int forward(Ff &f, Scratch s, const void *x, const void *w_in, const void *w_out, const void *b_in, const void *b_out, const void *residual, void *out) {
   if (few(f)) {
-    float *h = (float *)s.take((size_t)f.n * f.hidden * sizeof(float));
+    const int h_stride = (f.hidden + 3) & ~3;
+    float *h = (float *)s.take((size_t)f.n * h_stride * sizeof(float));
     const int vec_in = f.c % (16 / (int)sizeof(T)) == 0 && ((uintptr_t)w_in & 15) == 0, vec_out = f.hidden % (16 / (int)sizeof(T)) == 0 && ((uintptr_t)w_out & 15) == 0;
     const size_t room = (size_t)kR * ((f.c + 7) & ~7) * sizeof(float);
     cudaError_t e = allow_smem((const void *)ff_few_hidden_kernel<T>, room);
     if (e == cudaSuccess)
       e = launch_ready(ff_few_hidden_kernel<T>, dim3(ceil_div(f.hidden, 8), ceil_div(f.n, kR)), dim3(256), room, f.st, (const T *)x, f.n, f.c, f.hidden, (const T *)w_in,
-                       (const T *)b_in, f.act, h, vec_in);
+                       (const T *)b_in, f.act, h, h_stride, vec_in);
     if (e == cudaSuccess)
-      e = launch_ready(ff_few_out_kernel<T>, dim3(ceil_div(f.c_out, 8), ceil_div(f.n, kR)), dim3(256), 0, f.st, (const float *)h, f.n, f.hidden, f.c_out, (const T *)w_out,
+      e = launch_ready(ff_few_out_kernel<T>, dim3(ceil_div(f.c_out, 8), ceil_div(f.n, kR)), dim3(256), 0, f.st, (const float *)h, h_stride, f.n, f.hidden, f.c_out, (const T *)w_out,
                        (const T *)b_out, (const T *)residual, (T *)out, vec_out);
     if (e != cudaSuccess) return fail(SSC_ERR_CUDA, "gated_ff_fwd: %s", cudaGetErrorString(e));
     f.launches += 2;
@@ -1361,35 +1390,36 @@ int backward(Ff &f, Scratch s, const void *x, const void *gy, const void *w_in, 
     if (gw_out)
       if (int k = filter_product<T>(f, gm, hm, 1, f.c_out, f.hidden, split_out, part_out, more)) return k;
     const size_t plane = (size_t)rows * pitch;
-    if (gb_in)
-      for (int half = 0; half < 2 && e == cudaSuccess; ++half) {
-        float *to = cols_in + (size_t)half * kColumnShares * f.hidden;
-        const dim3 grid(ceil_div(f.hidden, 32), kColumnShares);
-        if (sizeof(T) == 2)
-          e = launch_ready(ff_columns_kernel<T>, grid, dim3(256), 0, f.st, (const T *)dgu + half * plane, rows, f.hidden, pitch, 1, plane, to, more);
-        else
-          e = launch_ready(ff_columns_kernel<__nv_bfloat16>, grid, dim3(256), 0, f.st, (const __nv_bfloat16 *)dgu + half * plane, rows, f.hidden, pitch, 3, 2 * plane, to,
-                           more);
-        ++f.launches;
-      }
+    if (gb_in && e == cudaSuccess) {
+      const dim3 grid(ceil_div(f.hidden, 32), kColumnShares, 2);
+      if (sizeof(T) == 2)
+        e = launch_ready(ff_columns_kernel<T>, grid, dim3(256), 0, f.st, (const T *)dgu, rows, f.hidden, pitch, 1, (size_t)0, plane, cols_in, more);
+      else
+        e = launch_ready(ff_columns_kernel<__nv_bfloat16>, grid, dim3(256), 0, f.st, (const __nv_bfloat16 *)dgu, rows, f.hidden, pitch, 3, 2 * plane, plane, cols_in, more);
+      ++f.launches;
+    }
     if (gb_out && e == cudaSuccess) {
       e = launch_ready(ff_columns_kernel<T>, dim3(ceil_div(f.c_out, 32), kColumnShares), dim3(256), 0, f.st, (const T *)gy + r * f.c_out, rows, f.c_out, f.c_out, 1, (size_t)0,
-                       cols_out, more);
+                       (size_t)0, cols_out, more);
       ++f.launches;
     }
   }
-  if (gw_in && e == cudaSuccess) e = sum_parts<T>(f, part_in, split_in, size_in, gw_in);
-  if (gw_out && e == cudaSuccess) e = sum_parts<T>(f, part_out, split_out, size_out, gw_out);
-  if (gb_in)
-    for (int half = 0; half < 2 && e == cudaSuccess; ++half)
-      e = sum_parts<T>(f, cols_in + (size_t)half * kColumnShares * f.hidden, kColumnShares, f.hidden, (T *)gb_in + (size_t)half * f.hidden);
-  if (gb_out && e == cudaSuccess) e = sum_parts<T>(f, cols_out, kColumnShares, f.c_out, gb_out);
+  SumJobs jobs = {};
+  unsigned blocks = 0;
+  if (gw_in) add_job(jobs, blocks, part_in, split_in, size_in, gw_in);
+  if (gw_out) add_job(jobs, blocks, part_out, split_out, size_out, gw_out);
+  if (gb_in) add_job(jobs, blocks, cols_in, kColumnShares, 2 * (size_t)f.hidden, gb_in);
+  if (gb_out) add_job(jobs, blocks, cols_out, kColumnShares, f.c_out, gb_out);
+  if (blocks > 0 && e == cudaSuccess) {
+    e = launch_ready(ff_sum_kernel<T>, dim3(blocks), dim3(256), 0, f.st, jobs);
+    ++f.launches;
+  }
   if (e != cudaSuccess) return fail(SSC_ERR_CUDA, "gated_ff_bwd: %s", cudaGetErrorString(e));
   return SSC_OK;
 }
 
 size_t scratch_bytes_for(const Ff &f, bool back) {
-  if (!back && few(f)) return align_up((size_t)f.n * f.hidden * sizeof(float), 256) + 256;
+  if (!back && few(f)) return align_up((size_t)f.n * ((f.hidden + 3) & ~3) * sizeof(float), 256) + 256;
   const long long most = rows_at_once(f, back);
   const size_t hidden = align_up((size_t)most * pitch_of(f.hidden) * 2 * planes_for(f.type), 256);
   size_t b = 256 + operand_bytes(f.type, 2ll * f.hidden, f.c) + operand_bytes(f.type, f.c_out, f.hidden) + operand_bytes(f.type, most, f.c);
