@@ -6,6 +6,7 @@ inference compute the same.  Scalars are centred and scaled, fields of order l >
 their squared norm, which keeps the layer equivariant."""
 import functools
 import itertools
+import weakref
 
 import torch
 import torch.nn as nn
@@ -129,15 +130,20 @@ class GroupNorm(nn.Module):
     def __repr__(self):
         return "{} (Rs={}, num_groups={}, eps={})".format(self.__class__.__name__, self.Rs, self.num_groups, self.eps)
 
-    def _apply_to(self, input, rows):
-        """input with `rows`(features, offsets) in place of its features."""
-        if torch.is_grad_enabled() and (input.raw()[0].requires_grad or any(p.requires_grad for p in self.parameters())):
+    def rows(self, features, offsets):
+        return group_norm(features, offsets, self.Rs, self.num_groups, self.weight, self.bias, self.eps, self.activation)
+
+    @staticmethod
+    def apply_rows(input, rows, parameters):
+        """input (a SparseTensor) with rows(features, offsets) in the place of its features; parameters: those that `rows` uses."""
+        if torch.is_grad_enabled() and (input.raw()[0].requires_grad or any(p.requires_grad for p in parameters)):
             input.features = rows(input.features, input.get_offsets())
             return input
         # (nothing to record: a pending row count stays on the device)
         input.features = rows(input.raw()[0], input.get_offsets())
         if input.pending():
-            input._rows.post.append(lambda f: rows(f, input.get_offsets()))
+            whose = weakref.ref(input)      # (called by the tensor itself; a cycle would keep its rows until the collector comes)
+            input._rows.post.append(lambda f: rows(f, whose().get_offsets()))
         return input
 
     def norm_and_gate(self, input, act):
@@ -156,8 +162,7 @@ class GroupNorm(nn.Module):
                 out = _ext._stored_type(f.shape[0], layout.c, layout.c_out, layout.c_out, _ext.get_feature_storage()) or out
             return _ext.group_norm(f, offsets, layout, self.weight, self.bias, self.eps, codes, out)
 
-        return self._apply_to(input, rows)
+        return self.apply_rows(input, rows, self.parameters())
 
     def forward(self, input):
-        return self._apply_to(input, lambda f, offsets: group_norm(f, offsets, self.Rs, self.num_groups, self.weight, self.bias, self.eps,
-                                                                   self.activation))
+        return self.apply_rows(input, self.rows, self.parameters())

@@ -15,6 +15,7 @@ from ss_conv.activation import Activation
 from ss_conv.batchnorm import BatchNorm
 from ss_conv.convolution import Convolution
 from ss_conv.dropout import Dropout
+from ss_conv.feedforward import GatedFeedForward
 from ss_conv.groupnorm import GroupNorm
 from ss_conv.sp_ops.tensor import SparseTensor
 from ss_conv.sp_ops.voxelize import Point2Voxel, Voxel2Point
@@ -101,6 +102,20 @@ class SS_Conv(nn.Module):
         if self.dropout is not None:
             x = self.dropout(x)
         return x
+
+
+class SS_FeedForward(nn.Module):
+    """x + GatedFeedForward(GroupNorm(x)) on the rows of a SparseTensor of scalars (channels of order 0), for the heads behind the
+    convolutions, where the reference has plain linear layers (LineMOD/model.py:22-138).  Each sample is normalised by itself; no row
+    depends on another sample."""
+
+    def __init__(self, channels, hidden_channels, norm_groups=1, activation=F.silu, bias=False):
+        super().__init__()
+        self.norm = GroupNorm([(channels, 0)], norm_groups)
+        self.ff = GatedFeedForward(channels, hidden_channels, activation=activation, bias=bias)
+
+    def forward(self, x):
+        return self.norm.apply_rows(x, lambda f, offsets: self.ff.rows(self.norm.rows(f, offsets), f), self.parameters())
 
 
 class Feature_Steering_Module(nn.Module):
