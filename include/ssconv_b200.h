@@ -598,8 +598,7 @@ int ssc_gate_bwd(const float *x, const float *gy, int n, int c_total, int c_out,
  * group_copies [n_group].  weight [n_field] and bias [n_scalar] float32 or NULL.  Activations: 0 identity, 1 relu, 2 sigmoid,
  * 3 silu, 4 gelu (erf).  out_type is `type`, or any for float32 rows.  stats [batch, n_group, 2] float32 receives mean (0 for l > 0) and
  * (variance + eps)^-1/2 of every sample that has rows, which the backward call reads.  Sums are float32, in a fixed order.
- * c is at most 512 channels, 1024 / 2048 where c and c - n_gate are multiples of 2 / 4,
- * with at most 512 gates.  Rows and scratch
+ * c is at most 2048 channels, with at most 512 gates.  Rows and scratch
  * start at multiples of 16 bytes.  scratch: ssc_group_norm_scratch_bytes(...) (forward: n_field = n_scalar = 0 will do).  status: as in
  * ssc_conv_fwd.  gx has the type of x; d_weight [n_field], d_bias [n_scalar] float32. */
 size_t ssc_group_norm_scratch_bytes(int batch, int n_group, int n_field, int n_scalar);

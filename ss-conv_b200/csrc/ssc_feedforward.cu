@@ -870,13 +870,15 @@ __global__ void __launch_bounds__(256) ff_planes_kernel(const T *__restrict__ sr
   }
 }
 
-// Sums of shares, in order: out[i] = sum over `parts` of part[k * total + i], for up to five arrays in one launch.
+// Sums of shares, in order: out[i] = sum over `parts` of part[k * total + i] (+ bias, residual), for up to five arrays in one launch.
 struct SumJob {
   const float *part;
   void *out;
-  int parts;
-  size_t total;               // values
-  unsigned first;             // block
+  const void *bias, *residual;      // of rows of `cols` values (or null); out and residual with rows of `pitch`
+  int parts, cols, pitch;
+  size_t total;                     // values
+  unsigned first;                   // block
+  int few;                          // few sums of many shares: a warp to each instead of a thread
 };
 struct SumJobs {
   SumJob job[5];
@@ -888,35 +890,62 @@ __global__ void __launch_bounds__(256) ff_sum_kernel(const SumJobs jobs) {
   int j = 0;
   while (j + 1 < jobs.many && blockIdx.x >= jobs.job[j + 1].first) ++j;
   const SumJob &s = jobs.job[j];
-  const size_t i = (size_t)(blockIdx.x - s.first) * 256 + threadIdx.x;
-  if (i >= s.total) return;
   float v = 0.f;
+  size_t i = (size_t)(blockIdx.x - s.first) * 256 + threadIdx.x;
+  if (s.few) {
+    i = (size_t)(blockIdx.x - s.first) * 8 + (threadIdx.x >> 5);
+    if (i >= s.total) return;
+#pragma unroll 4
+    for (int k = threadIdx.x & 31; k < s.parts; k += 32) v += s.part[(size_t)k * s.total + i];
+    for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    if ((threadIdx.x & 31) != 0) return;
+  } else {
+    if (i >= s.total) return;
 #pragma unroll 8
-  for (int k = 0; k < s.parts; ++k) v += s.part[(size_t)k * s.total + i];
-  ((T *)s.out)[i] = (T)v;
+    for (int k = 0; k < s.parts; ++k) v += s.part[(size_t)k * s.total + i];
+  }
+  size_t at = i;
+  if (s.cols != 0) {
+    const size_t row = i / (unsigned)s.cols;
+    const int col = (int)(i - row * (unsigned)s.cols);
+    at = row * s.pitch + col;
+    if (s.bias) v += (float)((const T *)s.bias)[col];
+    if (s.residual) v += (float)((const T *)s.residual)[at];
+  }
+  ((T *)s.out)[at] = (T)v;
 }
 
 // Column sums of one or two matrices [rows][pitch] (planes of float32 ones added up), a block's share of the rows: part[blockIdx.y][matrices * cols].
+// A thread has eight columns; rows start at multiples of 16 bytes.
 template <class T>
 __global__ void __launch_bounds__(256) ff_columns_kernel(const T *__restrict__ src, long long rows, int cols, int pitch, int planes, size_t plane, size_t matrix,
                                                          float *__restrict__ part, int accumulate) {
   after_previous();
-  __shared__ float sm[8][32];
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+  __shared__ float sm[256][9];
+  const int groups = min((cols + 7) / 8 - (int)blockIdx.x * 32, 32), R = 256 / groups, g = threadIdx.x % groups, w = threadIdx.x / groups, c0 = (blockIdx.x * 32 + g) * 8;
   const long long lo = rows * blockIdx.y / gridDim.y, hi = rows * (blockIdx.y + 1) / gridDim.y;
-  float v = 0.f;
-  if (col < cols)
+  float v[8] = {};
+  if (w < R)
     for (int k = planes - 1; k >= 0; --k) {
-      const T *from = src + blockIdx.z * matrix + k * plane + col;
+      const T *from = src + blockIdx.z * matrix + k * plane + c0;
 #pragma unroll 4
-      for (long long r = lo + w; r < hi; r += 8) v += (float)from[r * pitch];
+      for (long long r = lo + w; r < hi; r += R) {
+        struct alignas(16) { T v[8]; } q;
+        *(int4 *)&q = *(const int4 *)(from + r * pitch);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += (float)q.v[i];
+      }
     }
-  sm[w][lane] = v;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sm[threadIdx.x][i] = v[i];
   __syncthreads();
-  if (w == 0 && col < cols) {
-    for (int i = 1; i < 8; ++i) v += sm[i][lane];
+  for (int t = threadIdx.x; t < groups * 8; t += 256) {
+    const int col = blockIdx.x * 256 + t;
+    if (col >= cols) continue;
+    float sum = 0.f;
+    for (int i = 0; i < R; ++i) sum += sm[i * groups + t / 8][t % 8];
     float *o = part + ((size_t)blockIdx.y * gridDim.z + blockIdx.z) * cols + col;
-    *o = accumulate ? *o + v : v;
+    *o = accumulate ? *o + sum : sum;
   }
 }
 
@@ -955,10 +984,21 @@ __device__ __forceinline__ void dot_rows(const T *__restrict__ w, const float *_
       }
     }
   } else {
-    for (int i = lane; i < k; i += 32)
+    constexpr int U = 8;
+    for (int i0 = lane; i0 < k; i0 += 32 * U) {
+      float q[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) q[u] = i0 + 32 * u < k ? (float)w[i0 + 32 * u] : 0.f;
 #pragma unroll
       for (int r = 0; r < kR; ++r)
-        if (r < live) acc[r] = fmaf((float)w[i], xs[(size_t)r * stride + i], acc[r]);
+        if (r < live) {
+          float x[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u) x[u] = i0 + 32 * u < k ? xs[(size_t)r * stride + i0 + 32 * u] : 0.f;
+#pragma unroll
+          for (int u = 0; u < U; ++u) acc[r] = fmaf(q[u], x[u], acc[r]);
+        }
+    }
   }
 #pragma unroll
   for (int r = 0; r < kR; ++r)
@@ -1142,9 +1182,11 @@ Segment segment(int k, int boxes_b) {
 // Result tiles of 128 or 256 columns.
 int tile_columns(int cols) { return cols <= 128 ? 128 : 256; }
 
-// C [rows][cols] = A B' (+ bias, residual) as rows of T; B as stored (b_mn: [k][cols]).
+int row_splits(const Ff &f, long long rows, int blocks, int cols);
+
+// C [rows][cols] = A B' (+ bias, residual) as rows of T; B as stored (b_mn: [k][cols]).  part: room for shares of the sum.
 template <class T>
-int rows_product(Ff &f, const Matrix &a, const Matrix &b, int b_mn, bool halves, int k, int cols, const void *bias, const void *residual, void *out, int pitch = 0) {
+int rows_product(Ff &f, const Matrix &a, const Matrix &b, int b_mn, bool halves, int k, int cols, const void *bias, const void *residual, void *out, float *part, int pitch = 0) {
   FfMaps maps = {};
   FfParams p = {};
   if (int e = make_map(&maps.a[0], a, f.type == SSC_PREC_F16)) return e;
@@ -1161,11 +1203,26 @@ int rows_product(Ff &f, const Matrix &a, const Matrix &b, int b_mn, bool halves,
   p.n_seg = 1;
   p.rows = (int)a.rows;
   p.cols = cols;
-  p.pitch = pitch ? pitch : cols;
   p.tiles_m = ceil_div(p.rows, kTileM);
   p.m_half = 1 << 30;
   p.tiles_n = ceil_div(cols, p.step_n);
-  p.splits = 1;
+  p.splits = row_splits(f, p.rows, p.seg[0].blocks, cols);
+  if (p.splits > 1) {
+    const size_t total = (size_t)p.rows * cols;
+    p.pitch = cols;
+    p.plane = total;
+    p.out = part;
+    p.boxes = make_out_map(&maps.out[0], part, p.rows, cols, cols, p.splits, SSC_PREC_FP32);
+    if (int e = launch_gemm<kPart, T>(f, maps, p)) return e;
+    SumJobs jobs = {};
+    jobs.many = 1;
+    jobs.job[0] = {part, out, bias, residual, p.splits, cols, pitch ? pitch : cols, total, 0, 0};
+    const cudaError_t e = launch_ready(ff_sum_kernel<T>, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, f.st, jobs);
+    if (e != cudaSuccess) return fail(SSC_ERR_CUDA, "gated_ff: %s", cudaGetErrorString(e));
+    ++f.launches;
+    return SSC_OK;
+  }
+  p.pitch = pitch ? pitch : cols;
   p.bias = bias;
   p.residual = residual;
   p.out = out;
@@ -1311,11 +1368,33 @@ int filter_product(Ff &f, const Matrix &a, const Matrix &b, int halves, int m, i
   return launch_gemm<kPart, T>(f, maps, p);
 }
 
-void add_job(SumJobs &jobs, unsigned &blocks, const float *part, int parts, size_t total, void *out) {
-  jobs.job[jobs.many++] = {part, out, parts, total, blocks};
-  blocks += (unsigned)((total + 255) / 256);
+void add_job(SumJobs &jobs, unsigned &blocks, const float *part, int parts, size_t total, void *out, int few) {
+  jobs.job[jobs.many++] = {part, out, nullptr, nullptr, parts, 0, 0, total, blocks, few};
+  blocks += (unsigned)(few ? (total + 7) / 8 : (total + 255) / 256);
 }
-constexpr int kColumnShares = 32;
+// Shares of the rows of a column sum: four blocks to an SM, at least 64 rows to a share.
+int column_shares(const Ff &f, long long rows, int cols, int matrices) {
+  long long s = 4ll * sm_count() / ((long long)ceil_div(cols, 256) * matrices);
+  if (s > rows / 64) s = rows / 64;
+  return s < 1 ? 1 : (int)s;
+}
+
+// Shares of the sum of a product whose tiles are too few for the pairs of CTAs, or a few too many: what a pair does at the longest, in steps of a
+// block (0.3 us), with a dozen for a tile's start and end, and the shares written and read once more (2 MB a step).
+int row_splits(const Ff &f, long long rows, int blocks, int cols) {
+  const long long pairs = sm_count() / 2, tiles = (long long)ceil_div(rows, kTileM) * ceil_div(cols, tile_columns(cols)), each = planes_for(f.type) == 3 ? 6 : 1;
+  long long best = 0;
+  int take = 1;
+  for (int s = 1; s <= 16 && s <= blocks && (s == 1 || tiles * s <= 4 * pairs); ++s) {
+    const long long way = (tiles * s + pairs - 1) / pairs * (ceil_div(blocks, s) * each + 12) + (s > 1 ? 10 + s * rows * cols * 8 / 2000000 : 0);
+    if (s == 1 || way < best) best = way, take = s;
+  }
+  return take;
+}
+size_t row_split_bytes(const Ff &f, long long rows, int blocks, int cols) {
+  const int s = rows > 0 ? row_splits(f, rows, blocks, cols) : 1;
+  return s > 1 ? align_up((size_t)s * rows * cols * sizeof(float), 256) : 0;
+}
 
 // Rows of one go, so that what lies between the products is at most about a gigabyte.
 long long rows_at_once(const Ff &f, bool backward) {
@@ -1323,6 +1402,20 @@ long long rows_at_once(const Ff &f, bool backward) {
   long long rows = (1ll << 30) / per / kTileM * kTileM;
   if (rows < 16 * kTileM) rows = 16 * kTileM;
   return rows < f.n ? rows : f.n;
+}
+
+// Room for the shares of the products that give rows (rows_product), for a whole turn of rows and for the last one.
+size_t parts_bytes(const Ff &f, long long most, bool back) {
+  const long long last = most > 0 ? f.n % most : 0;
+  const int c = ceil_div(f.c_out, kBox), h = ceil_div(f.hidden, kBox);
+  size_t b = 0;
+  for (const long long rows : {most, last}) {
+    const size_t one = back ? row_split_bytes(f, rows, 2 * h, f.c) : row_split_bytes(f, rows, h, f.c_out);
+    const size_t two = back && f.type == SSC_PREC_FP32 ? row_split_bytes(f, rows, c, f.hidden) : 0;
+    if (one > b) b = one;
+    if (two > b) b = two;
+  }
+  return b;
 }
 
 // Rows up to which the weights are read once by a warp to an output instead of by tiles of 128 rows.
@@ -1350,13 +1443,14 @@ int forward(Ff &f, Scratch s, const void *x, const void *w_in, const void *w_out
   const long long most = rows_at_once(f, false);
   const int pitch = pitch_of(f.hidden), planes = planes_for(f.type);
   void *h = s.take((size_t)most * pitch * 2 * planes);
+  float *part = (float *)s.take(parts_bytes(f, most, false));
   for (long long r = 0; r < f.n; r += most) {
     const long long rows = f.n - r < most ? f.n - r : most;
     Scratch here = s;
     const Matrix xm = operand<T>(f, here, (const T *)x + r * f.c, rows, f.c, 1);
     if (int e = gate_product<T>(f, xm, wi, b_in, h)) return e;
     const Matrix hm = {h, rows, f.hidden, pitch, planes};
-    if (int e = rows_product<T>(f, hm, wo, 0, false, f.hidden, f.c_out, b_out, residual ? (const T *)residual + r * f.c_out : nullptr, (T *)out + r * f.c_out)) return e;
+    if (int e = rows_product<T>(f, hm, wo, 0, false, f.hidden, f.c_out, b_out, residual ? (const T *)residual + r * f.c_out : nullptr, (T *)out + r * f.c_out, part)) return e;
   }
   return SSC_OK;
 }
@@ -1365,6 +1459,7 @@ template <class T>
 int backward(Ff &f, Scratch s, const void *x, const void *gy, const void *w_in, const void *w_out, const void *b_in, void *gx, void *gw_in, void *gw_out, void *gb_in,
              void *gb_out) {
   const Matrix wi = operand<T>(f, s, w_in, 2ll * f.hidden, f.c, 2), wo = operand<T>(f, s, w_out, f.c_out, f.hidden, 1);
+  using U = std::conditional_t<sizeof(T) == 4, __nv_bfloat16, T>;
   const long long most = rows_at_once(f, true);
   const int pitch = pitch_of(f.hidden), planes = planes_for(f.type);
   const size_t size_in = 2 * (size_t)f.hidden * f.c, size_out = (size_t)f.c_out * f.hidden;
@@ -1372,7 +1467,9 @@ int backward(Ff &f, Scratch s, const void *x, const void *gy, const void *w_in, 
   void *h = s.take((size_t)most * pitch * 2 * planes), *dgu = s.take((size_t)most * pitch * 4 * planes);
   float *dh = planes == 3 ? (float *)s.take((size_t)most * pitch * sizeof(float)) : nullptr;
   float *part_in = (float *)s.take(split_in * size_in * sizeof(float)), *part_out = (float *)s.take(split_out * size_out * sizeof(float));
-  float *cols_in = (float *)s.take((size_t)kColumnShares * 2 * f.hidden * sizeof(float)), *cols_out = (float *)s.take((size_t)kColumnShares * f.c_out * sizeof(float));
+  const int shares_in = column_shares(f, most, f.hidden, 2), shares_out = column_shares(f, most, f.c_out, 1);
+  float *cols_in = (float *)s.take((size_t)shares_in * 2 * f.hidden * sizeof(float)), *cols_out = (float *)s.take((size_t)shares_out * f.c_out * sizeof(float));
+  float *part = (float *)s.take(parts_bytes(f, most, true));
   cudaError_t e = cudaSuccess;
   for (long long r = 0; r < f.n; r += most) {
     const long long rows = f.n - r < most ? f.n - r : most;
@@ -1380,36 +1477,33 @@ int backward(Ff &f, Scratch s, const void *x, const void *gy, const void *w_in, 
     const int more = r > 0;
     const Matrix xm = operand<T>(f, here, (const T *)x + r * f.c, rows, f.c, 1), gm = operand<T>(f, here, (const T *)gy + r * f.c_out, rows, f.c_out, 1);
     if (dh)
-      if (int k = rows_product<T>(f, gm, wo, 1, false, f.c_out, f.hidden, nullptr, nullptr, dh, pitch)) return k;
+      if (int k = rows_product<T>(f, gm, wo, 1, false, f.c_out, f.hidden, nullptr, nullptr, dh, part, pitch)) return k;
     if (int k = back_product<T>(f, xm, wi, gm, wo, b_in, dh, h, dgu)) return k;
     const Matrix hm = {h, rows, f.hidden, pitch, planes}, dm = {dgu, rows, f.hidden, pitch, 2 * planes};
     if (gx)
-      if (int k = rows_product<T>(f, dm, wi, 1, true, f.hidden, f.c, nullptr, nullptr, (T *)gx + r * f.c)) return k;
+      if (int k = rows_product<T>(f, dm, wi, 1, true, f.hidden, f.c, nullptr, nullptr, (T *)gx + r * f.c, part)) return k;
     if (gw_in)
       if (int k = filter_product<T>(f, dm, xm, 2, f.hidden, f.c, split_in, part_in, more)) return k;
     if (gw_out)
       if (int k = filter_product<T>(f, gm, hm, 1, f.c_out, f.hidden, split_out, part_out, more)) return k;
     const size_t plane = (size_t)rows * pitch;
     if (gb_in && e == cudaSuccess) {
-      const dim3 grid(ceil_div(f.hidden, 32), kColumnShares, 2);
-      if (sizeof(T) == 2)
-        e = launch_ready(ff_columns_kernel<T>, grid, dim3(256), 0, f.st, (const T *)dgu, rows, f.hidden, pitch, 1, (size_t)0, plane, cols_in, more);
-      else
-        e = launch_ready(ff_columns_kernel<__nv_bfloat16>, grid, dim3(256), 0, f.st, (const __nv_bfloat16 *)dgu, rows, f.hidden, pitch, 3, 2 * plane, plane, cols_in, more);
+      const dim3 grid(ceil_div(f.hidden, 256), shares_in, 2);
+      e = launch_ready(ff_columns_kernel<U>, grid, dim3(256), 0, f.st, (const U *)dgu, rows, f.hidden, pitch, planes, planes == 3 ? 2 * plane : (size_t)0, plane, cols_in, more);
       ++f.launches;
     }
     if (gb_out && e == cudaSuccess) {
-      e = launch_ready(ff_columns_kernel<T>, dim3(ceil_div(f.c_out, 32), kColumnShares), dim3(256), 0, f.st, (const T *)gy + r * f.c_out, rows, f.c_out, f.c_out, 1, (size_t)0,
-                       (size_t)0, cols_out, more);
+      e = launch_ready(ff_columns_kernel<U>, dim3(ceil_div(f.c_out, 256), shares_out), dim3(256), 0, f.st, (const U *)gm.p, rows, f.c_out, gm.pitch, planes,
+                       (size_t)rows * gm.pitch, (size_t)0, cols_out, more);
       ++f.launches;
     }
   }
   SumJobs jobs = {};
   unsigned blocks = 0;
-  if (gw_in) add_job(jobs, blocks, part_in, split_in, size_in, gw_in);
-  if (gw_out) add_job(jobs, blocks, part_out, split_out, size_out, gw_out);
-  if (gb_in) add_job(jobs, blocks, cols_in, kColumnShares, 2 * (size_t)f.hidden, gb_in);
-  if (gb_out) add_job(jobs, blocks, cols_out, kColumnShares, f.c_out, gb_out);
+  if (gw_in) add_job(jobs, blocks, part_in, split_in, size_in, gw_in, 0);
+  if (gw_out) add_job(jobs, blocks, part_out, split_out, size_out, gw_out, 0);
+  if (gb_in) add_job(jobs, blocks, cols_in, shares_in, 2 * (size_t)f.hidden, gb_in, 1);
+  if (gb_out) add_job(jobs, blocks, cols_out, shares_out, f.c_out, gb_out, 1);
   if (blocks > 0 && e == cudaSuccess) {
     e = launch_ready(ff_sum_kernel<T>, dim3(blocks), dim3(256), 0, f.st, jobs);
     ++f.launches;
@@ -1423,11 +1517,12 @@ size_t scratch_bytes_for(const Ff &f, bool back) {
   const long long most = rows_at_once(f, back);
   const size_t hidden = align_up((size_t)most * pitch_of(f.hidden) * 2 * planes_for(f.type), 256);
   size_t b = 256 + operand_bytes(f.type, 2ll * f.hidden, f.c) + operand_bytes(f.type, f.c_out, f.hidden) + operand_bytes(f.type, most, f.c);
-  if (!back) return b + hidden;
+  if (!back) return b + hidden + parts_bytes(f, most, false);
   const size_t size_in = 2 * (size_t)f.hidden * f.c, size_out = (size_t)f.c_out * f.hidden;
   b += operand_bytes(f.type, most, f.c_out) + 3 * hidden + 512 + (f.type == SSC_PREC_FP32 ? align_up((size_t)most * pitch_of(f.hidden) * sizeof(float), 256) : 0);
   b += align_up(filter_splits(most, 2, f.hidden, f.c) * size_in * 4, 256) + align_up(filter_splits(most, 1, f.c_out, f.hidden) * size_out * 4, 256);
-  return b + align_up((size_t)kColumnShares * 8 * f.hidden, 256) + align_up((size_t)kColumnShares * 4 * f.c_out, 256);
+  b += parts_bytes(f, most, true);
+  return b + align_up((size_t)column_shares(f, most, f.hidden, 2) * 8 * f.hidden, 256) + align_up((size_t)column_shares(f, most, f.c_out, 1) * 4 * f.c_out, 256);
 }
 
 constexpr int kMostChannels = 65536;

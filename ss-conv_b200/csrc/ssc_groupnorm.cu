@@ -50,21 +50,34 @@ constexpr int kGnStages = 8;
 constexpr int kGnGateRows = 4;             // rows side by side in the gates' part of the backward passes, where a row leaves room for fewer
 constexpr int kGnSum = 32;                  // columns of d_weight | d_bias to a block of the second backward pass
 
-// Rows of T, VEC channels at a time.
+// Rows of T, VEC channels to a thread.  WHOLE: the channels are a multiple of VEC, so that rows start at multiples of VEC; else the last thread of
+// a row has fewer (`many`), and values are read and written one by one.  (A channel to a thread where they are no multiple took three times as long:
+// forward and backward of 171981 rows of 135 channels in fp32 617 us.)
 template <class T, int VEC>
 struct alignas(sizeof(T) * VEC) Pack { T v[VEC]; };
-template <class T, int VEC>
-__device__ __forceinline__ void load(const T *p, float *v) {
-  const Pack<T, VEC> k = *(const Pack<T, VEC> *)p;
+template <class T, int VEC, bool WHOLE>
+__device__ __forceinline__ void load(const T *p, float *v, int many) {
+  if (WHOLE) {
+    const Pack<T, VEC> k = *(const Pack<T, VEC> *)p;
 #pragma unroll
-  for (int q = 0; q < VEC; ++q) v[q] = (float)k.v[q];
+    for (int q = 0; q < VEC; ++q) v[q] = (float)k.v[q];
+  } else {
+#pragma unroll
+    for (int q = 0; q < VEC; ++q) v[q] = q < many ? (float)p[q] : 0.f;
+  }
 }
-template <class T, int VEC>
-__device__ __forceinline__ void store(T *p, const float *v) {
-  Pack<T, VEC> k;
+template <class T, int VEC, bool WHOLE>
+__device__ __forceinline__ void store(T *p, const float *v, int many) {
+  if (WHOLE) {
+    Pack<T, VEC> k;
 #pragma unroll
-  for (int q = 0; q < VEC; ++q) k.v[q] = (T)v[q];
-  *(Pack<T, VEC> *)p = k;
+    for (int q = 0; q < VEC; ++q) k.v[q] = (T)v[q];
+    *(Pack<T, VEC> *)p = k;
+  } else {
+#pragma unroll
+    for (int q = 0; q < VEC; ++q)
+      if (q < many) p[q] = (T)v[q];
+  }
 }
 
 // The block's range of rows as tiles of a ring in shared memory, which thread 0 feeds as it goes: one tile behind, so that it does not wait for
@@ -195,7 +208,7 @@ struct GnWalk {
 // First pass, forward: mean and sum of squared distances of each group of a piece.  A thread takes four rows at a time, exactly
 // (mean first), and adds them to its running values (Chan et al. 1979): sums of squares and of values alone would lose the
 // variance of rows far from zero.
-template <class T, int VEC>
+template <class T, int VEC, bool WHOLE>
 __global__ void __launch_bounds__(kGnThreads, 1) gn_stats_kernel(GnArgs a) {
   after_previous();
   extern __shared__ __align__(128) char smem[];
@@ -205,11 +218,11 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_stats_kernel(GnArgs a) {
   ring.open(a, blockIdx.x, smem, bars, &abort_flag, sizeof(T), 0);
   const int t = threadIdx.x;
   float *sm = (float *)(smem + a.stages * a.stage_bytes);       // [R][c] means, [R][c] squares
-  const int slots = a.c / VEC, R = a.threads / slots, ty = t / slots, ch = (t - ty * slots) * VEC;
+  const int slots = (a.c + VEC - 1) / VEC, R = a.threads / slots, ty = t / slots, ch = (t - ty * slots) * VEC, many = min(VEC, a.c - ch);
   const bool works = ty < R;
   float *sq_s = sm + R * a.c, *sums = sq_s + R * a.c, centred[VEC];       // sums: [c] twice
 #pragma unroll
-  for (int q = 0; q < VEC; ++q) centred[q] = works && a.t.scalar_of_channel[ch + q] >= 0 ? 1.f : 0.f;
+  for (int q = 0; q < VEC; ++q) centred[q] = works && q < many && a.t.scalar_of_channel[ch + q] >= 0 ? 1.f : 0.f;
   GnWalk walk;
   if (ring.r0 < ring.r1) walk.find(a, ring.r0);
   for (int row = ring.r0; row < ring.r1;) {
@@ -224,7 +237,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_stats_kernel(GnArgs a) {
         for (; i + 3 * R < stop; i += 4 * R) {
           float v[4][VEC];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) load<T, VEC>(x + (i + u * R) * a.c, v[u]);
+          for (int u = 0; u < 4; ++u) load<T, VEC, WHOLE>(x + (i + u * R) * a.c, v[u], many);
           const float f = __fdividef(4.f, have + 4.f);
 #pragma unroll
           for (int q = 0; q < VEC; ++q) {
@@ -240,7 +253,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_stats_kernel(GnArgs a) {
         }
         for (; i < stop; i += R) {
           float v[VEC];
-          load<T, VEC>(x + i * a.c, v);
+          load<T, VEC, WHOLE>(x + i * a.c, v, many);
           const float f = __fdividef(1.f, have + 1.f);
 #pragma unroll
           for (int q = 0; q < VEC; ++q) {
@@ -257,10 +270,11 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_stats_kernel(GnArgs a) {
     if (walk.live(a)) {
       if (works) {
 #pragma unroll
-        for (int q = 0; q < VEC; ++q) {
-          sm[ty * a.c + ch + q] = mean[q];
-          sq_s[ty * a.c + ch + q] = sq[q];
-        }
+        for (int q = 0; q < VEC; ++q)
+          if (q < many) {
+            sm[ty * a.c + ch + q] = mean[q];
+            sq_s[ty * a.c + ch + q] = sq[q];
+          }
       }
       __shared__ float count[kGnThreads];
       if (works && ch == 0) count[ty] = have;
@@ -341,7 +355,7 @@ __device__ __forceinline__ void sample_stats(const GnArgs &a, const GnWalk &k, f
 
 // Second pass, forward.  The gates of a tile's rows are computed first, by all threads, into one of two buffers in turn: one wait a
 // tile.
-template <class T, class TO, int VEC, bool GATED>
+template <class T, class TO, int VEC, bool WHOLE, bool GATED>
 __global__ void __launch_bounds__(kGnThreads, 1) gn_apply_kernel(GnArgs a) {
   after_previous();
   extern __shared__ __align__(128) char smem[];
@@ -353,7 +367,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_apply_kernel(GnArgs a) {
   constexpr bool EXACT = sizeof(TO) == 4;
   float *gs = (float *)(smem + a.stages * a.stage_bytes);       // [n_group][2]
   float *gates = gs + 2 * a.n_group;                            // 2 x [tile][n_gate]
-  const int slots = a.c_out / VEC, R = a.threads / slots, ty = t / slots, ch = (t - ty * slots) * VEC;
+  const int slots = (a.c_out + VEC - 1) / VEC, R = a.threads / slots, ty = t / slots, ch = (t - ty * slots) * VEC, many = min(VEC, a.c_out - ch);
   const bool works = ty < R;
   TO *out = (TO *)a.out + ch;
   float w[VEC], b[VEC];
@@ -361,7 +375,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_apply_kernel(GnArgs a) {
   bool mixed = false;                                           // scalars to be activated beside other channels
 #pragma unroll
   for (int q = 0; q < VEC; ++q) {
-    const int c = works ? ch + q : 0, sc = a.t.scalar_of_channel[c];
+    const int c = works && q < many ? ch + q : 0, sc = a.t.scalar_of_channel[c];
     group[q] = 2 * a.t.group_of_channel[c];
     w[q] = a.weight ? a.weight[a.t.field_of_channel[c]] : 1.f;
     b[q] = sc >= 0 && a.bias ? a.bias[sc] : 0.f;
@@ -413,8 +427,8 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_apply_kernel(GnArgs a) {
           float v[2][VEC];
           const bool two = i + R < last - first;
           if (live) {
-            load<T, VEC>(tile + i * a.c + ch, v[0]);
-            load<T, VEC>(tile + (two ? i + R : i) * a.c + ch, v[1]);
+            load<T, VEC, WHOLE>(tile + i * a.c + ch, v[0], many);
+            load<T, VEC, WHOLE>(tile + (two ? i + R : i) * a.c + ch, v[1], many);
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -442,8 +456,8 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_apply_kernel(GnArgs a) {
 #pragma unroll
             for (int k = 0; k < 2 * VEC; ++k) (&v[0][0])[k] = 0.f;
           }
-          store<TO, VEC>(out + (size_t)(first + i) * a.c_out, v[0]);
-          if (two) store<TO, VEC>(out + (size_t)(first + i + R) * a.c_out, v[1]);
+          store<TO, VEC, WHOLE>(out + (size_t)(first + i) * a.c_out, v[0], many);
+          if (two) store<TO, VEC, WHOLE>(out + (size_t)(first + i + R) * a.c_out, v[1], many);
         }
       }
       ring.release(a, last);
@@ -459,7 +473,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_apply_kernel(GnArgs a) {
 // Both backward passes.  SUMS: the sums of dz and dz xhat of each channel, as the groups' sums of a and a xhat of each piece and as the block's
 // share of the parameters' gradients.  Else dx; the first blocks add up the parameters' gradients, kGnSum of them each.
 // The gates of a tile's rows come first, by all threads: value, and (from the products with their fields) dz of the gate channels.
-template <class T, int VEC, bool GATED, bool SUMS>
+template <class T, int VEC, bool WHOLE, bool GATED, bool SUMS>
 __global__ void __launch_bounds__(kGnThreads, 1) gn_bwd_kernel(GnArgs a, int sum_blocks) {
   after_previous();
   extern __shared__ __align__(128) char smem[];
@@ -485,7 +499,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_bwd_kernel(GnArgs a, int sum
   GnRing ring;
   ring.open(a, block, smem, bars, &abort_flag, sizeof(T), sizeof(T));
   constexpr bool EXACT = sizeof(T) == 4;
-  const int slots = a.c_out / VEC, R = a.threads / slots, ty = t / slots, ch = (t - ty * slots) * VEC;
+  const int slots = (a.c_out + VEC - 1) / VEC, R = a.threads / slots, ty = t / slots, ch = (t - ty * slots) * VEC, many = min(VEC, a.c_out - ch);
   const bool works = ty < R;
   const int GR = GATED ? min(a.threads / a.n_gate, max(R, kGnGateRows)) : 1, gj = GATED ? t % a.n_gate : 0, gr = GATED ? t / a.n_gate : 0;
   float *gs = (float *)(smem + a.stages * a.stage_bytes);       // !SUMS: [n_group][2]
@@ -500,7 +514,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_bwd_kernel(GnArgs a, int sum
   unsigned centred = 0;
 #pragma unroll
   for (int q = 0; q < VEC; ++q) {
-    const int c = works ? ch + q : 0, sc = a.t.scalar_of_channel[c];
+    const int c = works && q < many ? ch + q : 0, sc = a.t.scalar_of_channel[c];
     group[q] = a.t.group_of_channel[c];
     w[q] = a.weight ? a.weight[a.t.field_of_channel[c]] : 1.f;
     b[q] = sc >= 0 && a.bias ? a.bias[sc] : 0.f;
@@ -603,8 +617,8 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_bwd_kernel(GnArgs a, int sum
           const int at[2] = {i, two ? i + R : i};
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            load<T, VEC>(tile + at[u] * a.c + ch, hat[u]);
-            load<T, VEC>(grad + at[u] * a.c_out + ch, dz[u]);
+            load<T, VEC, WHOLE>(tile + at[u] * a.c + ch, hat[u], many);
+            load<T, VEC, WHOLE>(grad + at[u] * a.c_out + ch, dz[u], many);
 #pragma unroll
             for (int q = 0; q < VEC; ++q) hat[u][q] = (hat[u][q] - mu[q]) * r[q];
           }
@@ -640,7 +654,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_bwd_kernel(GnArgs a, int sum
             for (int u = 0; u < 2; ++u) {
 #pragma unroll
               for (int q = 0; q < VEC; ++q) dz[u][q] = r[q] * (fmaf(dz[u][q], w[q], -s1[q]) - hat[u][q] * s2[q]);
-              if (u == 0 || two) store<T, VEC>(out + (size_t)(first + at[u]) * a.c, dz[u]);
+              if (u == 0 || two) store<T, VEC, WHOLE>(out + (size_t)(first + at[u]) * a.c, dz[u], many);
             }
           }
         }
@@ -657,10 +671,11 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_bwd_kernel(GnArgs a, int sum
       __syncthreads();
       if (works) {
 #pragma unroll
-        for (int q = 0; q < VEC; ++q) {
-          sums[ty * a.c + ch + q] = s1[q];
-          second[ty * a.c + ch + q] = s2[q];
-        }
+        for (int q = 0; q < VEC; ++q)
+          if (q < many) {
+            sums[ty * a.c + ch + q] = s1[q];
+            second[ty * a.c + ch + q] = s2[q];
+          }
       }
       if (GATED && gr < GR) {
         sums[gr * a.c + a.c_out + gj] = g1;
@@ -708,19 +723,25 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_bwd_kernel(GnArgs a, int sum
 
 int type_bytes(int type) { return type == SSC_PREC_FP32 ? 4 : 2; }
 
-// (eight channels of two rows with their gradients are more than a thread's registers)
-int gn_vec(int c, int c_out, int type, bool grads) {
-  int v = grads ? 4 : 16 / type_bytes(type);
-  while (v > 1 && (c % v || c_out % v)) v /= 2;
-  return v;
+// Channels to a thread: 16 bytes of them, four with their gradients (eight channels of two rows with gradients are more than a thread's
+// registers) and where rows are no multiple.
+struct GnVec {
+  int vec;
+  bool whole;
+};
+GnVec gn_vec(int c, int c_out, int type, bool grads) {
+  const int most = grads ? 4 : 16 / type_bytes(type);
+  if (c % most == 0 && c_out % most == 0) return {most, true};
+  return {4, c % 4 == 0 && c_out % 4 == 0};
 }
 constexpr int kGnBlocks = 2;               // to an SM
 
 // Tiles of four rows to a thread, two where gradients come with them (8 to 16 KB, a multiple of 16 bytes); a ring of up to 88 KB.
 void gn_shape(GnArgs &a, int type, int vec, bool grads) {
   const int bytes = a.c * type_bytes(type);
-  a.threads = a.c / vec > 256 || a.n_gate > 256 ? kGnThreads : 256;
-  const int rows = a.threads / (a.c / vec);
+  const int wide = (a.c + vec - 1) / vec;
+  a.threads = wide > 256 || a.n_gate > 256 ? kGnThreads : 256;
+  const int rows = a.threads / wide;
   const long long slots = (long long)sm_count() * kGnBlocks;
   int each = grads ? 2 : 4;
   while ((rows * each * bytes) % 16 || (rows * each * a.c_out * type_bytes(type)) % 16) each *= 2;
@@ -763,28 +784,28 @@ int gn_fill(GnArgs &a, const int32_t *table, const char *what) {
   return SSC_OK;
 }
 
-template <class T, class TO, int VEC>
+template <class T, class TO, int VEC, bool WHOLE>
 cudaError_t gn_fwd(const GnArgs &a, cudaStream_t st) {
   const dim3 block(a.threads), grid(a.blocks);
-  const size_t ring = (size_t)a.stages * a.stage_bytes, rows = a.threads / (a.c / VEC);
+  const size_t ring = (size_t)a.stages * a.stage_bytes, rows = a.threads / ((a.c + VEC - 1) / VEC);
   const size_t stats = ring + 2 * (rows + 1) * a.c * sizeof(float), room = ring + (2 * (size_t)a.n_group + 2 * (size_t)a.tile * a.n_gate) * sizeof(float);
-  auto apply = a.n_gate ? gn_apply_kernel<T, TO, VEC, true> : gn_apply_kernel<T, TO, VEC, false>;
-  cudaError_t e = allow_smem((const void *)gn_stats_kernel<T, VEC>, stats);
+  auto apply = a.n_gate ? gn_apply_kernel<T, TO, VEC, WHOLE, true> : gn_apply_kernel<T, TO, VEC, WHOLE, false>;
+  cudaError_t e = allow_smem((const void *)gn_stats_kernel<T, VEC, WHOLE>, stats);
   if (e == cudaSuccess) e = allow_smem((const void *)apply, room);
-  if (e == cudaSuccess) e = launch_ready(gn_stats_kernel<T, VEC>, grid, block, stats, st, a);
+  if (e == cudaSuccess) e = launch_ready(gn_stats_kernel<T, VEC, WHOLE>, grid, block, stats, st, a);
   return e == cudaSuccess ? launch_ready(apply, grid, block, room, st, a) : e;
 }
 
-template <class T, int VEC>
+template <class T, int VEC, bool WHOLE>
 cudaError_t gn_bwd(const GnArgs &a, cudaStream_t st) {
   const dim3 block(a.threads);
   const size_t ring = (size_t)a.stages * a.stage_bytes;
-  size_t rows = a.threads / (a.c_out / VEC);
+  size_t rows = a.threads / ((a.c_out + VEC - 1) / VEC);
   if (a.n_gate && rows < (size_t)kGnGateRows) rows = kGnGateRows;
   const size_t gates = 2 * (size_t)a.tile * a.n_gate;
   const size_t first = ring + (gates + 2 * (rows + 1) * a.c) * sizeof(float), second = ring + (gates + 2 * (size_t)a.n_group) * sizeof(float);
-  auto one = a.n_gate ? gn_bwd_kernel<T, VEC, true, true> : gn_bwd_kernel<T, VEC, false, true>;
-  auto two = a.n_gate ? gn_bwd_kernel<T, VEC, true, false> : gn_bwd_kernel<T, VEC, false, false>;
+  auto one = a.n_gate ? gn_bwd_kernel<T, VEC, WHOLE, true, true> : gn_bwd_kernel<T, VEC, WHOLE, false, true>;
+  auto two = a.n_gate ? gn_bwd_kernel<T, VEC, WHOLE, true, false> : gn_bwd_kernel<T, VEC, WHOLE, false, false>;
   cudaError_t e = allow_smem((const void *)one, first);
   if (e == cudaSuccess) e = allow_smem((const void *)two, second);
   const int sum_blocks = ceil_div(a.n_field + a.n_scalar, kGnSum);
@@ -793,21 +814,14 @@ cudaError_t gn_bwd(const GnArgs &a, cudaStream_t st) {
 }
 
 template <class T, class TO>
-cudaError_t gn_fwd_vec(const GnArgs &a, int vec, cudaStream_t st) {
-  switch (vec) {
-    case 8: if constexpr (sizeof(T) == 2) return gn_fwd<T, TO, 8>(a, st);
-    case 4: return gn_fwd<T, TO, 4>(a, st);
-    case 2: return gn_fwd<T, TO, 2>(a, st);
-    default: return gn_fwd<T, TO, 1>(a, st);
-  }
+cudaError_t gn_fwd_vec(const GnArgs &a, GnVec v, cudaStream_t st) {
+  if constexpr (sizeof(T) == 2)
+    if (v.vec == 8) return gn_fwd<T, TO, 8, true>(a, st);
+  return v.whole ? gn_fwd<T, TO, 4, true>(a, st) : gn_fwd<T, TO, 4, false>(a, st);
 }
 template <class T>
-cudaError_t gn_bwd_vec(const GnArgs &a, int vec, cudaStream_t st) {
-  switch (vec) {
-    case 4: return gn_bwd<T, 4>(a, st);
-    case 2: return gn_bwd<T, 2>(a, st);
-    default: return gn_bwd<T, 1>(a, st);
-  }
+cudaError_t gn_bwd_vec(const GnArgs &a, GnVec v, cudaStream_t st) {
+  return v.whole ? gn_bwd<T, 4, true>(a, st) : gn_bwd<T, 4, false>(a, st);
 }
 bool known_type(int t) { return t == SSC_PREC_FP32 || t == SSC_PREC_F16 || t == SSC_PREC_BF16; }
 
@@ -830,10 +844,10 @@ extern "C" int ssc_group_norm_fwd(const void *x, int type, int n, int c, const i
   a.status = status;
   if (int e = gn_fill(a, table, "group_norm_fwd")) return e;
   if (n == 0) return SSC_OK;
-  const int vec = gn_vec(c, a.c_out, type, false);
+  const GnVec vec = gn_vec(c, a.c_out, type, false);
   SSC_REQUIRE(n_gate <= kGnThreads, "group_norm_fwd: %d gates, at most %d", n_gate, kGnThreads);
-  SSC_REQUIRE(c / vec <= kGnThreads, "group_norm_fwd: %d channels, at most %d of this divisibility", c, kGnThreads * vec);
-  gn_shape(a, type, vec, false);
+  SSC_REQUIRE(c <= 4 * kGnThreads, "group_norm_fwd: %d channels, at most %d", c, 4 * kGnThreads);
+  gn_shape(a, type, vec.vec, false);
   if (scratch == nullptr || ((uintptr_t)scratch & 15) != 0 || scratch_bytes < gn_scratch(batch, n_group, 0)) return fail(SSC_ERR_SCRATCH, "group_norm_fwd: scratch too small");
   a.partial = (float *)scratch;
   const cudaStream_t st = as_stream(stream);
@@ -868,10 +882,10 @@ extern "C" int ssc_group_norm_bwd(const void *x, const void *gy, int type, int n
     if (e != cudaSuccess) return fail(SSC_ERR_CUDA, "group_norm_bwd: %s", cudaGetErrorString(e));
     return SSC_OK;
   }
-  const int vec = gn_vec(c, a.c_out, type, true);
+  const GnVec vec = gn_vec(c, a.c_out, type, true);
   SSC_REQUIRE(n_gate <= kGnThreads, "group_norm_bwd: %d gates, at most %d", n_gate, kGnThreads);
-  SSC_REQUIRE(c / vec <= kGnThreads, "group_norm_bwd: %d channels, at most %d of this divisibility", c, kGnThreads * vec);
-  gn_shape(a, type, vec, true);
+  SSC_REQUIRE(c <= 4 * kGnThreads, "group_norm_bwd: %d channels, at most %d", c, 4 * kGnThreads);
+  gn_shape(a, type, vec.vec, true);
   if (scratch == nullptr || ((uintptr_t)scratch & 15) != 0 || scratch_bytes < gn_scratch(batch, n_group, n_field + n_scalar))
     return fail(SSC_ERR_SCRATCH, "group_norm_bwd: scratch too small");
   a.partial = (float *)scratch;

@@ -68,7 +68,10 @@ CASES = [
     ([5, 0, 1, 300], [(64, 0)], 32, F.silu),
     ([0, 700], [(2, 0), (2, 1), (2, 2), (2, 3), (6, 0)], 1, GATE),
     ([1021, 33], [(9, 0), (3, 1), (3, 2), (6, 0)], 3, GATE),            # 45 channels and gates: one channel at a time
-    ([513], [(4, 0), (2, 1)], 2, (F.gelu, None)),                       # fields of order l > 0 without gates
+    ([513], [(4, 0), (2, 1)], 2, (F.gelu, None)),
+    ([77, 500], [(2047, 0)], 23, F.silu),                               # wide, no multiple of anything
+    ([600], [(5, 0), (3, 2)], 1, None),
+    ([50, 900], [(7, 0), (1, 1), (2, 3), (3, 0)], 1, GATE),                       # fields of order l > 0 without gates
     ([129, 64], [(3, 1), (3, 0)], 3, (None, torch.sigmoid)),            # no scalars but the gates
     ([2000], [(1, 0)], 1, F.gelu),
     ([40, 60], [(510, 0)], 2, F.relu),
@@ -281,8 +284,10 @@ def test_refusals(cuda):
         group_norm(x, off.cpu(), Rs)
     with pytest.raises(ValueError, match="weight"):
         group_norm(x, off, Rs, weight=torch.ones(5, device=cuda))
-    with pytest.raises(ValueError, match="at most 512"):
-        group_norm(torch.zeros(4, 513, device=cuda), off, [(513, 0)])
+    with pytest.raises(ValueError, match="at most 2048"):
+        group_norm(torch.zeros(4, 2049, device=cuda), off, [(2049, 0)])
+    with pytest.raises(ValueError, match="513 gates"):
+        group_norm(torch.zeros(4, 2052, device=cuda), off, [(513, 1), (513, 0)], activation=(None, torch.sigmoid))
     assert group_norm(x[:0], torch.zeros(2, dtype=torch.int32, device=cuda), Rs).shape == (0, 6)
     e = x[:0].requires_grad_(True)
     w = torch.ones(6, device=cuda, requires_grad=True)
