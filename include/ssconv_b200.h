@@ -598,7 +598,7 @@ int ssc_gate_bwd(const float *x, const float *gy, int n, int c_total, int c_out,
  * group_copies [n_group].  weight [n_field] and bias [n_scalar] float32 or NULL.  Activations: 0 identity, 1 relu, 2 sigmoid,
  * 3 silu, 4 gelu (erf).  out_type is `type`, or any for float32 rows.  stats [batch, n_group, 2] float32 receives mean (0 for l > 0) and
  * (variance + eps)^-1/2 of every sample that has rows, which the backward call reads.  Sums are float32, in a fixed order.
- * c is at most 2048 channels, with at most 512 gates.  Rows and scratch
+ * c is at most 2048 channels, with at most 512 gates, n at most 2^30.  Rows and scratch
  * start at multiples of 16 bytes.  scratch: ssc_group_norm_scratch_bytes(...) (forward: n_field = n_scalar = 0 will do).  status: as in
  * ssc_conv_fwd.  gx has the type of x; d_weight [n_field], d_bias [n_scalar] float32. */
 size_t ssc_group_norm_scratch_bytes(int batch, int n_group, int n_field, int n_scalar);
@@ -617,7 +617,7 @@ int ssc_group_norm_bwd(const void *x, const void *gy, int type, int n, int c, co
  * `type` (SSC_PREC_FP32 / F16 / BF16); the biases and the residual may be NULL.  act: 0 identity, 1 relu, 2 sigmoid, 3 silu,
  * 4 gelu (erf).  Products are added in float32; float32 operands are used to 24 bits; in 16 bits the hidden rows h = act(.) * (.), and
  * in the backward call their gradients, are rounded to the rows' type (up to 16 rows forward: not rounded).  A value that is not
- * finite makes what depends on it infinite or NaN.  Sizes are at most 65536; any address and width is accepted, 16-bit widths that are
+ * finite makes what depends on it infinite or NaN.  Widths are at most 65536, rows at most 2^30; any address and width is accepted, 16-bit widths that are
  * multiples of 8 at addresses that are multiples of 16 are read in place, others are copied to scratch first.
  * scratch: ssc_gated_ff_scratch_bytes(...) bytes, 16-byte aligned; rows are taken in turns so that it stays below about
  * a gigabyte beside the weights.  Sums have a fixed order.

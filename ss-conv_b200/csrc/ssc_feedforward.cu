@@ -1528,7 +1528,7 @@ size_t scratch_bytes_for(const Ff &f, bool back) {
 constexpr int kMostChannels = 65536;
 int ff_check(const Ff &f, const char *what) {
   SSC_REQUIRE(f.type == SSC_PREC_FP32 || f.type == SSC_PREC_F16 || f.type == SSC_PREC_BF16, "%s: unknown type", what);
-  SSC_REQUIRE(f.n >= 0 && f.c >= 1 && f.hidden >= 1 && f.c_out >= 1 && f.c <= kMostChannels && f.hidden <= kMostChannels && f.c_out <= kMostChannels, "%s: bad sizes", what);
+  SSC_REQUIRE(f.n >= 0 && f.n <= 1 << 30 && f.c >= 1 && f.hidden >= 1 && f.c_out >= 1 && f.c <= kMostChannels && f.hidden <= kMostChannels && f.c_out <= kMostChannels, "%s: bad sizes", what);
   SSC_REQUIRE(f.act >= 0 && f.act <= 4, "%s: unknown activation", what);
   return SSC_OK;
 }

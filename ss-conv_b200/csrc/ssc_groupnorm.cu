@@ -762,7 +762,7 @@ size_t gn_scratch(int batch, int n_group, int n_cols) {
 }
 
 int gn_fill(GnArgs &a, const int32_t *table, const char *what) {
-  SSC_REQUIRE(a.n >= 0 && a.batch >= 1 && a.c >= 1 && a.c_out >= 1 && a.n_gate >= 0 && a.c_out + a.n_gate == a.c, "%s: bad sizes", what);
+  SSC_REQUIRE(a.n >= 0 && a.n <= 1 << 30 && a.batch >= 1 && a.c >= 1 && a.c_out >= 1 && a.n_gate >= 0 && a.c_out + a.n_gate == a.c, "%s: bad sizes", what);
   SSC_REQUIRE(a.n_group >= 1 && a.n_group <= a.c && a.n_field >= 1 && a.n_field <= a.c && a.n_scalar >= 0 && a.n_scalar <= a.n_field, "%s: bad layout", what);
   SSC_REQUIRE(a.scalar_act >= 0 && a.scalar_act <= 4 && a.gate_act >= 0 && a.gate_act <= 4, "%s: unknown activation", what);
   SSC_REQUIRE(a.eps > 0.f, "%s: eps must be positive", what);

@@ -57,7 +57,7 @@ std::string shape_of(const Tensor &t) {
 void check_rows(const Tensor &x) {
   TORCH_CHECK(x.is_cuda(), "ssconv_b200 runs on CUDA tensors only (got a ", c10::DeviceTypeName(x.device().type(), true), " tensor)");
   TORCH_CHECK_TYPE(code_of(x.scalar_type()) >= 0, "features must be float32, float16 or bfloat16 (got ", x.scalar_type(), ")");
-  TORCH_CHECK_VALUE(x.dim() == 2 && x.size(0) < (int64_t)1 << 31, "features must be [N, C] with fewer than 2^31 rows (got ", shape_of(x), ")");
+  TORCH_CHECK_VALUE(x.dim() == 2 && x.size(0) <= (int64_t)1 << 30, "features must be [N, C] with at most 2^30 rows (got ", shape_of(x), ")");
 }
 bool recorded(std::initializer_list<const Tensor *> all) {
   if (!at::GradMode::is_enabled()) return false;

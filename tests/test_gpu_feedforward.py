@@ -135,6 +135,30 @@ def test_some_gradients_alone_and_differences(cuda):
         assert abs(num.item() - flat[at].item()) <= 1e-2 * max(1.0, abs(flat[at].item())), name
 
 
+def test_rows_taken_in_turns(cuda):
+    """More rows than one turn's scratch holds: the rows of all turns, the gradients of the weights over all of them, and the same bits
+    twice.  float32, so the errors are those of the norm test below."""
+    from ss_conv.feedforward import gated_feedforward
+    from ss_conv import _ext
+    n, c, h = 70001, 16, 2048
+    one, all_ = (int(_ext.lib().ssc_gated_ff_scratch_bytes(0, k, c, h, c, 1)) for k in (20000, n))
+    assert all_ < 3 * one                                       # (three turns or more)
+    t, gy = inputs(n, c, h, c, torch.float32, True, False, 12)
+    names = ["x", "w_in", "w_out", "b_in", "b_out"]
+    dev = {k: t[k].to(cuda).requires_grad_(True) for k in names}
+    d64 = {k: t[k].double().to(cuda).requires_grad_(True) for k in names}
+    runs = []
+    for _ in range(2):
+        y = gated_feedforward(*(dev[k] for k in names))
+        runs.append([y.detach(), *torch.autograd.grad(y, [dev[k] for k in names], gy.to(cuda))])
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+    want = reference({**d64, "residual": None}, F.silu)
+    exact = [want.detach(), *torch.autograd.grad(want, [d64[k] for k in names], gy.double().to(cuda))]
+    for name, a, b in zip(["y"] + names, runs[0], exact):
+        assert ((a.double() - b).norm() / b.norm()).item() < 2e-6, name
+    assert (runs[0][0][-1].double() - exact[0][-1]).abs().max() < 1e-4 and (runs[0][1][-1].double() - exact[1][-1]).abs().max() < 1e-4
+
+
 def test_every_choice_of_gradients(cuda):
     """Arguments that are absent, and those that ask for no gradient, in all combinations: each gradient is its own argument's."""
     import itertools

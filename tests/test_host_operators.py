@@ -43,7 +43,7 @@ def test_library_refuses_bad_arguments_of_the_norm():
                                     None, None, 0, None)
 
     assert forward() == 0                                               # no rows: nothing to do
-    for bad in (dict(type=1), dict(type=2, out_type=0), dict(n=-1), dict(c=0), dict(batch=0), dict(fields=9), dict(scalars=9), dict(groups=0),
+    for bad in (dict(type=1), dict(type=2, out_type=0), dict(n=-1), dict(n=2 ** 30 + 1), dict(c=0), dict(batch=0), dict(fields=9), dict(scalars=9), dict(groups=0),
                 dict(gates=8), dict(act=5), dict(eps=0.0), dict(table=None)):
         assert forward(**bad) == 1, bad
     assert forward(n=5) == 3 and b"scratch" in L.ssc_last_error()
@@ -59,7 +59,7 @@ def test_feedforward_refusals():
         return L.ssc_gated_ff_fwd(64, type, n, c, hidden, out, w, 64, None, None, None, act, 64, None, None, 0, None)
 
     assert forward() == 0
-    for bad in (dict(type=1), dict(type=4), dict(n=-1), dict(c=0), dict(hidden=0), dict(out=0), dict(hidden=65537), dict(act=5), dict(act=-1), dict(w=None)):
+    for bad in (dict(type=1), dict(type=4), dict(n=-1), dict(n=2 ** 30 + 1), dict(c=0), dict(hidden=0), dict(out=0), dict(hidden=65537), dict(act=5), dict(act=-1), dict(w=None)):
         assert forward(**bad) == 1, bad
     assert forward(n=5) == 3 and b"scratch" in L.ssc_last_error()
     assert L.ssc_gated_ff_bwd(64, 64, 0, 5, 8, 8, 8, 64, 64, None, 3, 64, None, None, None, None, None, None, 0, None) == 3
@@ -76,5 +76,5 @@ def test_feedforward_scratch_is_bounded_and_covers_its_pieces():
     L = _ext.lib()
     for kind in (0, 2, 3):
         for back in (0, 1):
-            sizes = [int(L.ssc_gated_ff_scratch_bytes(kind, n, 512, 2048, 512, back)) for n in (0, 1, 16, 17, 64, 65, 1000, 100000, 1000000, 2 ** 31 - 1)]
+            sizes = [int(L.ssc_gated_ff_scratch_bytes(kind, n, 512, 2048, 512, back)) for n in (0, 1, 16, 17, 64, 65, 1000, 100000, 1000000, 2 ** 30)]
             assert max(sizes) < 3 * 2 ** 30 and all(s > 0 for s in sizes)
