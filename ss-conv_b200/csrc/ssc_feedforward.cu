@@ -276,10 +276,10 @@ __device__ __forceinline__ void finish_back(const FfParams &p, const FfMaps &map
   act_slopes<sizeof(T) == 4, 16>(v, s, p.act);
 #pragma unroll
   for (int i = 0; i < 16; ++i) h[i] = v[i];
-  multiply<16>(h, u);           // act(g) u
-  multiply<16>(u, s);
-  multiply<16>(u, d);           // dh u act'(g)
-  multiply<16>(v, d);           // dh act(g)
+  multiply<16>(h, h, u);        // act(g) u
+  multiply<16>(u, u, s);
+  multiply<16>(u, u, d);        // dh u act'(g)
+  multiply<16>(v, v, d);        // dh act(g)
   if constexpr (sizeof(T) == 2) {
     if (half == 0) {            // three boxes at a time
       if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
@@ -327,7 +327,7 @@ __device__ __forceinline__ void finish(const FfParams &p, const FfMaps &maps, Ou
         add16<T>(u[q], (const T *)p.bias + p.cols + n + 16 * q, left, 0);
       }
       act_values<sizeof(T) == 4, 16>(v[q], p.act);
-      multiply<16>(v[q], u[q]);
+      multiply<16>(v[q], v[q], u[q]);
     }
     send_hidden<T>(box, &maps.out[0], v, n, row0, 0, 1);
     return;
@@ -803,7 +803,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHiddenThreads, 1) f
               add16<T>(w[i], (const T *)p.bias + p.cols + n + 16 * i, left, 0);
             }
             act_values<sizeof(T) == 4, 16>(v[i], p.act);
-            multiply<16>(v[i], w[i]);
+            multiply<16>(v[i], v[i], w[i]);
           }
           if constexpr (sizeof(T) == 2) {
             if (q == 0) at = box.room();

@@ -220,9 +220,9 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_stats_kernel(GnArgs a) {
   float *sm = (float *)(smem + a.stages * a.stage_bytes);       // [R][c] means, [R][c] squares
   const int slots = (a.c + VEC - 1) / VEC, R = a.threads / slots, ty = t / slots, ch = (t - ty * slots) * VEC, many = min(VEC, a.c - ch);
   const bool works = ty < R;
-  float *sq_s = sm + R * a.c, *sums = sq_s + R * a.c, centred[VEC];       // sums: [c] twice
+  float *sq_s = sm + R * a.c, *sums = sq_s + R * a.c, centred[VEC], quarter[VEC];       // sums: [c] twice
 #pragma unroll
-  for (int q = 0; q < VEC; ++q) centred[q] = works && q < many && a.t.scalar_of_channel[ch + q] >= 0 ? 1.f : 0.f;
+  for (int q = 0; q < VEC; ++q) centred[q] = works && q < many && a.t.scalar_of_channel[ch + q] >= 0 ? 1.f : 0.f, quarter[q] = 0.25f * centred[q];
   GnWalk walk;
   if (ring.r0 < ring.r1) walk.find(a, ring.r0);
   for (int row = ring.r0; row < ring.r1;) {
@@ -239,16 +239,22 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_stats_kernel(GnArgs a) {
 #pragma unroll
           for (int u = 0; u < 4; ++u) load<T, VEC, WHOLE>(x + (i + u * R) * a.c, v[u], many);
           const float f = __fdividef(4.f, have + 4.f);
+          float mb[VEC], d[VEC], s[VEC];
+          multiply_add<VEC>(mb, v[0], 1.f, v[1]);
+          multiply_add<VEC>(d, v[2], 1.f, v[3]);
+          multiply_add<VEC>(mb, mb, 1.f, d);
+          multiply<VEC>(mb, mb, quarter);
 #pragma unroll
-          for (int q = 0; q < VEC; ++q) {
-            const float mb = ((v[0][q] + v[1][q]) + (v[2][q] + v[3][q])) * (0.25f * centred[q]);
-            float s = 0.f;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) s = fmaf(v[u][q] - mb, v[u][q] - mb, s);
-            const float d = mb - mean[q];
-            mean[q] = fmaf(d, f, mean[q]);
-            sq[q] += fmaf(d * d, have * f, s);
+          for (int u = 0; u < 4; ++u) {
+            multiply_add<VEC>(d, mb, -1.f, v[u]);
+            if (u == 0) multiply<VEC>(s, d, d);
+            else multiply_add<VEC>(s, d, d, s);
           }
+          multiply_add<VEC>(d, mean, -1.f, mb);
+          multiply_add<VEC>(mean, d, f, mean);
+          multiply<VEC>(d, d, d);
+          multiply_add<VEC>(s, d, have * f, s);
+          multiply_add<VEC>(sq, sq, 1.f, s);
           have += 4.f;
         }
         for (; i < stop; i += R) {
@@ -429,10 +435,8 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_apply_kernel(GnArgs a) {
           if (live) {
             load<T, VEC, WHOLE>(tile + i * a.c + ch, v[0], many);
             load<T, VEC, WHOLE>(tile + (two ? i + R : i) * a.c + ch, v[1], many);
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-              for (int q = 0; q < VEC; ++q) v[u][q] = fmaf(v[u][q], scale[q], shift[q]);
+            multiply_add<VEC>(v[0], v[0], (const float *)scale, (const float *)shift);
+            multiply_add<VEC>(v[1], v[1], (const float *)scale, (const float *)shift);
             if (!mixed) {
               if (gate[0] == -1) act_values<EXACT, 2 * VEC>(&v[0][0], a.scalar_act);
             } else {
@@ -579,8 +583,8 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_bwd_kernel(GnArgs a, int sum
         __syncthreads();
 #pragma unroll
         for (int q = 0; q < VEC; ++q) {
-          s1[q] = centred >> q & 1 ? gs[2 * group[q]] : 0.f;
-          s2[q] = gs[2 * group[q] + 1];
+          s1[q] = centred >> q & 1 ? -gs[2 * group[q]] : 0.f;
+          s2[q] = -gs[2 * group[q] + 1];
         }
         if (GATED) {
           g1 = gs[2 * gg];
@@ -619,15 +623,13 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_bwd_kernel(GnArgs a, int sum
           for (int u = 0; u < 2; ++u) {
             load<T, VEC, WHOLE>(tile + at[u] * a.c + ch, hat[u], many);
             load<T, VEC, WHOLE>(grad + at[u] * a.c_out + ch, dz[u], many);
-#pragma unroll
-            for (int q = 0; q < VEC; ++q) hat[u][q] = (hat[u][q] - mu[q]) * r[q];
+            multiply_add<VEC>(hat[u], mu, -1.f, hat[u]);
+            multiply<VEC>(hat[u], hat[u], r);
           }
           if (scalars) {
             float z[2][VEC], slope[2][VEC];
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-              for (int q = 0; q < VEC; ++q) z[u][q] = fmaf(hat[u][q], w[q], b[q]);
+            for (int u = 0; u < 2; ++u) multiply_add<VEC>(z[u], hat[u], w, b);
             act_slopes<EXACT, 2 * VEC>(&z[0][0], &slope[0][0], a.scalar_act);
 #pragma unroll
             for (int u = 0; u < 2; ++u)
@@ -643,17 +645,19 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_bwd_kernel(GnArgs a, int sum
                 if (gate[q] >= 0) dz[u][q] *= gates[at[u] * a.n_gate + gate[q]];
           }
           if (SUMS) {
-#pragma unroll
-            for (int q = 0; q < VEC; ++q) {
-              s1[q] += two ? dz[0][q] + dz[1][q] : dz[0][q];
-              s2[q] = fmaf(dz[0][q], hat[0][q], s2[q]);
-              if (two) s2[q] = fmaf(dz[1][q], hat[1][q], s2[q]);
+            multiply_add<VEC>(s1, s1, 1.f, dz[0]);
+            multiply_add<VEC>(s2, dz[0], hat[0], s2);
+            if (two) {
+              multiply_add<VEC>(s1, s1, 1.f, dz[1]);
+              multiply_add<VEC>(s2, dz[1], hat[1], s2);
             }
           } else {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-#pragma unroll
-              for (int q = 0; q < VEC; ++q) dz[u][q] = r[q] * (fmaf(dz[u][q], w[q], -s1[q]) - hat[u][q] * s2[q]);
+              // (s1 and s2 are negative here)
+              multiply_add<VEC>(dz[u], dz[u], w, s1);
+              multiply_add<VEC>(dz[u], hat[u], s2, dz[u]);
+              multiply<VEC>(dz[u], dz[u], r);
               if (u == 0 || two) store<T, VEC, WHOLE>(out + (size_t)(first + at[u]) * a.c, dz[u], many);
             }
           }
