@@ -835,12 +835,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHiddenThreads, 1) f
 }
 
 // Rows [rows][cols] of float32 as three bfloat16 planes, or 16-bit rows that TMA cannot read as they are (a width or an address
-// that is no multiple of 16 bytes), to rows of `pitch` elements.
+// that is no multiple of 16 bytes), to rows of `pitch` elements: the operands of a call in one launch.
+struct PlaneJob {
+  const void *src;
+  void *dst;
+  long long rows;
+  int cols, pitch;
+  unsigned first;                   // block
+};
+struct PlaneJobs {
+  PlaneJob job[4];
+  int many;
+};
 template <class T>
-__global__ void __launch_bounds__(256) ff_planes_kernel(const T *__restrict__ src, long long rows, int cols, int pitch, void *dst) {
+__global__ void __launch_bounds__(256) ff_planes_kernel(const PlaneJobs jobs) {
   after_previous();
-  const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
-  const int per = pitch / 8;
+  int j = 0;
+  while (j + 1 < jobs.many && blockIdx.x >= jobs.job[j + 1].first) ++j;
+  const PlaneJob &s = jobs.job[j];
+  const T *src = (const T *)s.src;
+  void *dst = s.dst;
+  const long long rows = s.rows, t = (long long)(blockIdx.x - s.first) * 256 + threadIdx.x;
+  const int cols = s.cols, pitch = s.pitch, per = pitch / 8;
   const long long row = t / per;
   if (row >= rows) return;
   const int c0 = (int)(t - row * per) * 8;
@@ -915,19 +931,30 @@ __global__ void __launch_bounds__(256) ff_sum_kernel(const SumJobs jobs) {
   ((T *)s.out)[at] = (T)v;
 }
 
-// Column sums of one or two matrices [rows][pitch] (planes of float32 ones added up), a block's share of the rows: part[blockIdx.y][matrices * cols].
+// Column sums of matrices [rows][pitch] (planes of float32 ones added up), a block's share of the rows: part[blockIdx.y * stride + column].
 // A thread has eight columns; rows start at multiples of 16 bytes.
+struct Columns {
+  const void *src;
+  int cols, pitch, shares;
+  size_t plane, stride;             // planes lie so far apart
+  float *part;
+};
+struct ColumnJobs {
+  Columns job[3];
+};
 template <class T>
-__global__ void __launch_bounds__(256) ff_columns_kernel(const T *__restrict__ src, long long rows, int cols, int pitch, int planes, size_t plane, size_t matrix,
-                                                         float *__restrict__ part, int accumulate) {
+__global__ void __launch_bounds__(256) ff_columns_kernel(const ColumnJobs jobs, long long rows, int planes, int accumulate) {
   after_previous();
   __shared__ float sm[256][9];
+  const Columns &s = jobs.job[blockIdx.z];
+  const int cols = s.cols, pitch = s.pitch;
+  if ((int)blockIdx.x * 256 >= cols || (int)blockIdx.y >= s.shares) return;
   const int groups = min((cols + 7) / 8 - (int)blockIdx.x * 32, 32), R = 256 / groups, g = threadIdx.x % groups, w = threadIdx.x / groups, c0 = (blockIdx.x * 32 + g) * 8;
-  const long long lo = rows * blockIdx.y / gridDim.y, hi = rows * (blockIdx.y + 1) / gridDim.y;
+  const long long lo = rows * blockIdx.y / s.shares, hi = rows * (blockIdx.y + 1) / s.shares;
   float v[8] = {};
   if (w < R)
     for (int k = planes - 1; k >= 0; --k) {
-      const T *from = src + blockIdx.z * matrix + k * plane + c0;
+      const T *from = (const T *)s.src + k * s.plane + c0;
 #pragma unroll 4
       for (long long r = lo + w; r < hi; r += R) {
         struct alignas(16) { T v[8]; } q;
@@ -944,7 +971,7 @@ __global__ void __launch_bounds__(256) ff_columns_kernel(const T *__restrict__ s
     if (col >= cols) continue;
     float sum = 0.f;
     for (int i = 0; i < R; ++i) sum += sm[i * groups + t / 8][t % 8];
-    float *o = part + ((size_t)blockIdx.y * gridDim.z + blockIdx.z) * cols + col;
+    float *o = s.part + blockIdx.y * s.stride + col;
     *o = accumulate ? *o + sum : sum;
   }
 }
@@ -1119,22 +1146,30 @@ struct Ff {
   cudaStream_t st;
   int32_t *status;
   int launches;
-  cudaError_t err;
+  PlaneJobs planes;         // operands still to be laid out, and their blocks
+  unsigned plane_blocks;
 };
 
-// The matrix as TMA reads it: itself, or planes / padded rows in scratch.
+// The matrix as TMA reads it: itself, or planes / padded rows in scratch, which lay_out fills.
 template <class T>
 Matrix operand(Ff &f, Scratch &s, const void *p, long long rows, int cols, int each) {
   const int pitch = pitch_of(cols), planes = planes_for(f.type);
   if (sizeof(T) == 2 && cols % 8 == 0 && ((uintptr_t)p & 15) == 0) return {p, rows / each, cols, cols, each};
   void *to = s.take((size_t)rows * pitch * 2 * planes);
   if (s.base != nullptr) {
-    const long long threads = rows * (pitch / 8);
-    const cudaError_t e = launch_ready(ff_planes_kernel<T>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, f.st, (const T *)p, rows, cols, pitch, to);
-    if (e != cudaSuccess) f.err = e;
-    ++f.launches;
+    f.planes.job[f.planes.many++] = {p, to, rows, cols, pitch, f.plane_blocks};
+    f.plane_blocks += (unsigned)((rows * (pitch / 8) + 255) / 256);
   }
   return {to, rows / each, cols, pitch, planes * each};
+}
+template <class T>
+int lay_out(Ff &f) {
+  if (f.planes.many == 0) return SSC_OK;
+  const cudaError_t e = launch_ready(ff_planes_kernel<T>, dim3(f.plane_blocks), dim3(256), 0, f.st, f.planes);
+  f.planes.many = 0;
+  f.plane_blocks = 0;
+  ++f.launches;
+  return e == cudaSuccess ? SSC_OK : fail(SSC_ERR_CUDA, "gated_ff: %s", cudaGetErrorString(e));
 }
 // (what operand() may take of the scratch; whether an address is aligned is not known when sizes are asked for)
 size_t operand_bytes(int type, long long rows, int cols) { return align_up((size_t)rows * pitch_of(cols) * 2 * planes_for(type), 256); }
@@ -1448,6 +1483,7 @@ int forward(Ff &f, Scratch s, const void *x, const void *w_in, const void *w_out
     const long long rows = f.n - r < most ? f.n - r : most;
     Scratch here = s;
     const Matrix xm = operand<T>(f, here, (const T *)x + r * f.c, rows, f.c, 1);
+    if (int e = lay_out<T>(f)) return e;
     if (int e = gate_product<T>(f, xm, wi, b_in, h)) return e;
     const Matrix hm = {h, rows, f.hidden, pitch, planes};
     if (int e = rows_product<T>(f, hm, wo, 0, false, f.hidden, f.c_out, b_out, residual ? (const T *)residual + r * f.c_out : nullptr, (T *)out + r * f.c_out, part)) return e;
@@ -1470,12 +1506,12 @@ int backward(Ff &f, Scratch s, const void *x, const void *gy, const void *w_in, 
   const int shares_in = column_shares(f, most, f.hidden, 2), shares_out = column_shares(f, most, f.c_out, 1);
   float *cols_in = (float *)s.take((size_t)shares_in * 2 * f.hidden * sizeof(float)), *cols_out = (float *)s.take((size_t)shares_out * f.c_out * sizeof(float));
   float *part = (float *)s.take(parts_bytes(f, most, true));
-  cudaError_t e = cudaSuccess;
   for (long long r = 0; r < f.n; r += most) {
     const long long rows = f.n - r < most ? f.n - r : most;
     Scratch here = s;
     const int more = r > 0;
     const Matrix xm = operand<T>(f, here, (const T *)x + r * f.c, rows, f.c, 1), gm = operand<T>(f, here, (const T *)gy + r * f.c_out, rows, f.c_out, 1);
+    if (int k = lay_out<T>(f)) return k;
     if (dh)
       if (int k = rows_product<T>(f, gm, wo, 1, false, f.c_out, f.hidden, nullptr, nullptr, dh, part, pitch)) return k;
     if (int k = back_product<T>(f, xm, wi, gm, wo, b_in, dh, h, dgu)) return k;
@@ -1487,14 +1523,16 @@ int backward(Ff &f, Scratch s, const void *x, const void *gy, const void *w_in, 
     if (gw_out)
       if (int k = filter_product<T>(f, gm, hm, 1, f.c_out, f.hidden, split_out, part_out, more)) return k;
     const size_t plane = (size_t)rows * pitch;
-    if (gb_in && e == cudaSuccess) {
-      const dim3 grid(ceil_div(f.hidden, 256), shares_in, 2);
-      e = launch_ready(ff_columns_kernel<U>, grid, dim3(256), 0, f.st, (const U *)dgu, rows, f.hidden, pitch, planes, planes == 3 ? 2 * plane : (size_t)0, plane, cols_in, more);
-      ++f.launches;
-    }
-    if (gb_out && e == cudaSuccess) {
-      e = launch_ready(ff_columns_kernel<U>, dim3(ceil_div(f.c_out, 256), shares_out), dim3(256), 0, f.st, (const U *)gm.p, rows, f.c_out, gm.pitch, planes,
-                       (size_t)rows * gm.pitch, (size_t)0, cols_out, more);
+    if (gb_in || gb_out) {
+      ColumnJobs jobs = {};
+      int many = 0;
+      for (int i = 0; gb_in && i < 2; ++i)
+        jobs.job[many++] = {(const U *)dgu + i * plane, f.hidden, pitch, shares_in, planes == 3 ? 2 * plane : 0, 2 * (size_t)f.hidden, cols_in + (size_t)i * f.hidden};
+      if (gb_out) jobs.job[many++] = {gm.p, f.c_out, gm.pitch, shares_out, (size_t)rows * gm.pitch, (size_t)f.c_out, cols_out};
+      const int widest = gb_in && (!gb_out || f.hidden > f.c_out) ? f.hidden : f.c_out;
+      const int shares = gb_in && (!gb_out || shares_in > shares_out) ? shares_in : shares_out;
+      const cudaError_t e = launch_ready(ff_columns_kernel<U>, dim3(ceil_div(widest, 256), shares, many), dim3(256), 0, f.st, jobs, rows, planes, more);
+      if (e != cudaSuccess) return fail(SSC_ERR_CUDA, "gated_ff_bwd: %s", cudaGetErrorString(e));
       ++f.launches;
     }
   }
@@ -1504,11 +1542,11 @@ int backward(Ff &f, Scratch s, const void *x, const void *gy, const void *w_in, 
   if (gw_out) add_job(jobs, blocks, part_out, split_out, size_out, gw_out, 0);
   if (gb_in) add_job(jobs, blocks, cols_in, shares_in, 2 * (size_t)f.hidden, gb_in, 1);
   if (gb_out) add_job(jobs, blocks, cols_out, shares_out, f.c_out, gb_out, 1);
-  if (blocks > 0 && e == cudaSuccess) {
-    e = launch_ready(ff_sum_kernel<T>, dim3(blocks), dim3(256), 0, f.st, jobs);
+  if (blocks > 0) {
+    const cudaError_t e = launch_ready(ff_sum_kernel<T>, dim3(blocks), dim3(256), 0, f.st, jobs);
+    if (e != cudaSuccess) return fail(SSC_ERR_CUDA, "gated_ff_bwd: %s", cudaGetErrorString(e));
     ++f.launches;
   }
-  if (e != cudaSuccess) return fail(SSC_ERR_CUDA, "gated_ff_bwd: %s", cudaGetErrorString(e));
   return SSC_OK;
 }
 
@@ -1545,7 +1583,7 @@ extern "C" size_t ssc_gated_ff_scratch_bytes(int type, int n, int c, int hidden,
 extern "C" int ssc_gated_ff_fwd(const void *x, int type, int n, int c, int hidden, int c_out, const void *w_in, const void *w_out, const void *b_in, const void *b_out,
                                 const void *residual, int act, void *out, int32_t *status, void *scratch, size_t scratch_bytes, void *stream) {
   using namespace ssc;
-  Ff f = {type, n, c, hidden, c_out, act, as_stream(stream), status, 0, cudaSuccess};
+  Ff f = {type, n, c, hidden, c_out, act, as_stream(stream), status, 0, {}, 0};
   if (int e = ff_check(f, "gated_ff_fwd")) return e;
   SSC_REQUIRE(w_in && w_out && (n == 0 || (x && out)), "gated_ff_fwd: null pointer");
   if (n == 0) return SSC_OK;
@@ -1556,7 +1594,6 @@ extern "C" int ssc_gated_ff_fwd(const void *x, int type, int n, int c, int hidde
                                  : forward<__nv_bfloat16>(f, s, x, w_in, w_out, b_in, b_out, residual, out);
   note_launches(f.launches);
   if (e != SSC_OK) return e;
-  if (f.err != cudaSuccess) return fail(SSC_ERR_CUDA, "gated_ff_fwd: %s", cudaGetErrorString(f.err));
   SSC_CHECK_LAUNCH("gated_ff_fwd");
   return SSC_OK;
 }
@@ -1564,7 +1601,7 @@ extern "C" int ssc_gated_ff_fwd(const void *x, int type, int n, int c, int hidde
 extern "C" int ssc_gated_ff_bwd(const void *x, const void *gy, int type, int n, int c, int hidden, int c_out, const void *w_in, const void *w_out, const void *b_in, int act,
                                 void *gx, void *gw_in, void *gw_out, void *gb_in, void *gb_out, int32_t *status, void *scratch, size_t scratch_bytes, void *stream) {
   using namespace ssc;
-  Ff f = {type, n, c, hidden, c_out, act, as_stream(stream), status, 0, cudaSuccess};
+  Ff f = {type, n, c, hidden, c_out, act, as_stream(stream), status, 0, {}, 0};
   if (int e = ff_check(f, "gated_ff_bwd")) return e;
   SSC_REQUIRE(w_in && w_out && (n == 0 || (x && gy)), "gated_ff_bwd: null pointer");
   if (n == 0) {
@@ -1584,7 +1621,6 @@ extern "C" int ssc_gated_ff_bwd(const void *x, const void *gy, int type, int n, 
                                  : backward<__nv_bfloat16>(f, s, x, gy, w_in, w_out, b_in, gx, gw_in, gw_out, gb_in, gb_out);
   note_launches(f.launches);
   if (e != SSC_OK) return e;
-  if (f.err != cudaSuccess) return fail(SSC_ERR_CUDA, "gated_ff_bwd: %s", cudaGetErrorString(f.err));
   SSC_CHECK_LAUNCH("gated_ff_bwd");
   return SSC_OK;
 }
