@@ -7,9 +7,11 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 #include <ATen/DeviceGuard.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include <optional>
@@ -64,6 +66,27 @@ bool recorded(std::initializer_list<const Tensor *> all) {
   for (const Tensor *t : all)
     if (t->defined() && t->requires_grad()) return true;
   return false;
+}
+// Recording into a CUDA graph: gradients of a leaf that an earlier result of the default stream still holds on to would be added up on that
+// stream, which cannot take part: the backward pass would end the process.  So the call is refused.  (Looked at as far as leaves, tensors converted
+// from them and results of the default stream.)
+void recordable(std::initializer_list<const Tensor *> all, const Tensor &x) {
+  const c10::DeviceIndex device = x.device().index();
+  const c10::Stream ordinary = c10::cuda::getDefaultCUDAStream(device);
+  if (c10::cuda::getCurrentCUDAStream(device).unwrap() == ordinary) return;
+  bool foreign = false;
+  auto look = [&](torch::autograd::Node *f) { foreign |= f != nullptr && f->stream() == ordinary; };
+  for (const Tensor *t : all) {
+    if (!t->defined() || !t->requires_grad()) continue;
+    if (t->is_leaf()) {
+      look(torch::autograd::impl::try_get_grad_accumulator(*t).get());
+    } else {
+      look(t->grad_fn().get());
+      for (const torch::autograd::Edge &e : t->grad_fn()->next_edges()) look(e.function.get());
+    }
+  }
+  TORCH_CHECK(!foreign || c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None,
+              "a result computed before this recording still holds the gradient graph of the same tensors: drop it (its loss) before recording");
 }
 void first_gradient(const char *what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, ": gradients of gradients are not available (create_graph)");
@@ -146,6 +169,7 @@ Tensor norm(const Tensor &features, const Tensor &weight_in, const Tensor &bias_
   const Tensor x = aligned(features), offsets = offsets_in.contiguous();
   const Tensor weight = weight_in.defined() ? weight_in.to(at::kFloat).contiguous() : weight_in, bias = bias_in.defined() ? bias_in.to(at::kFloat).contiguous() : bias_in;
   if (recorded({&x, &weight, &bias})) {
+    recordable({&features, &weight_in, &bias_in}, features);
     const Tensor y = NormNode::apply(x, maybe(weight), maybe(bias), offsets, table, status, k);
     return out_type == y.scalar_type() ? y : y.to(out_type);
   }
@@ -225,7 +249,9 @@ Tensor feedforward(const Tensor &x, const Tensor &w_in, const Tensor &w_out, con
   wants("residual", residual, {x.size(0), c_out});
   auto flat = [](const Tensor &t) { return t.defined() ? t.contiguous() : t; };
   const Tensor a = flat(x), b = flat(w_in), d = flat(w_out), e = flat(b_in), f = flat(b_out), g = flat(residual);
-  return recorded({&a, &b, &d, &e, &f, &g}) ? Tensor(FfNode::apply(a, b, d, maybe(e), maybe(f), maybe(g), status, act)) : ff_forward(a, b, d, e, f, g, status, act);
+  if (!recorded({&a, &b, &d, &e, &f, &g})) return ff_forward(a, b, d, e, f, g, status, act);
+  recordable({&x, &w_in, &w_out, &b_in, &b_out, &residual}, x);
+  return FfNode::apply(a, b, d, maybe(e), maybe(f), maybe(g), status, act);
 }
 
 // ------------------------------------------------------------------------------------------ Python

@@ -129,3 +129,41 @@ def test_two_streams_and_two_graphs_at_once(cuda):
                 g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("converted", [False, True])
+def test_a_training_pass_is_recorded_without_results_from_before(cuda, converted):
+    """With an eager result of the same parameters alive (on the default stream) a recording is refused; without it, it replays."""
+    from ss_conv.feedforward import gated_feedforward
+    from ss_conv.groupnorm import group_norm
+    off = torch.tensor([0, 300, 700], dtype=torch.int32, device=cuda)
+    g = torch.Generator("cuda").manual_seed(5)
+    r = lambda *s: torch.randn(*s, generator=g, device=cuda)  # noqa: E731
+    dtype = torch.bfloat16 if converted else torch.float32
+    x, gy = r(700, 32).to(dtype), r(700, 32).to(dtype)
+    params = [p.requires_grad_() for p in (r(32), r(32), r(2, 48, 32) / 6, r(32, 48) / 7)]
+
+    def norm():
+        return group_norm(x, off, [(32, 0)], 8, params[0], params[1], activation=F.silu)
+
+    def ff():
+        return gated_feedforward(x, params[2].to(dtype), params[3].to(dtype), residual=x)
+
+    for step, mine in ((norm, params[:2]), (ff, params[2:])):
+        want = torch.autograd.grad(step(), mine, gy)
+        alive = step()
+        side = torch.cuda.Stream()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            torch.zeros(8, device=cuda)
+            with pytest.raises(RuntimeError, match="before this recording"):
+                step()
+        del alive, graph
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = torch.autograd.grad(step(), mine, gy)
+        for t in got:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
