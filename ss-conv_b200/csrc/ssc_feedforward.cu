@@ -103,12 +103,23 @@ __device__ __forceinline__ void add16(float *v, const T *p, int left, int vec) {
       if (i < left) v[i] += (float)p[i];
   }
 }
-// v as three bfloat16 planes; what is not finite is in the first one alone.
-__device__ __forceinline__ void planes_of(float v, float &a, float &b, float &c) {
-  a = __bfloat162float(__float2bfloat16_rn(v));
-  const float r = v - a;
-  b = fabsf(a) < INFINITY ? __bfloat162float(__float2bfloat16_rn(r)) : 0.f;
-  c = fabsf(a) < INFINITY ? r - b : 0.f;
+// The next of three bfloat16 planes of v, a word to two values; v keeps what is left.  What is not finite is in the first plane alone.
+template <int N, bool FIRST>
+__device__ __forceinline__ void next_plane(float *v, uint32_t *w) {
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const __nv_bfloat162 k = __floats2bfloat162_rn(v[i], v[i + 1]);
+    w[i / 2] = *(const uint32_t *)&k;
+    const float a = __uint_as_float(w[i / 2] << 16), b = __uint_as_float(w[i / 2] & 0xFFFF0000u);
+    const float2 left = halves(fma_pair(pair_of(a, b), pair_of(-1.f, -1.f), pair_of(v[i], v[i + 1])));
+    v[i] = !FIRST || fabsf(a) < INFINITY ? left.x : 0.f;
+    v[i + 1] = !FIRST || fabsf(b) < INFINITY ? left.y : 0.f;
+  }
+}
+template <int N>
+__device__ __forceinline__ void next_plane(float *v, uint32_t *w, int plane) {
+  if (plane == 0) next_plane<N, true>(v, w);
+  else next_plane<N, false>(v, w);
 }
 
 // A warp's way out of 32 rows of up to 32 columns: each lane puts its row's 16 columns into the warp's shared memory, one lane sends the box off.  Rows
@@ -136,21 +147,24 @@ struct Outbox {
     if (++slot == slots) slot = 0;
     return here;
   }
-  // 16 columns (part 0, 1 ... of the box) of the lane's row.
+  // 16 columns (part 0, 1 ... of the box) of the lane's row, as words or as values to be rounded.
+  template <int ROW_BYTES, int BYTES>
+  __device__ __forceinline__ void put_words(uint32_t box, int part, const uint32_t *w) {
+    const uint32_t lane = threadIdx.x & 31;
+    constexpr uint32_t mask = ROW_BYTES / 16 - 1;
+    const uint32_t row = box + lane * ROW_BYTES, turn = lane / (128 / ROW_BYTES) & mask;
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; ++i) {
+      const uint32_t to = row + (((uint32_t)(part * (BYTES / 16) + i) ^ turn) << 4);
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w[4 * i]), "r"(w[4 * i + 1]), "r"(w[4 * i + 2]), "r"(w[4 * i + 3]) : "memory");
+    }
+  }
   template <class V, int COLS = 32>
   __device__ __forceinline__ void put(uint32_t box, int part, const float *v) {
-    const uint32_t lane = threadIdx.x & 31;
-    constexpr int N = 16 / sizeof(V);
-    constexpr uint32_t row_bytes = COLS * sizeof(V), mask = row_bytes / 16 - 1;
-    const uint32_t row = box + lane * row_bytes, turn = lane / (128 / row_bytes) & mask;
+    struct alignas(16) { V v[16]; } k;
 #pragma unroll
-    for (int i = 0; i < 16 / N; ++i) {
-      struct alignas(16) { V v[N]; } k;
-#pragma unroll
-      for (int q = 0; q < N; ++q) k.v[q] = (V)v[i * N + q];
-      const uint32_t *w = (const uint32_t *)&k, to = row + (((uint32_t)(part * (16 / N) + i) ^ turn) << 4);
-      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-    }
+    for (int q = 0; q < 16; ++q) k.v[q] = (V)v[q];
+    put_words<COLS * sizeof(V), 16 * sizeof(V)>(box, part, (const uint32_t *)&k);
   }
   // One value of a box of 32 float32 columns.
   static __device__ __forceinline__ float get(uint32_t box, uint32_t row, uint32_t col) {
@@ -238,7 +252,7 @@ __device__ __forceinline__ void stored_dh(const FfParams &p, int row, int n, flo
 
 // A plane of 32 columns of hidden rows (16-bit, or one of the three of float32 rows) goes out as a box.
 template <class T>
-__device__ __forceinline__ void send_hidden(Outbox &box, const CUtensorMap *map, const float (*v)[16], int n, int row0, int z, int planes_apart) {
+__device__ __forceinline__ void send_hidden(Outbox &box, const CUtensorMap *map, float (*v)[16], int n, int row0, int z, int planes_apart) {
   if (sizeof(T) == 2) {
     const uint32_t at = box.room();
     box.put<T>(at, 0, v[0]);
@@ -250,14 +264,9 @@ __device__ __forceinline__ void send_hidden(Outbox &box, const CUtensorMap *map,
       const uint32_t at = box.room();
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float w[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float a, b, c;
-          planes_of(v[h][i], a, b, c);
-          w[i] = plane == 0 ? a : plane == 1 ? b : c;
-        }
-        box.put<__nv_bfloat16>(at, h, w);
+        uint32_t w[8];
+        next_plane<16>(v[h], w, plane);
+        box.put_words<64, 32>(at, h, w);
       }
       box.send(at, map, n, row0, z + plane * planes_apart);
     }
@@ -296,18 +305,13 @@ __device__ __forceinline__ void finish_back(const FfParams &p, const FfMaps &map
   } else if (left > 0) {
 #pragma unroll
     for (int o = 0; o < 3; ++o) {
-      const float *from = o == 0 ? h : o == 1 ? u : v;
+      float *from = o == 0 ? h : o == 1 ? u : v;
 #pragma unroll
       for (int plane = 0; plane < 3; ++plane) {
-        float w[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float a, b, c;
-          planes_of(from[i], a, b, c);
-          w[i] = plane == 0 ? a : plane == 1 ? b : c;
-        }
+        uint32_t w[8];
+        next_plane<16>(from, w, plane);
         const uint32_t at = box.room();
-        box.put<__nv_bfloat16, 16>(at, 0, w);
+        box.put_words<32, 32>(at, 0, w);
         box.send(at, o == 0 ? &maps.out[0] : &maps.out[1], n, row0, o == 0 ? plane : 2 * plane + o - 1);
       }
     }
@@ -860,29 +864,26 @@ __global__ void __launch_bounds__(256) ff_planes_kernel(const PlaneJobs jobs) {
   const long long row = t / per;
   if (row >= rows) return;
   const int c0 = (int)(t - row * per) * 8;
-  T v[8];
+  struct alignas(16) { T v[8]; } k;
+  const T *from = src + row * cols + c0;
+  if (cols % 8 == 0 && ((uintptr_t)src & 15) == 0) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = c0 + i < cols ? src[row * cols + c0 + i] : (T)0.f;
-  if (sizeof(T) == 2) {
-    struct alignas(16) { T v[8]; } k;
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) ((int4 *)&k)[i] = ((const int4 *)from)[i];
+  } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) k.v[i] = v[i];
+    for (int i = 0; i < 8; ++i) k.v[i] = c0 + i < cols ? from[i] : (T)0.f;
+  }
+  if constexpr (sizeof(T) == 2) {
     *(int4 *)((T *)dst + row * pitch + c0) = *(const int4 *)&k;
   } else {
-    struct alignas(16) { __nv_bfloat16 v[8]; } a, b, c;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float x, y, z;
-      planes_of((float)v[i], x, y, z);
-      a.v[i] = __float2bfloat16_rn(x);
-      b.v[i] = __float2bfloat16_rn(y);
-      c.v[i] = __float2bfloat16_rn(z);
-    }
     const size_t plane = (size_t)rows * pitch;
     __nv_bfloat16 *p = (__nv_bfloat16 *)dst + row * pitch + c0;
-    *(int4 *)p = *(const int4 *)&a;
-    *(int4 *)(p + plane) = *(const int4 *)&b;
-    *(int4 *)(p + 2 * plane) = *(const int4 *)&c;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      uint32_t w[4];
+      next_plane<8>(k.v, w, i);
+      *(int4 *)(p + i * plane) = *(const int4 *)w;
+    }
   }
 }
 
