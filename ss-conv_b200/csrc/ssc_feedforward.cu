@@ -67,7 +67,7 @@ struct FfParams {
   int pitch;                                   // of out
   size_t plane;                                // kPart: elements of a share
   int boxes;                                   // out (and out2) are stored by boxes (maps.out), else from registers
-  int vec;                                     // rows of out (and residual) are aligned to 32 bytes
+  int vec;                                     // rows of the residual are aligned to 16 bytes
   int accumulate;                              // kPart: add to what is there
   int32_t *status, *alarm;
 };
@@ -125,7 +125,7 @@ __device__ __forceinline__ void next_plane(float *v, uint32_t *w, int plane) {
 // A warp's way out of 32 rows of up to 32 columns: each lane puts its row's 16 columns into the warp's shared memory, one lane sends the box off.  Rows
 // from registers cost as much time as the products did (131072 rows 512 -> 2048 in bf16: 549 us, 394 without them).
 // Boxes of 32 columns: rows of 64 bytes (16-bit) or 128 (float32), or of 16 columns, 32 bytes; swizzled as the copy engine has it, which
-// keeps lanes on different banks.
+// keeps lanes on different banks.  (kBack of float32 rows, 16384 of 128 -> 512: 65 us; by boxes of 32 columns, which leave registers for half of the warps, 70.)
 struct Outbox {
   uint32_t at;             // the warp's shared memory: slots taken in turn
   uint32_t slot, slots, slot_bytes;
@@ -1262,7 +1262,7 @@ int rows_product(Ff &f, const Matrix &a, const Matrix &b, int b_mn, bool halves,
   p.bias = bias;
   p.residual = residual;
   p.out = out;
-  p.vec = p.pitch % (32 / (int)sizeof(T)) == 0 && (((uintptr_t)out | (uintptr_t)residual) & 31) == 0;
+  p.vec = p.pitch % (16 / (int)sizeof(T)) == 0 && ((uintptr_t)residual & 15) == 0;
   p.boxes = make_out_map(&maps.out[0], out, p.rows, cols, p.pitch, 1, f.type);
   return launch_gemm<kRows, T>(f, maps, p);
 }
@@ -1398,7 +1398,6 @@ int filter_product(Ff &f, const Matrix &a, const Matrix &b, int halves, int m, i
   p.tiles_n = ceil_div(cols, p.step_n);
   p.splits = splits;
   p.out = part;
-  p.vec = cols % 8 == 0;
   p.accumulate = accumulate;
   p.boxes = !accumulate && make_out_map(&maps.out[0], part, m, cols, cols, halves * splits, SSC_PREC_FP32);
   return launch_gemm<kPart, T>(f, maps, p);
