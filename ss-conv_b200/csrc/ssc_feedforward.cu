@@ -977,107 +977,105 @@ __global__ void __launch_bounds__(256) ff_columns_kernel(const ColumnJobs jobs, 
   }
 }
 
-// Few rows: the weights are read once and bound the time; a warp to an output, rows in shared memory, sums in float32 and h
-// never rounded.  kR rows at a time.
-constexpr int kR = 8;
-// acc[r] += sum over this lane's part of w[i] xs[r][i], all lanes' sums in the end.  xs: rows of `stride` floats, 16-byte aligned.
-template <class T>
-__device__ __forceinline__ void dot_rows(const T *__restrict__ w, const float *__restrict__ xs, int k, int stride, int live, float *acc, int vec) {
-  constexpr int N = 16 / sizeof(T);
-  const int lane = threadIdx.x & 31;
+// Few rows: float32 sums on plain lanes, h never rounded.  A warp takes kFewOutputs outputs of R rows at a time, so that what it loads of the rows serves
+// several outputs, and a share of the summed index, so that most loads are under way at once: one latency is what a call of a single row costs.
+constexpr int kFewOutputs = 4;
+constexpr int kFewRows = 8;        // R at most
+constexpr int kFewShares = 8;      // warps to a sum, at most
+
+template <class T, int N>
+__device__ __forceinline__ void take(const T *p, int left, int vec, float *v) {
   if (vec) {
-    constexpr int U = 4;                        // pieces of the weights in flight
-    for (int i0 = lane * N; i0 < k; i0 += 32 * N * U) {
-      int4 q[U];
+    struct alignas(16) { T v[N]; } k;
 #pragma unroll
-      for (int u = 0; u < U; ++u) q[u] = i0 + u * 32 * N < k ? *(const int4 *)(w + i0 + u * 32 * N) : make_int4(0, 0, 0, 0);
+    for (int i = 0; i < N * (int)sizeof(T) / 16; ++i) ((int4 *)&k)[i] = ((const int4 *)p)[i];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = i0 + u * 32 * N;
-        if (i >= k) continue;
-        struct alignas(16) { T v[N]; } piece;
-        *(int4 *)&piece = q[u];
+    for (int i = 0; i < N; ++i) v[i] = (float)k.v[i];
+  } else {
 #pragma unroll
-        for (int r = 0; r < kR; ++r)
-          if (r < live) {
+    for (int i = 0; i < N; ++i) v[i] = i < left ? (float)p[i] : 0.f;
+  }
+}
+
+// Sums over the lanes of M values: half of them go to the lane across, as long as there are two.
+template <int M, int D>
+__device__ __forceinline__ void fold(float *v, int lane) {
+  if constexpr (M > 1) {
 #pragma unroll
-            for (int e = 0; e < N; e += 4) {
-              const float4 x = *(const float4 *)(xs + (size_t)r * stride + i + e);
-              acc[r] = fmaf((float)piece.v[e], x.x, acc[r]);
-              acc[r] = fmaf((float)piece.v[e + 1], x.y, acc[r]);
-              acc[r] = fmaf((float)piece.v[e + 2], x.z, acc[r]);
-              acc[r] = fmaf((float)piece.v[e + 3], x.w, acc[r]);
-            }
-          }
-      }
+    for (int i = 0; i < M / 2; ++i) {
+      const float mine = lane & D ? v[i + M / 2] : v[i], other = lane & D ? v[i] : v[i + M / 2];
+      v[i] = mine + __shfl_xor_sync(0xffffffffu, other, D);
     }
   } else {
-    constexpr int U = 8;
-    for (int i0 = lane; i0 < k; i0 += 32 * U) {
-      float q[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) q[u] = i0 + 32 * u < k ? (float)w[i0 + 32 * u] : 0.f;
-#pragma unroll
-      for (int r = 0; r < kR; ++r)
-        if (r < live) {
-          float x[U];
-#pragma unroll
-          for (int u = 0; u < U; ++u) x[u] = i0 + 32 * u < k ? xs[(size_t)r * stride + i0 + 32 * u] : 0.f;
-#pragma unroll
-          for (int u = 0; u < U; ++u) acc[r] = fmaf(q[u], x[u], acc[r]);
-        }
-    }
+    v[0] += __shfl_xor_sync(0xffffffffu, v[0], D);
   }
-#pragma unroll
-  for (int r = 0; r < kR; ++r)
-    for (int d = 16; d > 0; d >>= 1) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], d);
+  if constexpr (D > 1) fold<(M > 1 ? M / 2 : 1), D / 2>(v, lane);
 }
 
-template <class T>
-__global__ void __launch_bounds__(256) ff_few_hidden_kernel(const T *__restrict__ x, int rows, int c, int hidden, const T *__restrict__ w_in, const T *__restrict__ b_in,
-                                                            int act, float *__restrict__ h, int h_stride, int vec) {
-  after_previous();
-  extern __shared__ __align__(16) float xs[];   // [kR][c rounded up to 8]
-  const int r0 = blockIdx.y * kR, live = min(kR, rows - r0), stride = (c + 7) & ~7;
-  for (int i = threadIdx.x; i < live * c; i += 256) {
-    const int r = i / c;
-    xs[r * stride + i - r * c] = (float)x[(size_t)(r0 + r) * c + i - r * c];
+// The sum of w[o][i] x[r][i] over i, for output o and row r (shared memory, every warp of a sum's `shares` has a part): this lane's, of value
+// lane % (outputs * R) = o * R + r, in the sum's first warp.  Rows behind `last` are that one.
+template <class T, class X, int R>
+__device__ __forceinline__ float few_sums(const T *const *w, const X *x, size_t x_stride, int r0, int last, int k, int shares, int vec, float (*parts)[32]) {
+  constexpr int N = 16 / sizeof(T), V = kFewOutputs * R;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = warp % shares;
+  float acc[V] = {};
+  for (int i = (share * 32 + lane) * N; i < k; i += 32 * N * shares) {
+    float a[kFewOutputs][N], b[R][N];
+#pragma unroll
+    for (int o = 0; o < kFewOutputs; ++o) take<T, N>(w[o] + i, k - i, vec, a[o]);
+#pragma unroll
+    for (int r = 0; r < R; ++r) take<X, N>(x + (size_t)min(r0 + r, last) * x_stride + i, k - i, vec, b[r]);
+#pragma unroll
+    for (int o = 0; o < kFewOutputs; ++o)
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[o * R + r] = fmaf(a[o][e], b[r][e], acc[o * R + r]);
   }
+  fold<V, 16>(acc, lane);
+  if (lane % (32 / V) == 0) parts[warp][lane / (32 / V)] = acc[0];
   __syncthreads();
-  const int j = blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (j >= hidden) return;
-  float g[kR] = {}, u[kR] = {};
-  dot_rows<T>(w_in + (size_t)j * c, xs, c, stride, live, g, vec);
-  dot_rows<T>(w_in + (size_t)(hidden + j) * c, xs, c, stride, live, u, vec);
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int r = 0; r < kR; ++r)
-    if (r < live && lane == r) {
-      const float bg = b_in ? (float)b_in[j] : 0.f, bu = b_in ? (float)b_in[hidden + j] : 0.f;
-      float a = g[r] + bg;
-      act_values<true, 1>(&a, act);
-      h[(size_t)(r0 + r) * h_stride + j] = a * (u[r] + bu);
-    }
+  float sum = 0.f;
+  if (share == 0)
+    for (int q = 0; q < shares; ++q) sum += parts[warp + q][lane % V];
+  return sum;
 }
 
-template <class T>
-__global__ void __launch_bounds__(256) ff_few_out_kernel(const float *__restrict__ h, int h_stride, int rows, int hidden, int c_out, const T *__restrict__ w_out, const T *__restrict__ b_out,
-                                                         const T *__restrict__ residual, T *__restrict__ y, int vec) {
+template <class T, int R>
+__global__ void __launch_bounds__(256) ff_few_hidden_kernel(const T *__restrict__ x, int rows, int c, int hidden, const T *__restrict__ w_in, const T *__restrict__ b_in,
+                                                            int act, float *__restrict__ h, int h_stride, int shares, int vec) {
   after_previous();
-  const int r0 = blockIdx.y * kR, live = min(kR, rows - r0);
-  const int o = blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (o >= c_out) return;
-  float v[kR] = {};
-  dot_rows<T>(w_out + (size_t)o * hidden, h + (size_t)r0 * h_stride, hidden, h_stride, live, v, vec);
-  const int lane = threadIdx.x & 31;
+  __shared__ float parts[8][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r0 = blockIdx.y * R;
+  const int j0 = (blockIdx.x * (blockDim.x / 32 / shares) + warp / shares) * (kFewOutputs / 2);
+  const T *w[kFewOutputs];                      // gate and up in turn
 #pragma unroll
-  for (int r = 0; r < kR; ++r)
-    if (r < live && lane == r) {
-      float out = v[r] + (b_out ? (float)b_out[o] : 0.f);
-      const size_t at = (size_t)(r0 + r) * c_out + o;
-      if (residual) out += (float)residual[at];
-      y[at] = (T)out;
-    }
+  for (int o = 0; o < kFewOutputs; ++o) w[o] = w_in + ((size_t)(o & 1) * hidden + min(j0 + o / 2, hidden - 1)) * c;
+  const float sum = few_sums<T, T, R>(w, x, c, r0, rows - 1, c, shares, vec, parts), up = __shfl_xor_sync(0xffffffffu, sum, R);
+  const int o = lane / R, j = j0 + o / 2, r = r0 + lane % R;
+  if (warp % shares != 0 || o >= kFewOutputs || (o & 1) || j >= hidden || r >= rows) return;
+  float g = sum + (b_in ? (float)b_in[j] : 0.f);
+  act_values<true, 1>(&g, act);
+  h[(size_t)r * h_stride + j] = g * (up + (b_in ? (float)b_in[hidden + j] : 0.f));
+}
+
+template <class T, int R>
+__global__ void __launch_bounds__(256) ff_few_out_kernel(const float *__restrict__ h, int h_stride, int rows, int hidden, int c_out, const T *__restrict__ w_out,
+                                                         const T *__restrict__ b_out, const T *__restrict__ residual, T *__restrict__ y, int shares, int vec) {
+  after_previous();
+  __shared__ float parts[8][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r0 = blockIdx.y * R;
+  const int o0 = (blockIdx.x * (blockDim.x / 32 / shares) + warp / shares) * kFewOutputs;
+  const T *w[kFewOutputs];
+#pragma unroll
+  for (int o = 0; o < kFewOutputs; ++o) w[o] = w_out + (size_t)min(o0 + o, c_out - 1) * hidden;
+  float sum = few_sums<T, float, R>(w, h, h_stride, r0, rows - 1, hidden, shares, vec, parts);
+  const int o = o0 + lane / R, r = r0 + lane % R;
+  if (warp % shares != 0 || lane / R >= kFewOutputs || o >= c_out || r >= rows) return;
+  if (b_out) sum += (float)b_out[o];
+  const size_t at = (size_t)r * c_out + o;
+  if (residual) sum += (float)residual[at];
+  y[at] = (T)sum;
 }
 
 // ------------------------------------------------------------------------------------------- host
@@ -1453,23 +1451,48 @@ size_t parts_bytes(const Ff &f, long long most, bool back) {
   return b;
 }
 
-// Rows up to which the weights are read once by a warp to an output instead of by tiles of 128 rows.
-bool few(const Ff &f) { return f.n <= (f.type == SSC_PREC_FP32 ? 64 : 16) && f.c <= 4096; }
+// Few rows: products on plain lanes instead of tiles of 256 rows, by what each was measured to take.  Plain lanes: 3.3 us, and for each (up to) eight
+// rows the weights at 2.0 (one row), 1.3 (four) or 0.8 (eight) a picosecond in float32, 2.9, 1.5 and 0.7 in 16 bits.  Tiles: 16 us and 10.5 ns
+// for each column of x and h in float32, 14 us and 2 ns in 16 bits, whatever the number of rows.  (us, c -> 4 c -> c: float32 8 rows of 256 4.5, 64 rows 13.1, by tiles
+// 29.7; 8 rows of 1024 19.7, 64 rows 132, by tiles 85.  bfloat16 1 row of 256 3.7, 16 rows 5.1, by tiles 17; 1 row of 1024 7.5, 16 rows 39, by tiles 24.)
+bool few(const Ff &f) {
+  if (f.n > kTileM) return false;
+  const bool single = f.type == SSC_PREC_FP32;
+  const long long weights = (2ll * f.c + f.c_out) * f.hidden, wide = (long long)f.c + f.hidden;
+  const long long fs = single ? (f.n == 1 ? 500 : f.n <= 4 ? 790 : 1280) : (f.n == 1 ? 340 : f.n == 2 ? 360 : f.n <= 4 ? 680 : 1400);
+  return 3300 + weights * ceil_div(f.n, kFewRows) / 1000 * fs / 1000 < (single ? 16000 + 21 * wide / 2 : 14000 + 2 * wide);
+}
+
+// Warps that share a sum of k terms: a piece to a lane each where that takes no more than kFewShares of them.
+int few_shares(int k, int piece) {
+  int s = 1;
+  while (s < kFewShares && s * 32 * piece < k) s *= 2;
+  return s;
+}
+template <class T, int R>
+cudaError_t few_rows(const Ff &f, const void *x, const void *w_in, const void *w_out, const void *b_in, const void *b_out, const void *residual, float *h, int h_stride,
+                     void *out) {
+  constexpr int N = 16 / (int)sizeof(T);
+  const int vec_in = f.c % N == 0 && (((uintptr_t)w_in | (uintptr_t)x) & 15) == 0, vec_out = f.hidden % N == 0 && ((uintptr_t)w_out & 15) == 0;
+  const int shares_in = few_shares(f.c, N), shares_out = few_shares(f.hidden, N), warps_in = shares_in < 4 ? 4 : shares_in, warps_out = shares_out < 4 ? 4 : shares_out;
+  const int rows = ceil_div(f.n, R);
+  cudaError_t e = launch_ready(ff_few_hidden_kernel<T, R>, dim3(ceil_div(f.hidden, kFewOutputs / 2 * (warps_in / shares_in)), rows), dim3(32 * warps_in), 0, f.st, (const T *)x, f.n,
+                               f.c, f.hidden, (const T *)w_in, (const T *)b_in, f.act, h, h_stride, shares_in, vec_in);
+  if (e == cudaSuccess)
+    e = launch_ready(ff_few_out_kernel<T, R>, dim3(ceil_div(f.c_out, kFewOutputs * (warps_out / shares_out)), rows), dim3(32 * warps_out), 0, f.st, (const float *)h, h_stride, f.n,
+                     f.hidden, f.c_out, (const T *)w_out, (const T *)b_out, (const T *)residual, (T *)out, shares_out, vec_out);
+  return e;
+}
 
 template <class T>
 int forward(Ff &f, Scratch s, const void *x, const void *w_in, const void *w_out, const void *b_in, const void *b_out, const void *residual, void *out) {
   if (few(f)) {
     const int h_stride = (f.hidden + 3) & ~3;
     float *h = (float *)s.take((size_t)f.n * h_stride * sizeof(float));
-    const int vec_in = f.c % (16 / (int)sizeof(T)) == 0 && ((uintptr_t)w_in & 15) == 0, vec_out = f.hidden % (16 / (int)sizeof(T)) == 0 && ((uintptr_t)w_out & 15) == 0;
-    const size_t room = (size_t)kR * ((f.c + 7) & ~7) * sizeof(float);
-    cudaError_t e = allow_smem((const void *)ff_few_hidden_kernel<T>, room);
-    if (e == cudaSuccess)
-      e = launch_ready(ff_few_hidden_kernel<T>, dim3(ceil_div(f.hidden, 8), ceil_div(f.n, kR)), dim3(256), room, f.st, (const T *)x, f.n, f.c, f.hidden, (const T *)w_in,
-                       (const T *)b_in, f.act, h, h_stride, vec_in);
-    if (e == cudaSuccess)
-      e = launch_ready(ff_few_out_kernel<T>, dim3(ceil_div(f.c_out, 8), ceil_div(f.n, kR)), dim3(256), 0, f.st, (const float *)h, h_stride, f.n, f.hidden, f.c_out, (const T *)w_out,
-                       (const T *)b_out, (const T *)residual, (T *)out, vec_out);
+    const cudaError_t e = f.n == 1   ? few_rows<T, 1>(f, x, w_in, w_out, b_in, b_out, residual, h, h_stride, out)
+                          : f.n == 2 ? few_rows<T, 2>(f, x, w_in, w_out, b_in, b_out, residual, h, h_stride, out)
+                          : f.n <= 4 ? few_rows<T, 4>(f, x, w_in, w_out, b_in, b_out, residual, h, h_stride, out)
+                                     : few_rows<T, kFewRows>(f, x, w_in, w_out, b_in, b_out, residual, h, h_stride, out);
     if (e != cudaSuccess) return fail(SSC_ERR_CUDA, "gated_ff_fwd: %s", cudaGetErrorString(e));
     f.launches += 2;
     return SSC_OK;

@@ -59,6 +59,25 @@ SIZES = [
 ]
 
 
+# More of them: rows on plain lanes in ones, twos, fours and eights with sums that end inside a piece, a warp or a share; tiles of more than 256 rows.
+SIZES += [
+    (2, 9, 65, 7, True, True, F.silu),
+    (4, 257, 5, 258, False, False, F.gelu),
+    (5, 40, 2050, 3, True, False, None),
+    (8, 4100, 24, 8, False, True, F.silu),
+    (9, 1025, 130, 31, True, True, torch.sigmoid),
+    (31, 128, 512, 66, False, False, F.silu),
+    (250, 33, 70, 12, True, True, F.relu),
+    (256, 64, 128, 64, False, True, F.silu),
+    (257, 65, 129, 257, True, False, F.silu),
+    (300, 17, 33, 5, True, True, F.gelu),
+    (383, 8, 72, 24, False, False, None),
+    (511, 100, 300, 76, True, True, torch.sigmoid),
+    (260, 600, 200, 64, False, True, F.silu),
+    (40, 2048, 2048, 512, True, False, F.gelu),
+]
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("size", range(len(SIZES)))
 def test_block_and_gradients(cuda, size, dtype):
