@@ -9,6 +9,11 @@
 // All of them are one kernel: pairs of CTAs with tiles of 256 rows in tensor memory, half of each operand in either CTA, operands by TMA, a warp
 // that issues the products and others that empty the accumulators, two of which are in turn.  Operands are 16-bit; float32 rows are the sum of
 // three bfloat16 planes (24 bits), and a product the sum of the six products of planes that reach 2^-24, the small ones first.
+//
+// 65536 rows 256 -> 1024 -> 256 in bf16, forward 124 us, backward 309 (rates of a cool GPU; 1.2 GHz under its power limit: 500 for both): gate, up and h
+// 75 (917 TFLOP/s of its two products, bound by the way out: 134 MB of h through shared memory), the way out 49, h, dg and du 139 (403 MB), dx 68, the
+// gradients of Win and Wo 56 and 37, their sums 9.  float32, 16384 rows 128 -> 512 -> 128, 265 us for both: h, dg and du 65, nine planes whose splitting and stores
+// bound it.  One row 256 -> 1024 -> 256 3.7 us, two launches and two latencies.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

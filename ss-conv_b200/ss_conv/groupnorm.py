@@ -1,7 +1,7 @@
 """Group normalisation of sparse rows with the gated activation behind it.
 
 The reference has batch norm only (SS_Conv_lib/ss_conv/batchnorm.py:13-136), whose statistics mix the samples of a batch;
-here every sample has its own, so a row's result does not depend on what else is in the batch, and training and
+here every sample has its own, so a row's result does not depend on what else is in the batch (but for the order of sums), and training and
 inference compute the same.  Scalars are centred and scaled, fields of order l > 0 are scaled by the mean of
 their squared norm, which keeps the layer equivariant."""
 import functools
