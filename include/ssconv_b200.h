@@ -616,7 +616,7 @@ int ssc_group_norm_bwd(const void *x, const void *gy, int type, int n, int c, co
  * x [n, c], w_in [2, hidden, c] (gate, up), w_out [c_out, hidden], b_in [2, hidden], b_out [c_out], residual and out [n, c_out], all of
  * `type` (SSC_PREC_FP32 / F16 / BF16); the biases and the residual may be NULL.  act: 0 identity, 1 relu, 2 sigmoid, 3 silu,
  * 4 gelu (erf).  Products are added in float32; float32 operands are used to 24 bits; in 16 bits the hidden rows h = act(.) * (.), and
- * in the backward call their gradients, are rounded to the rows' type (up to 16 rows forward: not rounded).  A value that is not
+ * in the backward call their gradients, are rounded to the rows' type (not in a forward call of up to 256 rows that takes the form for few).  A value that is not
  * finite makes what depends on it infinite or NaN.  Widths are at most 65536, rows at most 2^30; any address and width is accepted, 16-bit widths that are
  * multiples of 8 at addresses that are multiples of 16 are read in place, others are copied to scratch first.
  * scratch: ssc_gated_ff_scratch_bytes(...) bytes, 16-byte aligned; rows are taken in turns so that it stays below about

@@ -227,6 +227,11 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_stats_kernel(GnArgs a) {
   float *sq_s = sm + R * a.c, *sums = sq_s + R * a.c, centred[VEC], quarter[VEC];       // sums: [c] twice
 #pragma unroll
   for (int q = 0; q < VEC; ++q) centred[q] = works && q < many && a.t.scalar_of_channel[ch + q] >= 0 ? 1.f : 0.f, quarter[q] = 0.25f * centred[q];
+  // (what the ends of pieces look up first comes with the first rows)
+  const int lane = t & 31, first_group = t >> 5;
+  const int my_first = t < a.c ? a.t.group_first[a.t.group_of_channel[t]] : 0;
+  int my_from = 0, my_len = 0, my_copies = 1;
+  if (first_group < a.n_group) my_from = a.t.group_first[first_group], my_len = a.t.group_len[first_group], my_copies = a.t.group_copies[first_group];
   GnWalk walk;
   if (ring.r0 < ring.r1) walk.find(a, ring.r0);
   for (int row = ring.r0; row < ring.r1;) {
@@ -291,7 +296,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_stats_kernel(GnArgs a) {
       __syncthreads();
       // (about the first mean of the group from here on: near enough to all of them)
       for (int i = t; i < a.c; i += a.threads) {
-        const float about = sm[a.t.group_first[a.t.group_of_channel[i]]];
+        const float about = sm[i == t ? my_first : a.t.group_first[a.t.group_of_channel[i]]];
         float u = 0.f, v = 0.f;
         for (int r = 0; r < R; ++r) {
           const float d = sm[r * a.c + i] - about, nd = count[r] * d;
@@ -302,14 +307,14 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_stats_kernel(GnArgs a) {
         sums[a.c + i] = v;
       }
       __syncthreads();
-      const int lane = t & 31;
-      for (int g = t >> 5; g < a.n_group; g += a.threads >> 5) {
-        const int from = a.t.group_first[g], len = a.t.group_len[g];
+      for (int g = first_group; g < a.n_group; g += a.threads >> 5) {
+        const bool mine = g == first_group;
+        const int from = mine ? my_from : a.t.group_first[g], len = mine ? my_len : a.t.group_len[g], copies = mine ? my_copies : a.t.group_copies[g];
         float u = 0.f, v = 0.f;
         for (int i = lane; i < len; i += 32) u += sums[from + i], v += sums[a.c + from + i];
         for (int d = 16; d > 0; d >>= 1) u += __shfl_xor_sync(0xffffffffu, u, d), v += __shfl_xor_sync(0xffffffffu, v, d);
         if (lane == 0) {
-          const float n = (float)(end - begin) * (float)a.t.group_copies[g], mean = u / n;
+          const float n = (float)(end - begin) * (float)copies, mean = u / n;
           *(float2 *)(a.partial + ((size_t)(blockIdx.x + walk.s) * a.n_group + g) * 2) = {sm[from] + mean, fmaxf(v - u * mean, 0.f)};
         }
       }
@@ -744,14 +749,15 @@ GnVec gn_vec(int c, int c_out, int type, bool grads) {
 }
 constexpr int kGnBlocks = 2;               // to an SM
 
-// Tiles of four rows to a thread, two where gradients come with them (8 to 16 KB, a multiple of 16 bytes); a ring of up to 88 KB.
+// Tiles of four rows to a thread, two where gradients come with them but no gates (8 to 16 KB, a multiple of 16 bytes); a ring of up to 88 KB.  (96011 rows of
+// 64 + 12 channels: gradients with tiles of two rows 32 and 34 us, of four 29 and 31.  65536 of 256 without gates: two 40 and 40, four 43 and 41.)
 void gn_shape(GnArgs &a, int type, int vec, bool grads) {
   const int bytes = a.c * type_bytes(type);
   const int wide = (a.c + vec - 1) / vec;
   a.threads = wide > 256 || a.n_gate > 256 ? kGnThreads : 256;
   const int rows = a.threads / wide;
   const long long slots = (long long)sm_count() * kGnBlocks;
-  int each = grads ? 2 : 4;
+  int each = grads && a.n_gate == 0 ? 2 : 4;
   while ((rows * each * bytes) % 16 || (rows * each * a.c_out * type_bytes(type)) % 16) each *= 2;
   a.tile = rows * each;
   a.x_bytes = (uint32_t)align_up((size_t)a.tile * bytes, 128);
