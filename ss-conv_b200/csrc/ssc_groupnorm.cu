@@ -331,40 +331,78 @@ __device__ __forceinline__ void sample_pieces(const GnArgs &a, const GnWalk &k, 
   many = k.hi > k.lo ? (k.hi - 1) / a.range - first + 1 : 0;
 }
 __device__ __forceinline__ int piece_rows(const GnArgs &a, const GnWalk &k, int block) {
-  const long long lo = (long long)block * a.range;
-  return (int)(min(lo + a.range, (long long)k.hi) - max(lo, (long long)k.lo));
+  const int lo = block * a.range;          // (a range is a small share of at most 2^30 rows)
+  return min(lo + a.range, k.hi) - max(lo, k.lo);
 }
 
-// Lanes to a group where the pieces of a sample are added up: most samples have few.
-__device__ __forceinline__ int lanes_for(int many) { return many <= 4 ? 4 : many <= 8 ? 8 : 32; }
+// The sums (u, v) of each group over the partial results of a sample: add(group, piece, the first result, this one, u, v), end(group, u, v).
+// Few pieces: up to eight lanes to a group.  Many, as in a sample that all blocks share: lanes side by side read neighbouring groups, each warp
+// its share of the pieces.  (Two samples of 1750 rows in 290 pieces, 32 groups: a group to a warp, which fetches a sector for each of
+// its results, 16.3 us for the second pass forward, this way 11.5; one sample of 203437 rows, 8 groups 17.9 and 16.8.)
+constexpr int kGnPieces = 4;               // in flight
+template <class Add, class End>
+__device__ __forceinline__ void sample_sums(const GnArgs &a, const float *from, int many, Add add, End end) {
+  const float2 *all = (const float2 *)from;
+  const int lane = threadIdx.x & 31;
+  if (many <= 8) {
+    const int width = many <= 4 ? 4 : 8, at = lane & (width - 1);
+    for (int g0 = 0; g0 < a.n_group; g0 += a.threads / width) {
+      const int g = g0 + threadIdx.x / width;
+      float u = 0.f, v = 0.f;
+      if (g < a.n_group && at < many) add(g, at, all[g], all[(size_t)at * a.n_group + g], u, v);
+      for (int d = width / 2; d > 0; d >>= 1) u += __shfl_xor_sync(0xffffffffu, u, d), v += __shfl_xor_sync(0xffffffffu, v, d);
+      if (at == 0 && g < a.n_group) end(g, u, v);
+    }
+    return;
+  }
+  __shared__ float2 parts[kGnThreads / 32][32];
+  const int warp = threadIdx.x >> 5, warps = a.threads >> 5;
+  int wide = 1;
+  while (wide < a.n_group && wide < 32) wide *= 2;
+  const int step = warps * (32 / wide);
+  for (int g0 = 0; g0 < a.n_group; g0 += wide) {
+    const int g = g0 + (lane & (wide - 1));
+    float u = 0.f, v = 0.f;
+    if (g < a.n_group) {
+      const float2 about = all[g];
+      for (int i0 = warp * (32 / wide) + lane / wide; i0 < many; i0 += kGnPieces * step) {
+        float2 p[kGnPieces];
+#pragma unroll
+        for (int k = 0; k < kGnPieces; ++k) p[k] = all[(size_t)min(i0 + k * step, many - 1) * a.n_group + g];
+#pragma unroll
+        for (int k = 0; k < kGnPieces; ++k)
+          if (i0 + k * step < many) add(g, i0 + k * step, about, p[k], u, v);
+      }
+    }
+    for (int d = wide; d < 32; d *= 2) u += __shfl_xor_sync(0xffffffffu, u, d), v += __shfl_xor_sync(0xffffffffu, v, d);
+    if (lane < wide) parts[warp][lane] = {u, v};
+    __syncthreads();
+    if ((int)threadIdx.x < wide && g < a.n_group) {
+      for (int w = 1; w < warps; ++w) u += parts[w][lane].x, v += parts[w][lane].y;
+      end(g, u, v);
+    }
+    if (g0 + wide < a.n_group) __syncthreads();
+  }
+}
 
 // mu and r of the walk's sample, from the partial results of its pieces, to shared memory; the block with its first row keeps them.
 __device__ __forceinline__ void sample_stats(const GnArgs &a, const GnWalk &k, float *gs) {
   int first, many;
   sample_pieces(a, k, first, many);
-  const int width = lanes_for(many), lane = threadIdx.x & (width - 1), rows = k.hi - k.lo;
-  const float *from = a.partial + (size_t)(first + k.s) * a.n_group * 2;
-  for (int g0 = 0; g0 < a.n_group; g0 += a.threads / width) {
-    const int g = g0 + threadIdx.x / width;
-    float u = 0.f, v = 0.f, about = 0.f;
-    if (g < a.n_group) {
-      about = from[2 * g];
-      const float over = 1.0f / (float)a.t.group_copies[g];
-      for (int i = lane; i < many; i += width) {
-        const float2 p = *(const float2 *)(from + ((size_t)i * a.n_group + g) * 2);
-        const float d = p.x - about, nd = (float)piece_rows(a, k, first + i) * d;
+  const float rows = (float)(k.hi - k.lo);
+  sample_sums(
+      a, a.partial + (size_t)(first + k.s) * a.n_group * 2, many,
+      [&](int g, int i, float2 about, float2 p, float &u, float &v) {
+        const float d = p.x - about.x, nd = (float)piece_rows(a, k, first + i) * d;
         u += nd;
-        v += fmaf(nd, d, p.y * over);
-      }
-    }
-    for (int d = width / 2; d > 0; d >>= 1) u += __shfl_xor_sync(0xffffffffu, u, d), v += __shfl_xor_sync(0xffffffffu, v, d);
-    if (lane == 0 && g < a.n_group) {
-      const float mean = u / (float)rows;
-      const float2 r = {about + mean, 1.0f / sqrtf(fmaxf(v - u * mean, 0.f) / (float)rows + a.eps)};
-      *(float2 *)(gs + 2 * g) = r;
-      if (first == (int)blockIdx.x) *(float2 *)(a.stats + ((size_t)k.s * a.n_group + g) * 2) = r;
-    }
-  }
+        v += fmaf(nd, d, __fdividef(p.y, (float)a.t.group_copies[g]));
+      },
+      [&](int g, float u, float v) {
+        const float mean = u / rows;
+        const float2 r = {a.partial[((size_t)(first + k.s) * a.n_group + g) * 2] + mean, 1.0f / sqrtf(fmaxf(v - u * mean, 0.f) / rows + a.eps)};
+        *(float2 *)(gs + 2 * g) = r;
+        if (first == (int)blockIdx.x) *(float2 *)(a.stats + ((size_t)k.s * a.n_group + g) * 2) = r;
+      });
   __syncthreads();
 }
 
@@ -571,24 +609,18 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_bwd_kernel(GnArgs a, int sum
       if (!SUMS) {
         int first, many;
         sample_pieces(a, walk, first, many);
-        const int width = lanes_for(many), lane = t & (width - 1);
-        const float *from = a.partial + (size_t)(first + walk.s) * a.n_group * 2;
-        for (int g0 = 0; g0 < a.n_group; g0 += a.threads / width) {
-          const int g = g0 + t / width;
-          float u = 0.f, v = 0.f;
-          if (g < a.n_group)
-            for (int i = lane; i < many; i += width) {
-              const float2 p = *(const float2 *)(from + ((size_t)i * a.n_group + g) * 2);
+        const float rows = (float)(walk.hi - walk.lo);
+        sample_sums(
+            a, a.partial + (size_t)(first + walk.s) * a.n_group * 2, many,
+            [&](int, int, float2, float2 p, float &u, float &v) {
               u += p.x;
               v += p.y;
-            }
-          for (int d = width / 2; d > 0; d >>= 1) u += __shfl_xor_sync(0xffffffffu, u, d), v += __shfl_xor_sync(0xffffffffu, v, d);
-          if (lane == 0 && g < a.n_group) {
-            const float m = 1.0f / ((float)(walk.hi - walk.lo) * (float)a.t.group_copies[g]);
-            gs[2 * g] = u * m;
-            gs[2 * g + 1] = v * m;
-          }
-        }
+            },
+            [&](int g, float u, float v) {
+              const float m = 1.0f / (rows * (float)a.t.group_copies[g]);
+              gs[2 * g] = u * m;
+              gs[2 * g + 1] = v * m;
+            });
         __syncthreads();
 #pragma unroll
         for (int q = 0; q < VEC; ++q) {
@@ -750,7 +782,7 @@ GnVec gn_vec(int c, int c_out, int type, bool grads) {
 constexpr int kGnBlocks = 2;               // to an SM
 
 // Tiles of four rows to a thread, two where gradients come with them but no gates (8 to 16 KB, a multiple of 16 bytes); a ring of up to 88 KB.  (96011 rows of
-// 64 + 12 channels: gradients with tiles of two rows 32 and 34 us, of four 29 and 31.  65536 of 256 without gates: two 40 and 40, four 43 and 41.)
+// 64 + 12 channels: gradients with tiles of two rows 32 and 34 us, of four 29 and 30.  65536 of 256 without gates: two 40 and 40, four 43 and 41.)
 void gn_shape(GnArgs &a, int type, int vec, bool grads) {
   const int bytes = a.c * type_bytes(type);
   const int wide = (a.c + vec - 1) / vec;
@@ -758,6 +790,7 @@ void gn_shape(GnArgs &a, int type, int vec, bool grads) {
   const int rows = a.threads / wide;
   const long long slots = (long long)sm_count() * kGnBlocks;
   int each = grads && a.n_gate == 0 ? 2 : 4;
+  while (each > 1 && a.n <= slots * rows * (each / 2)) each /= 2;       // (few rows: more blocks; 3501 of 32 + 6 channels 9.9 us, 12.7 without)
   while ((rows * each * bytes) % 16 || (rows * each * a.c_out * type_bytes(type)) % 16) each *= 2;
   a.tile = rows * each;
   a.x_bytes = (uint32_t)align_up((size_t)a.tile * bytes, 128);
