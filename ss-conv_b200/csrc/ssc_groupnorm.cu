@@ -11,7 +11,7 @@
 // tiles: with loads in the threads themselves, registers for the rows in flight left room for two blocks of
 // 256 threads, which waited for memory half of the time.
 //
-// 786432 rows of 128 in bf16: sums 53 us (3.8 TB/s), second pass 85 (4.7 TB/s read and written).  65536 rows of 256 in float32, all in L2: 22 and 23, backward 40 and
+// 786432 rows of 128 in bf16: sums 52 us (3.9 TB/s), second pass 85 (4.7 TB/s read and written).  65536 rows of 256 in float32, all in L2: 22 and 23, backward 40 and
 // 40.  A launch on next to nothing takes 6 to 8 us (tables, offsets, the copies' first latency, sums at the end); from there on instructions bound it, 10 to 30 a value
 // at half of the issue slots: more warps, bigger tiles, and a second pass from the end (to find rows in L2) changed nothing or cost elsewhere.
 #include <cuda_bf16.h>

@@ -84,6 +84,9 @@ CASES = [
     ([1, 500000], [(40, 0)], 5, F.silu),                                # rings that go round several times
     ([150000, 2, 150001], [(8, 0), (4, 1), (4, 0)], 2, GATE),
     ([3] * 40 + [0] * 40 + [500], [(5, 0), (1, 2), (1, 0)], 1, GATE),   # many pieces to a block, rows of no multiple of anything
+    ([9000, 3000], [(80, 0)], 80, F.silu),                              # more groups than lanes, each in many pieces
+    ([6000], [(33, 0), (33, 1), (33, 0)], 33, GATE),
+    ([2500, 2500], [(5, 0), (5, 1), (5, 0)], 1, GATE),                  # three groups in many pieces
 ]
 
 
