@@ -3,8 +3,9 @@
 // The special-function unit (sixteen lanes a cycle and SM) bounds sigmoids: an exponential and a reciprocal each would be 46 us for the 100 M values
 // of 786432 rows of 128.  So two of them share a reciprocal: 1 / d0 = d1 / (d0 d1).  The exponential is the approximate one, two
 // steps and |z| 2^-24 relative, in what is added to one.  EXACT: the correctly rounded reciprocal of the product; otherwise, for
-// values that are rounded to 16 bits, the approximate one.  Denominators end at 2^62 (the product stays finite): sigmoids below 2^-62
-// become that.
+// values that are rounded to 16 bits, the approximate one.  Where a product of denominators is beyond 2^124, or not a number, all N values take a
+// reciprocal of their own: a sigmoid of a large negative argument has to be as small as it is, and 0 below 2^-125, since SiLU multiplies it by
+// the argument.
 // The kind is the same for a whole launch, so the branch on it stands outside the loop over the values: inside
 // it cost five times the arithmetic.
 #pragma once
@@ -19,23 +20,41 @@ __device__ __forceinline__ float exp2_quick(float v) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
+constexpr float kNoSigmoid = -87.f;         // exp(-87) = 2^-125.5
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float min_or_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// (of at least 2^-125)
+__device__ __forceinline__ float one_sigmoid(float z) { return quick_reciprocal(min_or_nan(1.0f + exp2_quick(-1.44269504f * z), 0x1p125f)); }
 template <bool EXACT, int N>
 __device__ __forceinline__ void sigmoids(const float *z, float *s) {
   const f32x2 one = pair_of(1.0f, 1.0f), log2e = pair_of(-1.44269504f, -1.44269504f);
+  float most = 0.f;
 #pragma unroll
   for (int i = 0; i + 1 < N; i += 2) {
     const float2 x = halves(mul_pair(pair_of(z[i], z[i + 1]), log2e));
-    const float2 e = halves(add_pair(pair_of(exp2_quick(x.x), exp2_quick(x.y)), one));
-    const float d0 = fminf(e.x, 0x1p62f), d1 = fminf(e.y, 0x1p62f);      // (a number for NaN too: the neighbour keeps its value)
-    const float p = d0 * d1;
+    const float2 d = halves(add_pair(pair_of(exp2_quick(x.x), exp2_quick(x.y)), one));
+    const float p = d.x * d.y;
+    most = max_or_nan(most, p);
     float r;
     if (EXACT) r = quick_reciprocal(p);
     else asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(p));
-    const float2 both = halves(mul_pair(pair_of(r, r), pair_of(d1, d0)));
+    const float2 both = halves(mul_pair(pair_of(r, r), pair_of(d.y, d.x)));
     s[i] = both.x;
     s[i + 1] = both.y;
   }
-  if (N % 2 == 1) s[N - 1] = quick_reciprocal(fminf(1.0f + exp2_quick(-1.44269504f * z[N - 1]), 0x1p62f));
+  if (N > 1 && !(most < 0x1p124f)) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = z[i] < kNoSigmoid ? 0.f : one_sigmoid(z[i]);
+  }
+  if (N % 2 == 1) s[N - 1] = one_sigmoid(z[N - 1]);
 }
 // Values two at a time: half the instructions.  a * b, a * b + c; each argument is an array or one number for all.
 __device__ __forceinline__ f32x2 pair_at(const float *a, int i) { return pair_of(a[i], a[i + 1]); }
@@ -75,10 +94,11 @@ __device__ __forceinline__ void act_values(float *v, int kind) {
     case 2:
       sigmoids<EXACT, N>(v, s);
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = v[i] == v[i] ? s[i] : v[i];
+      for (int i = 0; i < N; ++i) v[i] = s[i];
       break;
     case 3:
       sigmoids<EXACT, N>(v, s);
+      if (N % 2 == 1 && v[N - 1] < kNoSigmoid) s[N - 1] = 0.f;
       multiply<N>(v, v, s);
       break;
     case 4:
@@ -104,12 +124,13 @@ __device__ __forceinline__ void act_slopes(float *v, float *s, int kind) {
       sigmoids<EXACT, N>(v, s);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        v[i] = v[i] == v[i] ? s[i] : v[i];
+        v[i] = s[i];
         s[i] = v[i] * (1.f - v[i]);
       }
       break;
     case 3:
       sigmoids<EXACT, N>(v, s);
+      if (N % 2 == 1 && v[N - 1] < kNoSigmoid) s[N - 1] = 0.f;
       multiply<N>(v, v, s);
       {
         float rest[N];
