@@ -81,7 +81,8 @@ class _Layout(object):
         return kept
 
 
-@functools.lru_cache(maxsize=256)
+# (for good: a recorded graph and a kernel on another stream hold the address of a layout's table and no reference.  At most 90 KB each.)
+@functools.lru_cache(maxsize=None)
 def _layout(Rs, groups, gated, scalar_act):
     if not Rs or groups < 1 or any(m < 0 or l < 0 for m, l in Rs) or sum(m for m, _ in Rs) == 0:
         raise ValueError("Rs must be [(copies, order), ...] and the number of groups positive (got %s, %s)" % (list(Rs), groups))

@@ -1,0 +1,37 @@
+"""What the row operators keep from one call for the next: channel tables on the device and the status word."""
+import gc
+import weakref
+
+import pytest
+import torch
+
+CPU = torch.device("cpu")
+
+
+def test_channel_tables_outlive_any_number_of_layouts():
+    """A recorded graph holds a table's address and nothing else: tables stay for the life of the process."""
+    from ss_conv.groupnorm import GroupNorm, _layout, _plan
+    norm = GroupNorm([(777, 0)], 7)
+    table = _plan(tuple(norm.Rs), 7, None)[0].table(CPU)
+    where, alive = table.data_ptr(), weakref.ref(table)
+    del table
+    for m in range(1, 600):
+        _plan(((m, 1),), 1, None)[0].table(CPU)
+        _layout(((m, 2),), 1, False, False)
+    gc.collect()
+    assert alive() is not None
+    again = _plan(tuple(norm.Rs), 7, None)[0].table(CPU)
+    assert again is alive() and again.data_ptr() == where
+
+
+def test_plans_do_not_keep_modules():
+    """What is kept for good are tables, not the activation modules that calls were made with."""
+    from ss_conv.groupnorm import _plan
+    act = torch.nn.SiLU()
+    alive = weakref.ref(act)
+    _plan(((8, 0),), 2, act)
+    del act
+    for m in range(1, 300):
+        _plan(((m, 1),), 1, None)
+    gc.collect()
+    assert alive() is None
