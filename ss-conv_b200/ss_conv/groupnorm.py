@@ -77,6 +77,9 @@ class _Layout(object):
     def table(self, device):
         kept = self.tables.get(device)
         if kept is None:
+            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the channel tables of a group norm are uploaded by its first call, which cannot be inside a "
+                                   "recording: call it once before")
             kept = self.tables[device] = torch.tensor(self.rows, dtype=torch.int32).to(device)
         return kept
 

@@ -35,3 +35,18 @@ def test_plans_do_not_keep_modules():
         _plan(((m, 1),), 1, None)
     gc.collect()
     assert alive() is None
+
+
+def test_first_call_of_a_layout_inside_a_recording_is_refused(monkeypatch):
+    """Before anything reaches the device: the upload would void the recording.  A table that is there is handed out."""
+    from ss_conv.groupnorm import _layout
+    device = torch.device("cuda", 0)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    lay = _layout(((13, 0),), 13, False, False)
+    with pytest.raises(RuntimeError, match="call it once before"):
+        lay.table(device)
+    assert not lay.tables
+    lay.tables[device] = "there"
+    assert lay.table(device) == "there"
+    assert lay.table(CPU).dtype == torch.int32
+    lay.tables.clear()
