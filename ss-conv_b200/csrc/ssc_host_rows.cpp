@@ -116,6 +116,9 @@ Tensor norm_forward(const Tensor &x, const Tensor &weight, const Tensor &bias, c
 // A node takes what may be absent as an optional: absent ones have no edge, the others are numbered without them.
 typedef std::optional<Tensor> Maybe;
 Maybe maybe(const Tensor &t) { return t.defined() ? Maybe(t) : Maybe(); }
+// What the process keeps (channel tables, the status word) goes along as it is, not as a saved variable: those are checked for changes in place,
+// and clearing the status word is one.
+void keep(torch::autograd::AutogradContext *ctx, const char *name, const Tensor &t) { ctx->saved_data[name] = t; }
 
 struct NormNode : torch::autograd::Function<NormNode> {
   static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Maybe &maybe_weight, const Maybe &maybe_bias, const Tensor &offsets,
@@ -123,7 +126,9 @@ struct NormNode : torch::autograd::Function<NormNode> {
     const Tensor weight = maybe_weight.value_or(Tensor()), bias = maybe_bias.value_or(Tensor());
     Tensor stats;
     const Tensor y = norm_forward(x, weight, bias, offsets, table, status, k, x.scalar_type(), stats);
-    ctx->save_for_backward({x, weight, bias, offsets, table, status, stats});
+    ctx->save_for_backward({x, weight, bias, offsets, stats});
+    keep(ctx, "table", table);
+    keep(ctx, "status", status);
     ctx->saved_data["k"] = std::vector<int64_t>{k.n_field, k.n_scalar, k.n_group, k.n_gate, k.scalar_act, k.gate_act};
     ctx->saved_data["eps"] = k.eps;
     return y;
@@ -131,7 +136,8 @@ struct NormNode : torch::autograd::Function<NormNode> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
     first_gradient("group_norm");
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &offsets = saved[3], &table = saved[4], &status = saved[5], &stats = saved[6];
+    const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &offsets = saved[3], &stats = saved[4];
+    const Tensor table = ctx->saved_data["table"].toTensor(), status = ctx->saved_data["status"].toTensor();
     if (!grads[0].defined()) return torch::autograd::variable_list(7);
     const std::vector<int64_t> k = ctx->saved_data["k"].toIntVector();
     const c10::DeviceGuard guard(x.device());
@@ -194,7 +200,8 @@ struct FfNode : torch::autograd::Function<FfNode> {
                         const Maybe &residual, const Tensor &status, int64_t act) {
     const Tensor bias = b_in.value_or(Tensor());
     const Tensor y = ff_forward(x, w_in, w_out, bias, b_out.value_or(Tensor()), residual.value_or(Tensor()), status, act);
-    ctx->save_for_backward({x, w_in, w_out, bias, status});
+    ctx->save_for_backward({x, w_in, w_out, bias});
+    keep(ctx, "status", status);
     ctx->saved_data["act"] = act;
     ctx->saved_data["has"] = (b_in.has_value() ? 1 : 0) | (b_out.has_value() ? 2 : 0) | (residual.has_value() ? 4 : 0);
     return y;
@@ -202,7 +209,8 @@ struct FfNode : torch::autograd::Function<FfNode> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
     first_gradient("gated_feedforward");
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &w_in = saved[1], &w_out = saved[2], &b_in = saved[3], &status = saved[4];
+    const Tensor &x = saved[0], &w_in = saved[1], &w_out = saved[2], &b_in = saved[3];
+    const Tensor status = ctx->saved_data["status"].toTensor();
     torch::autograd::variable_list out(8);
     if (!grads[0].defined()) return out;
     const c10::DeviceGuard guard(x.device());

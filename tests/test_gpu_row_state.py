@@ -31,3 +31,41 @@ def test_new_layout_inside_a_recording(cuda):
     again.replay()
     torch.cuda.synchronize()
     assert torch.equal(y, want)
+
+
+def test_training_after_a_first_call_in_inference_mode(cuda, monkeypatch):
+    from ss_conv import _ext
+    from ss_conv.feedforward import gated_feedforward
+    from ss_conv.groupnorm import group_norm
+    monkeypatch.setattr(_ext, "_status", {})
+    g = torch.Generator("cuda").manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=g, device=cuda)  # noqa: E731
+    x, off, w_in, w_out = r(90, 34), offsets(cuda, 40, 90), r(2, 16, 34), r(34, 16)
+
+    def step(x):
+        return gated_feedforward(group_norm(x, off, [(34, 0)], 17, activation=F.silu), w_in, w_out)
+
+    with torch.inference_mode():
+        want = step(x)
+    leaf = x.clone().requires_grad_(True)
+    y = step(leaf)
+    assert torch.equal(y.detach(), want) and torch.autograd.grad(y.sum(), [leaf])[0].any()
+    _ext.check_status(cuda)
+
+
+def test_status_cleared_between_a_result_and_its_gradients(cuda):
+    """A problem of one batch is raised and cleared; the passes of the others go on."""
+    from ss_conv import _ext
+    from ss_conv.feedforward import gated_feedforward
+    from ss_conv.groupnorm import group_norm
+    g = torch.Generator("cuda").manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=g, device=cuda)  # noqa: E731
+    x, off, w_in, w_out = r(90, 32).requires_grad_(True), offsets(cuda, 40, 90), r(2, 16, 32), r(32, 16)
+    passes = (lambda: group_norm(x, off, [(32, 0)], 4), lambda: gated_feedforward(x, w_in, w_out))
+    want = [torch.autograd.grad(p().sum(), [x])[0] for p in passes]
+    for p, w in zip(passes, want):
+        y = p().sum()
+        _ext.status_word(cuda).fill_(1)
+        with pytest.raises(RuntimeError, match="kernel status 0x1"):
+            _ext.check_status(cuda)
+        assert torch.equal(torch.autograd.grad(y, [x])[0], w)
