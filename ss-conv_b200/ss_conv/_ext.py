@@ -296,7 +296,8 @@ def status_word(device):
     key = (device if isinstance(device, torch.device) else torch.device(device)).index
     if key not in _status:
         _open_alarm()
-        _status[key] = torch.zeros(1, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):       # (it is cleared in place in any mode)
+            _status[key] = torch.zeros(1, dtype=torch.int32, device=device)
     return _status[key]
 
 

@@ -80,7 +80,8 @@ class _Layout(object):
             if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("the channel tables of a group norm are uploaded by its first call, which cannot be inside a "
                                    "recording: call it once before")
-            kept = self.tables[device] = torch.tensor(self.rows, dtype=torch.int32).to(device)
+            with torch.inference_mode(False):       # (it serves training passes as well)
+                kept = self.tables[device] = torch.tensor(self.rows, dtype=torch.int32).to(device)
         return kept
 
 

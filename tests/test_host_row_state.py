@@ -50,3 +50,15 @@ def test_first_call_of_a_layout_inside_a_recording_is_refused(monkeypatch):
     assert lay.table(device) == "there"
     assert lay.table(CPU).dtype == torch.int32
     lay.tables.clear()
+
+
+def test_what_is_kept_is_no_inference_tensor(monkeypatch):
+    """The first call may be an evaluation under inference_mode; training passes use the same tensors afterwards."""
+    from ss_conv import _ext
+    from ss_conv.groupnorm import _layout
+    monkeypatch.setattr(_ext, "_status", {})
+    monkeypatch.setattr(_ext, "_open_alarm", lambda: None)
+    with torch.inference_mode():
+        assert not _layout(((14, 0),), 14, False, False).table(CPU).is_inference()
+        assert not _ext.status_word(CPU).is_inference()
+    _ext.status_word(CPU).zero_()
