@@ -88,6 +88,11 @@ void recordable(std::initializer_list<const Tensor *> all, const Tensor &x) {
   TORCH_CHECK(!foreign || c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None,
               "a result computed before this recording still holds the gradient graph of the same tensors: drop it (its loss) before recording");
 }
+// A tangent would be dropped without a word: the operators have no forward-mode derivative.
+void no_tangents(const char *what, std::initializer_list<const Tensor *> all) {
+  for (const Tensor *t : all)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), what, ": forward-mode derivatives are not available");
+}
 void first_gradient(const char *what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, ": gradients of gradients are not available (create_graph)");
 }
@@ -171,6 +176,7 @@ Tensor norm(const Tensor &features, const Tensor &weight_in, const Tensor &bias_
                     offsets_in.device(), ")");
   check_parameter("weight", weight_in, k.n_field, features);
   check_parameter("bias", bias_in, k.n_scalar, features);
+  no_tangents("group_norm", {&features, &weight_in, &bias_in});
   const c10::DeviceGuard guard(features.device());
   const Tensor x = aligned(features), offsets = offsets_in.contiguous();
   const Tensor weight = weight_in.defined() ? weight_in.to(at::kFloat).contiguous() : weight_in, bias = bias_in.defined() ? bias_in.to(at::kFloat).contiguous() : bias_in;
@@ -255,6 +261,7 @@ Tensor feedforward(const Tensor &x, const Tensor &w_in, const Tensor &w_out, con
   wants("bias_in", b_in, {2, hidden});
   wants("bias_out", b_out, {c_out});
   wants("residual", residual, {x.size(0), c_out});
+  no_tangents("gated_feedforward", {&x, &w_in, &w_out, &b_in, &b_out, &residual});
   auto flat = [](const Tensor &t) { return t.defined() ? t.contiguous() : t; };
   const Tensor a = flat(x), b = flat(w_in), d = flat(w_out), e = flat(b_in), f = flat(b_out), g = flat(residual);
   if (!recorded({&a, &b, &d, &e, &f, &g})) return ff_forward(a, b, d, e, f, g, status, act);

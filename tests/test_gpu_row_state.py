@@ -69,3 +69,25 @@ def test_status_cleared_between_a_result_and_its_gradients(cuda):
         with pytest.raises(RuntimeError, match="kernel status 0x1"):
             _ext.check_status(cuda)
         assert torch.equal(torch.autograd.grad(y, [x])[0], w)
+
+
+def test_tangents_are_refused(cuda):
+    """Each argument of either operator, recorded by autograd or not: a derivative of zero would be wrong."""
+    import torch.autograd.forward_ad as fa
+    from ss_conv.feedforward import gated_feedforward
+    from ss_conv.groupnorm import group_norm
+    off = offsets(cuda, 40, 90)
+    z = lambda *s: torch.ones(*s, device=cuda)  # noqa: E731
+    norm = dict(features=z(90, 16), weight=z(16), bias=z(16))
+    ff = dict(features=z(90, 16), weight_in=z(2, 8, 16), weight_out=z(16, 8), bias_in=z(2, 8), bias_out=z(16), residual=z(90, 16))
+    for call, args in ((lambda **k: group_norm(offsets=off, Rs=[(16, 0)], **k), norm), (gated_feedforward, ff)):
+        call(**args)
+        for name, v in args.items():
+            for leaf in (False, True):
+                with fa.dual_level():
+                    dual = fa.make_dual(v.clone().requires_grad_(leaf), torch.ones_like(v))
+                    with pytest.raises(RuntimeError, match="forward-mode"):
+                        call(**{**args, name: dual})
+                    with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                        call(**{**args, name: dual})
+                call(**args)
