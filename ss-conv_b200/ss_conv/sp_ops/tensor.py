@@ -228,10 +228,15 @@ class SparseTensor(object):
             if n != self._features.shape[0] or n != self._indices.shape[0]:
                 self._cut = n
             return False
-        with torch.set_grad_enabled(r.grad):
-            feats, self._indices = r.redo()   # (what works sample by sample looks at the new rows' indices)
-            for fn in r.post:
-                feats = fn(feats)
+        kept = self._indices
+        try:
+            with torch.set_grad_enabled(r.grad):
+                feats, self._indices = r.redo()   # (what works sample by sample looks at the new rows' indices)
+                for fn in r.post:
+                    feats = fn(feats)
+        except BaseException:
+            self._rows, self._indices = r, kept   # as it was: the next look recomputes, or raises again
+            raise
         self._features = feats
         self._recomputed = True
         return True

@@ -62,3 +62,28 @@ def test_what_is_kept_is_no_inference_tensor(monkeypatch):
         assert not _layout(((14, 0),), 14, False, False).table(CPU).is_inference()
         assert not _ext.status_word(CPU).is_inference()
     _ext.status_word(CPU).zero_()
+
+
+def test_rows_stay_pending_when_their_recomputation_fails():
+    """An operation behind a row count that did not fit raises: no half of the new rows is left behind, and the next look tries again."""
+    from ss_conv.sp_ops.tensor import PendingRows, SparseTensor
+    old, new = torch.zeros(4, 3), torch.arange(21.0).view(7, 3)
+    old_inds, new_inds = torch.zeros(4, 4, dtype=torch.int32), torch.ones(7, 4, dtype=torch.int32)
+    t = SparseTensor(old, old_inds, [8] * 3, 2)
+    t._rows = PendingRows(torch.tensor([7], dtype=torch.int32), 4, None, lambda: (new, new_inds))
+    t._rows.count.value = 7
+    fails, seen = [True, True], []
+
+    def rowwise(f):
+        seen.append(t.get_offsets().tolist())       # (sample by sample: of the new rows)
+        if fails and fails.pop():
+            raise RuntimeError("no room")
+        return f + 1
+
+    t._rows.post.append(rowwise)
+    for look in (lambda: t.features, lambda: t.indices):
+        with pytest.raises(RuntimeError, match="no room"):
+            look()
+        assert t.pending() and t._features is old and t._indices is old_inds
+    assert torch.equal(t.features, new + 1) and t.indices is new_inds and not t.pending()
+    assert seen == [[0, 0, 7]] * 3
