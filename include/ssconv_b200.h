@@ -619,8 +619,9 @@ int ssc_group_norm_bwd(const void *x, const void *gy, int type, int n, int c, co
  * in the backward call their gradients, are rounded to the rows' type (not in a forward call of up to 256 rows that takes the form for few).  A value that is not
  * finite makes what depends on it infinite or NaN.  Widths are at most 65536, rows at most 2^30; any address and width is accepted, 16-bit widths that are
  * multiples of 8 at addresses that are multiples of 16 are read in place, others are copied to scratch first.
- * scratch: ssc_gated_ff_scratch_bytes(...) bytes, 16-byte aligned; rows are taken in turns so that it stays below about
- * a gigabyte beside the weights.  Sums have a fixed order.
+ * scratch: ssc_gated_ff_scratch_bytes(...) bytes, 16-byte aligned; rows are taken in turns so that theirs is at most 2^30 bytes and
+ * shares of split sums 2^27, beside what the weights take (their planes or padded rows, and in the backward call their gradients in
+ * float32).  Sums have a fixed order.
  * ssc_gated_ff_bwd: gy [n, c_out]; gx, gw_in, gw_out, gb_in, gb_out of the shapes above, each may be NULL (the residual's
  * gradient is gy).  status: as in ssc_conv_fwd. */
 size_t ssc_gated_ff_scratch_bytes(int type, int n, int c, int hidden, int c_out, int backward);

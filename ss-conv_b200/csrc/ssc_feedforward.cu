@@ -1434,11 +1434,12 @@ size_t row_split_bytes(const Ff &f, long long rows, int blocks, int cols) {
   return s > 1 ? align_up((size_t)s * rows * cols * sizeof(float), 256) : 0;
 }
 
-// Rows of one go, so that what lies between the products is at most about a gigabyte.
+// Rows of one go, so that what lies between the products (planes or rows of h, dg, du, x and dy, dh of float32) is at most a gigabyte: 487 rows
+// of the widest there are, a tile or more.
 long long rows_at_once(const Ff &f, bool backward) {
-  const long long per = (long long)pitch_of(f.hidden) * 2 * planes_for(f.type) * (backward ? 3 : 1) + (long long)(pitch_of(f.c) + pitch_of(f.c_out)) * 2 * planes_for(f.type);
-  long long rows = (1ll << 30) / per / kTileM * kTileM;
-  if (rows < 16 * kTileM) rows = 16 * kTileM;
+  const long long hidden = 2 * planes_for(f.type) * (backward ? 3 : 1) + (backward && f.type == SSC_PREC_FP32 ? 4 : 0);
+  const long long per = pitch_of(f.hidden) * hidden + (long long)(pitch_of(f.c) + pitch_of(f.c_out)) * 2 * planes_for(f.type);
+  const long long rows = (1ll << 30) / per / kTileM * kTileM;
   return rows < f.n ? rows : f.n;
 }
 
