@@ -1,9 +1,9 @@
 // Activations of rows of scalars and their slopes: 0 identity, 1 relu, 2 sigmoid, 3 silu, 4 gelu (erf).
 //
 // The special-function unit (sixteen lanes a cycle and SM) bounds sigmoids: an exponential and a reciprocal each would be 46 us for the 100 M values
-// of 786432 rows of 128.  So two of them share a reciprocal: 1 / d0 = d1 / (d0 d1).  The exponential is the approximate one, two
-// steps and |z| 2^-24 relative, in what is added to one.  EXACT: the correctly rounded reciprocal of the product; otherwise, for
-// values that are rounded to 16 bits, the approximate one.  Where a product of denominators is beyond 2^124, or not a number, all N values take a
+// of 786432 rows of 128.  So two of them share a reciprocal: 1 / d0 = d1 / (d0 d1).  EXACT: the exponential to two steps,
+// the reciprocal of the product correctly rounded; otherwise, for values that are rounded to 16 bits, the approximate ones, of which the
+// exponential is off by |z| 2^-24 besides, the rounding of its exponent.  Where a product of denominators is beyond 2^124, or not a number, all N values take a
 // reciprocal of their own: a sigmoid of a large negative argument has to be as small as it is, and 0 below 2^-125, since SiLU multiplies it by
 // the argument.
 // The kind is the same for a whole launch, so the branch on it stands outside the loop over the values: inside
@@ -32,15 +32,27 @@ __device__ __forceinline__ float min_or_nan(float a, float b) {
   return r;
 }
 // (of at least 2^-125)
-__device__ __forceinline__ float one_sigmoid(float z) { return quick_reciprocal(min_or_nan(1.0f + exp2_quick(-1.44269504f * z), 0x1p125f)); }
+template <bool EXACT>
+__device__ __forceinline__ float one_sigmoid(float z) {
+  return quick_reciprocal(min_or_nan(1.0f + (EXACT ? expf(-z) : exp2_quick(-1.44269504f * z)), 0x1p125f));
+}
 template <bool EXACT, int N>
 __device__ __forceinline__ void sigmoids(const float *z, float *s) {
-  const f32x2 one = pair_of(1.0f, 1.0f), log2e = pair_of(-1.44269504f, -1.44269504f);
+  // log2 e as the float next to it and what is left
+  constexpr float kHigh = (float)1.4426950408889634, kLow = (float)(1.4426950408889634 - (double)kHigh), kLn2 = 0.69314718f;
+  const f32x2 one = pair_of(1.0f, 1.0f), high = pair_of(-kHigh, -kHigh);
   float most = 0.f;
 #pragma unroll
   for (int i = 0; i + 1 < N; i += 2) {
-    const float2 x = halves(mul_pair(pair_of(z[i], z[i + 1]), log2e));
-    const float2 d = halves(add_pair(pair_of(exp2_quick(x.x), exp2_quick(x.y)), one));
+    const f32x2 v = pair_of(z[i], z[i + 1]), t = mul_pair(v, high);
+    const float2 x = halves(t);
+    f32x2 e = pair_of(exp2_quick(x.x), exp2_quick(x.y));
+    if (EXACT) {
+      // what the product has lost, and its low part: 2^(t + left) = 2^t (1 + left ln 2) for a left below 2^-16
+      const f32x2 left = fma_pair(v, pair_of(-kLow, -kLow), fma_pair(v, high, mul_pair(t, pair_of(-1.f, -1.f))));
+      e = fma_pair(mul_pair(e, left), pair_of(kLn2, kLn2), e);
+    }
+    const float2 d = halves(add_pair(e, one));
     const float p = d.x * d.y;
     most = max_or_nan(most, p);
     float r;
@@ -52,9 +64,9 @@ __device__ __forceinline__ void sigmoids(const float *z, float *s) {
   }
   if (N > 1 && !(most < 0x1p124f)) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) s[i] = z[i] < kNoSigmoid ? 0.f : one_sigmoid(z[i]);
+    for (int i = 0; i < N; ++i) s[i] = z[i] < kNoSigmoid ? 0.f : one_sigmoid<EXACT>(z[i]);
   }
-  if (N % 2 == 1) s[N - 1] = one_sigmoid(z[N - 1]);
+  if (N % 2 == 1) s[N - 1] = one_sigmoid<EXACT>(z[N - 1]);
 }
 // Values two at a time: half the instructions.  a * b, a * b + c; each argument is an array or one number for all.
 __device__ __forceinline__ f32x2 pair_at(const float *a, int i) { return pair_of(a[i], a[i + 1]); }

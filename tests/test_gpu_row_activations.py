@@ -79,3 +79,21 @@ def test_norm_with_a_channel_switched_off(cuda, dtype):
     want = group_norm(x, off, [(16, 0)], 4, activation=F.silu)[:, keep]
     step = 10 * 2.0 ** -24 + (0 if dtype == torch.float32 else torch.finfo(dtype).eps)
     assert bool(((y[:, keep].double() - want.double()).abs() <= step * want.double().abs()).all())
+
+
+@pytest.mark.parametrize("n", [1, 300])
+@pytest.mark.parametrize("act", [F.silu, torch.sigmoid], ids=["silu", "sigmoid"])
+def test_float32_sigmoids_to_a_few_steps(cuda, n, act):
+    """From -80 to 80 the exponential is off by two steps of 2^-23 at most; what it is multiplied with to take the exponent to base two,
+    the one, the shared product, its reciprocal and the two products behind it are rounded, half a step each: eleven halves, sixteen allowed; the
+    slope has two more operations, one of them a sum of terms of the same sign beyond |z| = 2."""
+    z = torch.linspace(-70, 80, 1023)
+    z = z[z.abs() > 2]
+    value, slope = one_by_one(z, act, n, cuda)
+    want, want_slope = definition(z, act)
+    most = ((value.double().cpu() - want).abs() / want.abs()).max().item()
+    assert most < 16 * 2.0 ** -24, most
+    # (1 - s of a positive argument is a difference: off by half a step of one)
+    amount = want_slope.abs() + (z > 0) * (1 + z.double().abs())
+    most = ((slope.double().cpu() / n - want_slope).abs() / amount).max().item()
+    assert most < (20 + n / 8) * 2.0 ** -24, most
