@@ -597,7 +597,8 @@ int ssc_gate_bwd(const float *x, const float *gy, int n, int c_total, int c_out,
  * field_first [n_field], field_len [n_field], field_scalar [n_field], gate_field [n_gate], group_first [n_group], group_len [n_group],
  * group_copies [n_group].  weight [n_field] and bias [n_scalar] float32 or NULL.  Activations: 0 identity, 1 relu, 2 sigmoid,
  * 3 silu, 4 gelu (erf).  out_type is `type`, or any for float32 rows.  stats [batch, n_group, 2] float32 receives mean (0 for l > 0) and
- * (variance + eps)^-1/2 of every sample that has rows, which the backward call reads.  Sums are float32, in a fixed order.
+ * (variance + eps)^-1/2 of every sample that has rows, which the backward call reads.  Sums are float32, in a fixed order; the squares
+ * about the mean, added up over a group, have to be within float32's range.
  * c is at most 2048 channels, with at most 512 gates, n at most 2^30.  Rows and scratch
  * start at multiples of 16 bytes.  scratch: ssc_group_norm_scratch_bytes(...) (forward: n_field = n_scalar = 0 will do).  status: as in
  * ssc_conv_fwd.  gx has the type of x; d_weight [n_field], d_bias [n_scalar] float32. */

@@ -229,9 +229,10 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_stats_kernel(GnArgs a) {
   for (int q = 0; q < VEC; ++q) centred[q] = works && q < many && a.t.scalar_of_channel[ch + q] >= 0 ? 1.f : 0.f, quarter[q] = 0.25f * centred[q];
   // (what the ends of pieces look up first comes with the first rows)
   const int lane = t & 31, first_group = t >> 5;
-  const int my_first = t < a.c ? a.t.group_first[a.t.group_of_channel[t]] : 0;
-  int my_from = 0, my_len = 0, my_copies = 1;
-  if (first_group < a.n_group) my_from = a.t.group_first[first_group], my_len = a.t.group_len[first_group], my_copies = a.t.group_copies[first_group];
+  int my_from = 0, my_len = 0, shift = 0;
+  while (shift < 5 && a.c << (shift + 1) <= a.threads) ++shift;        // lanes to a channel at the end of a piece
+  const int part = t & ((1 << shift) - 1);
+  if (first_group < a.n_group) my_from = a.t.group_first[first_group], my_len = a.t.group_len[first_group];
   GnWalk walk;
   if (ring.r0 < ring.r1) walk.find(a, ring.r0);
   for (int row = ring.r0; row < ring.r1;) {
@@ -261,8 +262,8 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_stats_kernel(GnArgs a) {
           }
           multiply_add<VEC>(d, mean, -1.f, mb);
           multiply_add<VEC>(mean, d, f, mean);
-          multiply<VEC>(d, d, d);
-          multiply_add<VEC>(s, d, have * f, s);
+          multiply<VEC>(mb, d, have * f);
+          multiply_add<VEC>(s, mb, d, s);
           multiply_add<VEC>(sq, sq, 1.f, s);
           have += 4.f;
         }
@@ -274,7 +275,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_stats_kernel(GnArgs a) {
           for (int q = 0; q < VEC; ++q) {
             const float mb = v[q] * centred[q], d = mb - mean[q], e = v[q] - mb;
             mean[q] = fmaf(d, f, mean[q]);
-            sq[q] += fmaf(d * d, have * f, e * e);
+            sq[q] += fmaf(have * f * d, d, e * e);
           }
           have += 1.f;
         }
@@ -294,29 +295,48 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_stats_kernel(GnArgs a) {
       __shared__ float count[kGnThreads];
       if (works && ch == 0) count[ty] = have;
       __syncthreads();
-      // (about the first mean of the group from here on: near enough to all of them)
-      for (int i = t; i < a.c; i += a.threads) {
-        const float about = sm[i == t ? my_first : a.t.group_first[a.t.group_of_channel[i]]];
-        float u = 0.f, v = 0.f;
-        for (int r = 0; r < R; ++r) {
-          const float d = sm[r * a.c + i] - about, nd = count[r] * d;
-          u += nd;
-          v += fmaf(nd, d, sq_s[r * a.c + i]);
+      // the mean of what is put together first, then the squares about it: about a channel, a row or a piece that lies far from the
+      // others (a thousand spreads) they would be as many times the variance, 1e-5 of which is lost; and the mean once more, which is
+      // off by a rounding of such a one.  (3501 rows of 38 channels in 290 pieces 5.9 us for the pass, 5.7 in one go about a first mean; 786432 rows of
+      // 128 in bf16 52.9 and 50.4.)
+      const float rows = (float)(end - begin);
+      for (int i0 = 0; i0 < a.c; i0 += a.threads >> shift) {
+        const int i = i0 + (t >> shift), at = i < a.c ? i : 0;
+        const float about = sm[at];
+        float u = 0.f, v = 0.f, left = 0.f;
+#pragma unroll 2
+        for (int r = part; r < R; r += 1 << shift) u = fmaf(count[r], sm[r * a.c + at] - about, u);
+        for (int d = 1 << shift >> 1; d > 0; d >>= 1) u += __shfl_xor_sync(0xffffffffu, u, d);
+        const float mean = about + __fdividef(u, rows);
+#pragma unroll 2
+        for (int r = part; r < R; r += 1 << shift) {
+          const float d = sm[r * a.c + at] - mean, nd = count[r] * d;
+          left += nd;
+          v += fmaf(nd, d, sq_s[r * a.c + at]);
         }
-        sums[i] = u;
-        sums[a.c + i] = v;
+        for (int d = 1 << shift >> 1; d > 0; d >>= 1) left += __shfl_xor_sync(0xffffffffu, left, d), v += __shfl_xor_sync(0xffffffffu, v, d);
+        if (part == 0 && i < a.c) {
+          sums[i] = mean + __fdividef(left, rows);
+          sums[a.c + i] = v;
+        }
       }
       __syncthreads();
       for (int g = first_group; g < a.n_group; g += a.threads >> 5) {
         const bool mine = g == first_group;
-        const int from = mine ? my_from : a.t.group_first[g], len = mine ? my_len : a.t.group_len[g], copies = mine ? my_copies : a.t.group_copies[g];
+        const int from = mine ? my_from : a.t.group_first[g], len = mine ? my_len : a.t.group_len[g];
+        const float about = sums[from];
         float u = 0.f, v = 0.f;
-        for (int i = lane; i < len; i += 32) u += sums[from + i], v += sums[a.c + from + i];
-        for (int d = 16; d > 0; d >>= 1) u += __shfl_xor_sync(0xffffffffu, u, d), v += __shfl_xor_sync(0xffffffffu, v, d);
-        if (lane == 0) {
-          const float n = (float)(end - begin) * (float)copies, mean = u / n;
-          *(float2 *)(a.partial + ((size_t)(blockIdx.x + walk.s) * a.n_group + g) * 2) = {sm[from] + mean, fmaxf(v - u * mean, 0.f)};
+        for (int i = lane; i < len; i += 32) u += sums[from + i] - about;
+        for (int d = 16; d > 0; d >>= 1) u += __shfl_xor_sync(0xffffffffu, u, d);
+        const float mean = about + __fdividef(u, (float)len);
+        float left = 0.f;
+        for (int i = lane; i < len; i += 32) {
+          const float d = sums[from + i] - mean;
+          left += d;
+          v += fmaf(rows * d, d, sums[a.c + from + i]);
         }
+        for (int d = 16; d > 0; d >>= 1) left += __shfl_xor_sync(0xffffffffu, left, d), v += __shfl_xor_sync(0xffffffffu, v, d);
+        if (lane == 0) *(float2 *)(a.partial + ((size_t)(blockIdx.x + walk.s) * a.n_group + g) * 2) = {mean + __fdividef(left, (float)len), v};
       }
       __syncthreads();
     }
@@ -335,51 +355,67 @@ __device__ __forceinline__ int piece_rows(const GnArgs &a, const GnWalk &k, int 
   return min(lo + a.range, k.hi) - max(lo, k.lo);
 }
 
-// The sums (u, v) of each group over the partial results of a sample: add(group, piece, the first result, this one, u, v), end(group, u, v).
+// What pieces of a sample are put together from: sums, or rows with their mean and the squares about it (Chan et al. 1979).
+struct GnSums {
+  float u, v;
+  __device__ __forceinline__ void add(const GnSums &o) { u += o.u, v += o.v; }
+  __device__ __forceinline__ GnSums across(int d) const { return {__shfl_xor_sync(0xffffffffu, u, d), __shfl_xor_sync(0xffffffffu, v, d)}; }
+};
+struct GnMoments {
+  float rows, mean, sq;
+  __device__ __forceinline__ void add(const GnMoments &o) {
+    const float both = rows + o.rows, share = both > 0.f ? __fdividef(o.rows, both) : 0.f, d = o.mean - mean;
+    sq += fmaf(rows * share * d, d, o.sq);       // (nothing times any d is nothing: d * d may be beyond the range)
+    mean = fmaf(d, share, mean);
+    rows = both;
+  }
+  __device__ __forceinline__ GnMoments across(int d) const {
+    return {__shfl_xor_sync(0xffffffffu, rows, d), __shfl_xor_sync(0xffffffffu, mean, d), __shfl_xor_sync(0xffffffffu, sq, d)};
+  }
+};
+// V of each group over the partial results of a sample: load(group, piece, its result), end(group, V).
 // Few pieces: up to eight lanes to a group.  Many, as in a sample that all blocks share: lanes side by side read neighbouring groups, each warp
 // its share of the pieces.  (Two samples of 1750 rows in 290 pieces, 32 groups: a group to a warp, which fetches a sector for each of
 // its results, 16.3 us for the second pass forward, this way 11.5; one sample of 203437 rows, 8 groups 17.9 and 16.8.)
 constexpr int kGnPieces = 4;               // in flight
-template <class Add, class End>
-__device__ __forceinline__ void sample_sums(const GnArgs &a, const float *from, int many, Add add, End end) {
+template <class V, class Load, class End>
+__device__ __forceinline__ void sample_sums(const GnArgs &a, const float *from, int many, Load load, End end) {
   const float2 *all = (const float2 *)from;
   const int lane = threadIdx.x & 31;
   if (many <= 8) {
     const int width = many <= 4 ? 4 : 8, at = lane & (width - 1);
     for (int g0 = 0; g0 < a.n_group; g0 += a.threads / width) {
       const int g = g0 + threadIdx.x / width;
-      float u = 0.f, v = 0.f;
-      if (g < a.n_group && at < many) add(g, at, all[g], all[(size_t)at * a.n_group + g], u, v);
-      for (int d = width / 2; d > 0; d >>= 1) u += __shfl_xor_sync(0xffffffffu, u, d), v += __shfl_xor_sync(0xffffffffu, v, d);
-      if (at == 0 && g < a.n_group) end(g, u, v);
+      V v = {};
+      if (g < a.n_group && at < many) v = load(g, at, all[(size_t)at * a.n_group + g]);
+      for (int d = width / 2; d > 0; d >>= 1) v.add(v.across(d));
+      if (at == 0 && g < a.n_group) end(g, v);
     }
     return;
   }
-  __shared__ float2 parts[kGnThreads / 32][32];
+  __shared__ V parts[kGnThreads / 32][32];
   const int warp = threadIdx.x >> 5, warps = a.threads >> 5;
   int wide = 1;
   while (wide < a.n_group && wide < 32) wide *= 2;
   const int step = warps * (32 / wide);
   for (int g0 = 0; g0 < a.n_group; g0 += wide) {
     const int g = g0 + (lane & (wide - 1));
-    float u = 0.f, v = 0.f;
-    if (g < a.n_group) {
-      const float2 about = all[g];
+    V v = {};
+    if (g < a.n_group)
       for (int i0 = warp * (32 / wide) + lane / wide; i0 < many; i0 += kGnPieces * step) {
         float2 p[kGnPieces];
 #pragma unroll
         for (int k = 0; k < kGnPieces; ++k) p[k] = all[(size_t)min(i0 + k * step, many - 1) * a.n_group + g];
 #pragma unroll
         for (int k = 0; k < kGnPieces; ++k)
-          if (i0 + k * step < many) add(g, i0 + k * step, about, p[k], u, v);
+          if (i0 + k * step < many) v.add(load(g, i0 + k * step, p[k]));
       }
-    }
-    for (int d = wide; d < 32; d *= 2) u += __shfl_xor_sync(0xffffffffu, u, d), v += __shfl_xor_sync(0xffffffffu, v, d);
-    if (lane < wide) parts[warp][lane] = {u, v};
+    for (int d = wide; d < 32; d *= 2) v.add(v.across(d));
+    if (lane < wide) parts[warp][lane] = v;
     __syncthreads();
     if ((int)threadIdx.x < wide && g < a.n_group) {
-      for (int w = 1; w < warps; ++w) u += parts[w][lane].x, v += parts[w][lane].y;
-      end(g, u, v);
+      for (int w = 1; w < warps; ++w) v.add(parts[w][lane]);
+      end(g, v);
     }
     if (g0 + wide < a.n_group) __syncthreads();
   }
@@ -390,16 +426,11 @@ __device__ __forceinline__ void sample_stats(const GnArgs &a, const GnWalk &k, f
   int first, many;
   sample_pieces(a, k, first, many);
   const float rows = (float)(k.hi - k.lo);
-  sample_sums(
+  sample_sums<GnMoments>(
       a, a.partial + (size_t)(first + k.s) * a.n_group * 2, many,
-      [&](int g, int i, float2 about, float2 p, float &u, float &v) {
-        const float d = p.x - about.x, nd = (float)piece_rows(a, k, first + i) * d;
-        u += nd;
-        v += fmaf(nd, d, __fdividef(p.y, (float)a.t.group_copies[g]));
-      },
-      [&](int g, float u, float v) {
-        const float mean = u / rows;
-        const float2 r = {a.partial[((size_t)(first + k.s) * a.n_group + g) * 2] + mean, 1.0f / sqrtf(fmaxf(v - u * mean, 0.f) / rows + a.eps)};
+      [&](int g, int i, float2 p) { return GnMoments{(float)piece_rows(a, k, first + i), p.x, __fdividef(p.y, (float)a.t.group_copies[g])}; },
+      [&](int g, const GnMoments &m) {
+        const float2 r = {m.mean, 1.0f / sqrtf(m.sq / rows + a.eps)};
         *(float2 *)(gs + 2 * g) = r;
         if (first == (int)blockIdx.x) *(float2 *)(a.stats + ((size_t)k.s * a.n_group + g) * 2) = r;
       });
@@ -610,16 +641,12 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_bwd_kernel(GnArgs a, int sum
         int first, many;
         sample_pieces(a, walk, first, many);
         const float rows = (float)(walk.hi - walk.lo);
-        sample_sums(
-            a, a.partial + (size_t)(first + walk.s) * a.n_group * 2, many,
-            [&](int, int, float2, float2 p, float &u, float &v) {
-              u += p.x;
-              v += p.y;
-            },
-            [&](int g, float u, float v) {
+        sample_sums<GnSums>(
+            a, a.partial + (size_t)(first + walk.s) * a.n_group * 2, many, [&](int, int, float2 p) { return GnSums{p.x, p.y}; },
+            [&](int g, const GnSums &sum) {
               const float m = 1.0f / (rows * (float)a.t.group_copies[g]);
-              gs[2 * g] = u * m;
-              gs[2 * g + 1] = v * m;
+              gs[2 * g] = sum.u * m;
+              gs[2 * g + 1] = sum.v * m;
             });
         __syncthreads();
 #pragma unroll

@@ -1,0 +1,42 @@
+"""The 64-bit forms that the GPU tests of the row operators go by: the same numbers as torch's own derivatives, and rooms that a result of
+zeros does not fit in."""
+import numpy as np
+import pytest
+import torch
+import torch.nn.functional as F
+
+import row_references as R
+from test_gpu_groupnorm import CASES, GATE, reference
+from test_gpu_row_precision import NORM_CASES, norm_inputs, norm_room
+
+SMALL = [i for i, c in enumerate(CASES) if sum(c[0]) <= 3000]
+
+
+@pytest.mark.parametrize("case", SMALL)
+def test_norm_by_formulas_and_by_torch(case):
+    lengths, Rs, groups, act = CASES[case]
+    x, w, b, gy, offsets = norm_inputs(lengths, Rs, act, torch.float32, 300 + case)
+    found = R.group_norm(x.double(), offsets, Rs, groups, w.double(), b.double(), 1e-3, act, gy.double())
+    leaves = [t.double().requires_grad_(True) for t in (x, w, b)]
+    y = reference(leaves[0], offsets, Rs, groups, leaves[1], leaves[2], 1e-3, act)
+    grads = torch.autograd.grad(y, leaves, found["gy"])
+    for name, a in zip(("y", "x", "weight", "bias"), (y.detach(), *grads)):
+        assert ((found[name][0] - a).abs() <= 2.0 ** -44 * (found[name][1] + 1)).all(), name
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("case", [i for i, c in enumerate(NORM_CASES) if sum(c[0]) <= 60000])
+def test_rooms_reject_zeros(case, dtype):
+    """Whatever is not all rounding (the gradient of a sample of one row is none): the room is a small part of the result."""
+    lengths, Rs, groups, act = NORM_CASES[case]
+    x, w, b, gy, offsets = norm_inputs(lengths, Rs, act, dtype, 300 + case)
+    found = R.group_norm(x.double(), offsets, Rs, groups, w.double(), b.double(), 1e-3, act, gy.double())
+    for name in ("y", "x", "weight", "bias"):
+        if name in ("x", "weight") and max(lengths) == 1:
+            continue
+        want, room = found[name][0], norm_room(found[name], torch.float32 if name in ("weight", "bias") else dtype)
+        if name == "x":
+            some = torch.cat([torch.full((n,), n > 1) for n in lengths])
+            want, room = want[some], room[some]
+        if want.numel():
+            assert room.norm() < 0.03 * want.norm(), (name, (room.norm() / want.norm()).item())
