@@ -106,3 +106,40 @@ def group_norm(x, offsets, Rs, groups, w, b, eps, act, gy):
             found[k] = (value, squares.sqrt())
     return found
 
+
+
+def feedforward(t, act, gy):
+    """The gated feed-forward block and its gradients: name -> (value, size, rounded, stages).  t: x, w_in, w_out, b_in, b_out, residual (the last
+    three may be None) in 64 bits.
+
+    What errors that go either way are measured by: size, of sums in float32, is the root of the sum of the squares of the terms, with those of
+    the sums that the terms come from; rounded is the root of the sum of the squares of the terms that 16-bit rows round on the way.  stages:
+    products one behind the other."""
+    x, (wg, wu), wo = t["x"], t["w_in"], t["w_out"]
+    g, u = x @ wg.t(), x @ wu.t()
+    if t["b_in"] is not None:
+        g, u = g + t["b_in"][0], u + t["b_in"][1]
+    a, slope = activation(act, g)
+    h = a * u
+    y = h @ wo.t()
+    if t["b_out"] is not None:
+        y = y + t["b_out"]
+    if t["residual"] is not None:
+        y = y + t["residual"]
+    dh = gy @ wo
+    dg, du = dh * u * slope, dh * a
+    sq = lambda *v: [k * k for k in v]  # noqa: E731
+    x2, wg2, wu2, wo2, gy2 = sq(x, wg, wu, wo, gy)
+    # an error of g or u, steps of the root of its sum, goes on into h, dg and du; so does one of dh
+    g2, u2, dh2 = x2 @ wg2.t() + g * g, x2 @ wu2.t() + u * u, gy2 @ wo2 + dh * dh
+    h2 = g2 * u2 + h * h
+    dg2, du2 = dh2 * u2 + dg * dg, dh2 * g2 + du * du
+    out = {"y": (y, h2 @ wo2.t(), (h * h) @ wo2.t(), 2),
+           "x": (dg @ wg + du @ wu, dg2 @ wg2 + du2 @ wu2, (dg * dg) @ wg2 + (du * du) @ wu2, 3),
+           "w_in": (torch.stack([dg.t() @ x, du.t() @ x]), torch.stack([dg2.t() @ x2, du2.t() @ x2]), torch.stack([(dg * dg).t() @ x2, (du * du).t() @ x2]), 3),
+           "w_out": (gy.t() @ h, gy2.t() @ h2, gy2.t() @ (h * h), 2),
+           "b_in": (torch.stack([dg.sum(0), du.sum(0)]), torch.stack([dg2.sum(0), du2.sum(0)]), torch.stack([(dg * dg).sum(0), (du * du).sum(0)]), 2),
+           "b_out": (gy.sum(0), gy2.sum(0), torch.zeros_like(gy.sum(0)), 1)}
+    out = {k: (v, (squares + v * v).sqrt(), rounded.sqrt(), stages) for k, (v, squares, rounded, stages) in out.items()}
+    out["kink"] = (g.abs() / g2.sqrt()).min()           # how near a gate comes to zero
+    return out

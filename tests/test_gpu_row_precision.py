@@ -6,7 +6,8 @@ import torch
 import torch.nn.functional as F
 
 import row_references as R
-from test_gpu_groupnorm import CASES, GATE
+from test_gpu_feedforward import SIZES, inputs
+from test_gpu_groupnorm import CASES
 
 pytestmark = pytest.mark.gpu
 NORM_CASES = CASES
@@ -74,3 +75,69 @@ def test_norm_with_values_far_from_the_rest(cuda, outlier, rows, c, groups, dtyp
     else:
         x = 1e20 + 1e15 * x
     check_norm(cuda, x.to(dtype), w, b, gy.to(dtype), [0, rows], [(c, 0)], groups, 1e-5, F.silu)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("case", range(len(NORM_CASES)))
+def test_norm_value_by_value(cuda, case, dtype):
+    """Every value of the result and of all gradients, at the sizes and layouts where they can go wrong."""
+    lengths, Rs, groups, act = NORM_CASES[case]
+    x, w, b, gy, offsets = norm_inputs(lengths, Rs, act, dtype, 300 + case)
+    check_norm(cuda, x, w, b, gy, offsets, Rs, groups, 1e-3, act)
+
+
+# Half steps of a product's float32 sums: inside tensor memory an addition of sixteen terms may cut off, a step of 2^-23, half of it on average, and
+# after sixteen of them the sum goes on in registers, where half a step is lost each time, either way: 16, and as much again for the planes' products that
+# are left out, the parts, and the activation.
+FF_STEPS = 32
+
+
+def ff_room(found, dtype, part):
+    """For the norm of the errors over a part of a result.  16 bits: half a step of the result, and of the terms rounded before.  Few values may
+    add up to twice what many do on average."""
+    value, size, rounded, stages = found
+    value, size, rounded = part(value), part(size), part(rounded)
+    room = stages * FF_STEPS * R.HALF * size.norm()
+    half = 0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
+    return half * value.norm() + (2 if value.numel() < 32 else 1) * (room + half * rounded.norm())
+
+
+def parts(t):
+    """The whole, its first and last columns and rows, eighths of the rows and of the columns."""
+    yield lambda v: v
+    for i in ((0, 1), (-1, None)):
+        yield lambda v, i=i: v[..., i[0]:i[1]]
+        if t.dim() > 1:
+            yield lambda v, i=i: v[..., i[0]:i[1], :]
+    for dim in (-1, -2)[:t.dim()]:
+        for k in range(8):
+            if t.shape[dim] >= 8:
+                yield lambda v, k=k, dim=dim: v.chunk(8, dim)[min(k, len(v.chunk(8, dim)) - 1)]
+
+
+def ff_inputs(size, dtype):
+    n, c, h, o, bias, residual, act = SIZES[size]
+    return inputs(n, c, h, o, dtype, bias, residual, 500 + size)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("size", range(len(SIZES)))
+def test_feedforward_part_by_part(cuda, size, dtype):
+    from ss_conv.feedforward import gated_feedforward
+    t, gy = ff_inputs(size, dtype)
+    act = SIZES[size][-1]
+    names = [k for k in t if t[k] is not None]
+    on = lambda v: None if v is None else v.to(cuda)  # noqa: E731
+    dev = {k: None if v is None else on(v).requires_grad_(True) for k, v in t.items()}
+    y = gated_feedforward(dev["x"], dev["w_in"], dev["w_out"], dev["b_in"], dev["b_out"], act, dev["residual"])
+    got = {"y": y.detach(), **dict(zip(names, torch.autograd.grad(y, [dev[k] for k in names], on(gy))))}
+    found = R.feedforward({k: None if v is None else on(v).double() for k, v in t.items()}, act, on(gy).double())
+    for name in got:
+        if name == "residual":
+            continue
+        want = found[name][0]
+        assert got[name].shape == want.shape
+        far = got[name].double() - want
+        for part in parts(want):
+            room = ff_room(found[name], dtype, part)
+            assert part(far).norm() <= room, (name, part(far).shape, (part(far).norm() / room).item(), (part(far).norm() / part(want).norm()).item())

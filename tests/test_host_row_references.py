@@ -1,13 +1,13 @@
 """The 64-bit forms that the GPU tests of the row operators go by: the same numbers as torch's own derivatives, and rooms that a result of
 zeros does not fit in."""
-import numpy as np
 import pytest
 import torch
-import torch.nn.functional as F
 
 import row_references as R
-from test_gpu_groupnorm import CASES, GATE, reference
-from test_gpu_row_precision import NORM_CASES, norm_inputs, norm_room
+from test_gpu_groupnorm import CASES, reference
+from test_gpu_feedforward import SIZES
+from test_gpu_feedforward import reference as ff_reference
+from test_gpu_row_precision import FF_STEPS, NORM_CASES, ff_inputs, ff_room, norm_inputs, norm_room, parts
 
 SMALL = [i for i, c in enumerate(CASES) if sum(c[0]) <= 3000]
 
@@ -40,3 +40,25 @@ def test_rooms_reject_zeros(case, dtype):
             want, room = want[some], room[some]
         if want.numel():
             assert room.norm() < 0.03 * want.norm(), (name, (room.norm() / want.norm()).item())
+
+
+SMALL_FF = [i for i, s in enumerate(SIZES) if s[0] * s[2] <= 1500000]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("size", SMALL_FF)
+def test_feedforward_by_formulas_and_its_rooms(size, dtype):
+    """The formulas' numbers are torch's; zeros do not fit in the rooms; no gate comes so near to ReLU's kink that its slope is open."""
+    t, gy = ff_inputs(size, dtype)
+    act = SIZES[size][-1]
+    t64 = {k: None if v is None else v.double().requires_grad_(True) for k, v in t.items()}
+    found = R.feedforward({k: None if v is None else v.detach() for k, v in t64.items()}, act, gy.double())
+    y = ff_reference(t64, act)
+    names = [k for k in t if t[k] is not None and k != "residual"]
+    for name, a in zip(["y"] + names, (y.detach(), *torch.autograd.grad(y, [t64[k] for k in names], gy.double()))):
+        value, size_of = found[name][:2]
+        assert ((value - a).abs() <= 2.0 ** -44 * (size_of + 1)).all(), name
+        for part in parts(value):
+            # (one value may be small by chance: what the others around it are)
+            assert ff_room(found[name], dtype, part) < 0.05 * max(part(value).norm(), part(size_of).norm() / 8), name
+    assert act is not torch.nn.functional.relu or found["kink"] > 4 * FF_STEPS * R.HALF
