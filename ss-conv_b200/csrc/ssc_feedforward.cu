@@ -1099,6 +1099,16 @@ EncodeFn encode_fn() {
   return fn;
 }
 
+// fn(args...) needs a current context, which a thread has from its first call of the runtime that takes one: a thread of autograd's whose memory comes
+// out of a store may get here before.
+template <class... A>
+CUresult encode(EncodeFn fn, A... args) {
+  CUresult r = fn(args...);
+  int device;
+  if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess) r = fn(args...);
+  return r;
+}
+
 // `planes` matrices [rows][cols] with rows of `pitch` elements, one behind the other.
 struct Matrix {
   const void *p;
@@ -1111,7 +1121,7 @@ int make_map(CUtensorMap *map, const Matrix &m, bool f16) {
   const cuuint64_t dims[3] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows, (cuuint64_t)m.planes};
   const cuuint64_t strides[2] = {(cuuint64_t)m.pitch * 2, (cuuint64_t)m.pitch * 2 * (cuuint64_t)m.rows};
   const cuuint32_t box[3] = {kBox, kBox, 1}, each[3] = {1, 1, 1};
-  const CUresult r = fn(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(m.p), dims, strides, box, each,
+  const CUresult r = encode(fn, map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(m.p), dims, strides, box, each,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(SSC_ERR_CUDA, "gated_ff: no tensor map for [%lld, %d] (error %d)", m.rows, m.cols, (int)r);
   return SSC_OK;
@@ -1126,7 +1136,7 @@ bool make_out_map(CUtensorMap *map, const void *p, long long rows, int cols, int
   const cuuint64_t strides[2] = {(cuuint64_t)pitch * size, (cuuint64_t)pitch * size * (cuuint64_t)rows};
   const cuuint32_t box[3] = {(cuuint32_t)width, 32, 1}, each[3] = {1, 1, 1};
   const CUtensorMapDataType kind = type == SSC_PREC_FP32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == SSC_PREC_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  return fn(map, kind, 3, const_cast<void *>(p), dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, width * size == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : width * size == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B,
+  return encode(fn, map, kind, 3, const_cast<void *>(p), dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, width * size == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : width * size == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B,
             CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
