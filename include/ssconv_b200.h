@@ -618,7 +618,7 @@ int ssc_group_norm_bwd(const void *x, const void *gy, int type, int n, int c, co
  * `type` (SSC_PREC_FP32 / F16 / BF16); the biases and the residual may be NULL.  act: 0 identity, 1 relu, 2 sigmoid, 3 silu,
  * 4 gelu (erf).  Products are added in float32; float32 operands are used to 24 bits; in 16 bits the hidden rows h = act(.) * (.), and
  * in the backward call their gradients, are rounded to the rows' type (not in a forward call of up to 256 rows that takes the form for few).  A value that is not
- * finite makes what depends on it infinite or NaN.  Widths are at most 65536, rows at most 2^30; any address and width is accepted, 16-bit widths that are
+ * finite makes what depends on it infinite or NaN; so may, in float32, one above 3.39e38 (the largest bfloat16), and below 2^-110 bits are lost.  Widths are at most 65536, rows at most 2^30; any address and width is accepted, 16-bit widths that are
  * multiples of 8 at addresses that are multiples of 16 are read in place, others are copied to scratch first.
  * scratch: ssc_gated_ff_scratch_bytes(...) bytes, 16-byte aligned; rows are taken in turns so that theirs is at most 2^30 bytes and
  * shares of split sums 2^27, beside what the weights take (their planes or padded rows, and in the backward call their gradients in

@@ -9,10 +9,13 @@
 // All of them are one kernel: pairs of CTAs with tiles of 256 rows in tensor memory, half of each operand in either CTA, operands by TMA, a warp
 // that issues the products and others that empty the accumulators, two of which are in turn.  Operands are 16-bit; float32 rows are the sum of
 // three bfloat16 planes (24 bits), and a product the sum of the six products of planes that reach 2^-24, the small ones first.
+// Of 16-bit rows h, dg and du are rounded to 16 bits as well, as the operands they become: a second plane of each would double the products behind it and
+// what leaves the SM, which bounds them already.  Errors are 0.0024 (bf16) and 2.9e-4 (fp16) of a result that way, where
+// the rounding of the result alone is 0.0017 and 2.1e-4.  Few rows on plain lanes keep h in float32.
 //
-// 65536 rows 256 -> 1024 -> 256 in bf16, forward 124 us, backward 309 (rates of a cool GPU; 1.2 GHz under its power limit: 500 for both): gate, up and h
-// 75 (917 TFLOP/s of its two products, bound by the way out: 134 MB of h through shared memory), the way out 49, h, dg and du 139 (403 MB), dx 68, the
-// gradients of Win and Wo 56 and 37, their sums 9.  float32, 16384 rows 128 -> 512 -> 128, 265 us for both: h, dg and du 65, nine planes whose splitting and stores
+// 65536 rows 256 -> 1024 -> 256 in bf16, forward 126 us, backward 311 (rates of a cool GPU; under its power limit 500 for both): gate, up and h
+// 77 (893 TFLOP/s of its two products, bound by the way out: 134 MB of h through shared memory), the way out 49, h, dg and du 140 (403 MB), dx 68, the
+// gradients of Win and Wo 56 and 37, their sums 10.  float32, 16384 rows 128 -> 512 -> 128, 268 us for both: h, dg and du 68, nine planes whose splitting and stores
 // bound it.  One row 256 -> 1024 -> 256 3.7 us, two launches and two latencies.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -1345,7 +1348,8 @@ int gate_product(Ff &f, const Matrix &x, const Matrix &w_in, const void *b_in, v
   return launch_gemm<kGate, T>(f, maps, p);
 }
 
-// h, dg and du: gate and up again, and dh = dy Wo; float32 sums of three products are more than the registers, there dh has been multiplied before.
+// h, dg and du: gate and up again, and dh = dy Wo.  float32 rows have dh multiplied before: sums that leave tensor memory in between (more than 256 terms)
+// are kept in registers, which those of three products exceed.  (Narrower rows could have all three in tensor memory; that form is not there.)
 template <class T>
 int back_product(Ff &f, const Matrix &x, const Matrix &w_in, const Matrix &gy, const Matrix &w_out, const void *b_in, const float *dh, void *h, void *dgu) {
   FfMaps maps = {};

@@ -11,8 +11,8 @@
 // tiles: with loads in the threads themselves, registers for the rows in flight left room for two blocks of
 // 256 threads, which waited for memory half of the time.
 //
-// 786432 rows of 128 in bf16: sums 52 us (3.9 TB/s), second pass 85 (4.7 TB/s read and written).  65536 rows of 256 in float32, all in L2: 22 and 23, backward 40 and
-// 40.  A launch on next to nothing takes 6 to 8 us (tables, offsets, the copies' first latency, sums at the end); from there on instructions bound it, 10 to 30 a value
+// 786432 rows of 128 in bf16: sums 53 us (3.8 TB/s), second pass 84 (4.8 TB/s read and written).  65536 rows of 256 in float32, all in L2: 22 and 23, backward 41 and
+// 42.  A launch on next to nothing takes 6 to 8 us (tables, offsets, the copies' first latency, sums at the end); from there on instructions bound it, 10 to 30 a value
 // at half of the issue slots: more warps, bigger tiles, and a second pass from the end (to find rows in L2) changed nothing or cost elsewhere.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -795,8 +795,9 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_bwd_kernel(GnArgs a, int sum
 
 int type_bytes(int type) { return type == SSC_PREC_FP32 ? 4 : 2; }
 
-// Channels to a thread: 16 bytes of them, four with their gradients (eight channels of two rows with gradients are more than a thread's
-// registers) and where rows are no multiple.
+// Channels to a thread: 16 bytes of them, four with their gradients (eight channels of two rows with gradients exceed a thread's 128 registers by 160 to 270
+// bytes) and where rows are no multiple.  Gradients of bf16 rows by eight instead of four, both passes: 393216 rows of 128 with silu 105 and 115 us instead of 92 and 102,
+// without an activation 65 and 93 instead of 71 and 82, 200000 of 128 + 24 with gates 157 and 135 instead of 86 and 93.
 struct GnVec {
   int vec;
   bool whole;
