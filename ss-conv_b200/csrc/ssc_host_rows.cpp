@@ -14,8 +14,11 @@
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <memory>
 #include <optional>
 #include <string>
+#include <unordered_set>
+#include <vector>
 
 #include "../../include/ssconv_b200.h"
 
@@ -68,25 +71,28 @@ bool recorded(std::initializer_list<const Tensor *> all) {
   return false;
 }
 // Recording into a CUDA graph: gradients of a leaf that an earlier result of the default stream still holds on to would be added up on that
-// stream, which cannot take part: the backward pass would end the process.  So the call is refused.  (Looked at as far as leaves, tensors converted
-// from them and results of the default stream.)
+// stream, which cannot take part: the backward pass would end the process.  So the call is refused, however far behind its arguments such a
+// leaf (or another part of a graph of the default stream) lies.
 void recordable(std::initializer_list<const Tensor *> all, const Tensor &x) {
-  const c10::DeviceIndex device = x.device().index();
-  const c10::Stream ordinary = c10::cuda::getDefaultCUDAStream(device);
-  if (c10::cuda::getCurrentCUDAStream(device).unwrap() == ordinary) return;
-  bool foreign = false;
-  auto look = [&](torch::autograd::Node *f) { foreign |= f != nullptr && f->stream() == ordinary; };
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  const c10::Stream ordinary = c10::cuda::getDefaultCUDAStream(x.device().index());
+  std::vector<torch::autograd::Node *> next;
+  std::unordered_set<torch::autograd::Node *> seen;
+  auto look = [&](torch::autograd::Node *f) {
+    if (f != nullptr && seen.insert(f).second) next.push_back(f);
+  };
+  std::vector<std::shared_ptr<torch::autograd::Node>> leaves;       // (a leaf has its node only as long as somebody holds it)
   for (const Tensor *t : all) {
     if (!t->defined() || !t->requires_grad()) continue;
-    if (t->is_leaf()) {
-      look(torch::autograd::impl::try_get_grad_accumulator(*t).get());
-    } else {
-      look(t->grad_fn().get());
-      for (const torch::autograd::Edge &e : t->grad_fn()->next_edges()) look(e.function.get());
-    }
+    leaves.push_back(t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t) : t->grad_fn());
+    look(leaves.back().get());
   }
-  TORCH_CHECK(!foreign || c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None,
-              "a result computed before this recording still holds the gradient graph of the same tensors: drop it (its loss) before recording");
+  while (!next.empty()) {
+    torch::autograd::Node *f = next.back();
+    next.pop_back();
+    TORCH_CHECK(!(f->stream() == ordinary), "a result computed before this recording still holds the gradient graph of the same tensors: drop it (its loss) before recording");
+    for (const torch::autograd::Edge &e : f->next_edges()) look(e.function.get());
+  }
 }
 // A tangent would be dropped without a word: the operators have no forward-mode derivative.
 void no_tangents(const char *what, std::initializer_list<const Tensor *> all) {

@@ -91,3 +91,38 @@ def test_tangents_are_refused(cuda):
                     with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
                         call(**{**args, name: dual})
                 call(**args)
+
+
+@pytest.mark.parametrize("between", ["two operations", "a layer"])
+def test_recordings_look_for_earlier_graphs_behind_the_arguments(cuda, between):
+    """The leaf that an eager result still holds lies several operations behind the operator's arguments: refused as well (its backward pass
+    could not be recorded); with the result gone it is recorded and replays."""
+    from ss_conv.feedforward import gated_feedforward
+    from ss_conv.groupnorm import group_norm
+    g = torch.Generator("cuda").manual_seed(6)
+    r = lambda *s: torch.randn(*s, generator=g, device=cuda)  # noqa: E731
+    x, gy, off = r(500, 32), r(500, 32).bfloat16(), offsets(cuda, 200, 500)
+    w, scale = (r(2, 48, 32) / 6).requires_grad_(True), r(32).requires_grad_(True)
+    w_out = (r(32, 48) / 7).bfloat16()
+    if between == "two operations":
+        mine = [w]
+        step = lambda: gated_feedforward(x.bfloat16(), (w * 2).exp().to(torch.bfloat16) / 8, w_out)  # noqa: E731
+    else:
+        mine = [scale]
+        step = lambda: group_norm(torch.relu(x * scale).bfloat16() * 3, off, [(32, 0)], 8)  # noqa: E731
+    want = torch.autograd.grad(step(), mine, gy)
+    alive = step()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        torch.zeros(8, device=cuda)
+        with pytest.raises(RuntimeError, match="before this recording"):
+            step()
+    del alive, graph
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = torch.autograd.grad(step(), mine, gy)
+    for t in got:
+        t.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
