@@ -1448,7 +1448,7 @@ size_t row_split_bytes(const Ff &f, long long rows, int blocks, int cols) {
   return s > 1 ? align_up((size_t)s * rows * cols * sizeof(float), 256) : 0;
 }
 
-// Rows of one go, so that what lies between the products (planes or rows of h, dg, du, x and dy, dh of float32) is at most a gigabyte: 487 rows
+// Rows of one go, so that what lies between the products (planes or rows of h, dg, du, x and dy, dh of float32) is at most a gigabyte: 481 rows
 // of the widest there are, a tile or more.
 long long rows_at_once(const Ff &f, bool backward) {
   const long long hidden = 2 * planes_for(f.type) * (backward ? 3 : 1) + (backward && f.type == SSC_PREC_FP32 ? 4 : 0);
